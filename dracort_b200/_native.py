@@ -73,11 +73,19 @@ EXPORTED_SYMBOLS = (
     "draco_ipc_close",
     "draco_gguf_gemv_grouped_tp",
     "draco_tp_finish",
+    "draco_kv_cache_bytes",
+    "draco_kv_append",
+    "draco_kv_read",
+    "draco_attention_paged",
+    "draco_attention_paged_workspace_bytes",
+    "draco_verify_drafts",
 )
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 GEMM_MAX_PROBLEMS = 16
+KV_BF16 = 1
+KV_Q8_0 = 8
 
 
 class GemvProblem(ctypes.Structure):
@@ -141,6 +149,90 @@ class TpExchange(ctypes.Structure):
         ("counter_off", ctypes.c_int64),
         ("y_off", ctypes.c_int64 * 8),
         ("parity_stride", ctypes.c_int64 * 8),
+    ]
+
+
+class KvCache(ctypes.Structure):
+    """Mirror of ``draco_kv_cache``."""
+
+    _fields_ = [
+        ("type", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("page_size", ctypes.c_int),
+        ("n_pages", ctypes.c_int),
+        ("n_seqs", ctypes.c_int),
+        ("max_pages", ctypes.c_int),
+        ("table_stride", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+    ]
+
+
+class KvAppendArgs(ctypes.Structure):
+    """Mirror of ``draco_kv_append_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("ldq", ctypes.c_int64),
+        ("ldk", ctypes.c_int64),
+        ("ldv", ctypes.c_int64),
+        ("ldqo", ctypes.c_int64),
+        ("cos_table", ctypes.c_void_p),
+        ("sin_table", ctypes.c_void_p),
+        ("max_positions", ctypes.c_int64),
+        ("seq", ctypes.c_void_p),
+        ("pos", ctypes.c_void_p),
+        ("n", ctypes.c_int),
+        ("heads", ctypes.c_int),
+    ]
+
+
+class AttentionPagedArgs(ctypes.Structure):
+    """Mirror of ``draco_attention_paged_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("ldq", ctypes.c_int64),
+        ("ldo", ctypes.c_int64),
+        ("q_start", ctypes.c_void_p),
+        ("kv_len", ctypes.c_void_p),
+        ("n", ctypes.c_int),
+        ("heads", ctypes.c_int),
+        ("max_q", ctypes.c_int),
+        ("max_kv", ctypes.c_int),
+        ("scale", ctypes.c_float),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class VerifyArgs(ctypes.Structure):
+    """Mirror of ``draco_verify_args``."""
+
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("draft_probs", ctypes.c_void_p),
+        ("row_start", ctypes.c_void_p),
+        ("drafts", ctypes.c_void_p),
+        ("accept_u", ctypes.c_void_p),
+        ("sample_u", ctypes.c_void_p),
+        ("accepted", ctypes.c_void_p),
+        ("tokens", ctypes.c_void_p),
+        ("ld_logits", ctypes.c_int64),
+        ("ld_probs", ctypes.c_int64),
+        ("ld_tokens", ctypes.c_int64),
+        ("temperature", ctypes.c_float),
+        ("dtype", ctypes.c_int),
+        ("n", ctypes.c_int),
+        ("n_seqs", ctypes.c_int),
+        ("vocab", ctypes.c_int),
+        ("max_rows", ctypes.c_int),
     ]
 
 
@@ -235,6 +327,18 @@ def load() -> ctypes.CDLL:
         lib.draco_tp_finish.restype = c_int
         lib.draco_tp_finish.argtypes = [ctypes.POINTER(TpExchange), c_int, i64, i64, c_int, vp, i64, i64, c_int,
                                         vp, vp, vp]
+        lib.draco_kv_cache_bytes.restype = i64
+        lib.draco_kv_cache_bytes.argtypes = [c_int] * 5
+        lib.draco_kv_append.restype = c_int
+        lib.draco_kv_append.argtypes = [ctypes.POINTER(KvCache), ctypes.POINTER(KvAppendArgs), c_int, vp]
+        lib.draco_kv_read.restype = c_int
+        lib.draco_kv_read.argtypes = [ctypes.POINTER(KvCache), vp, vp, c_int, vp, vp, i64, i64, c_int, vp]
+        lib.draco_attention_paged.restype = c_int
+        lib.draco_attention_paged.argtypes = [ctypes.POINTER(KvCache), ctypes.POINTER(AttentionPagedArgs), c_int, vp]
+        lib.draco_attention_paged_workspace_bytes.restype = ctypes.c_size_t
+        lib.draco_attention_paged_workspace_bytes.argtypes = [ctypes.POINTER(KvCache)] + [c_int] * 5
+        lib.draco_verify_drafts.restype = c_int
+        lib.draco_verify_drafts.argtypes = [ctypes.POINTER(VerifyArgs), vp]
         lib.draco_gguf_gemv.restype = c_int
         lib.draco_gguf_gemv.argtypes = [c_int, vp, vp, vp, vp, c_int, i64, i64, vp, ctypes.c_size_t, vp]
         _lib = lib

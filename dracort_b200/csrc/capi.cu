@@ -6,6 +6,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "paged_attn.cuh"
 
 namespace draco {
 
@@ -442,4 +443,200 @@ int draco_swiglu_f32(const float* gate, const float* up, float* out, int64_t n, 
     return fail(DRACO_ERR_ALIGN, "swiglu_f32: gate, up and out must be 16-byte aligned");
   cudaError_t e = draco::launch_swiglu_f32(gate, up, out, n, (cudaStream_t)stream);
   return e == cudaSuccess ? ok() : cuda_fail(e, "swiglu_f32");
+}
+
+// ---------------------------------------------------------------------------
+// serving over a paged key/value cache
+// ---------------------------------------------------------------------------
+namespace draco {
+
+static bool kv_shape_ok(int type, int n_pages, int kv_heads, int page_size, int hd) {
+  return (type == DRACO_KV_BF16 || type == DRACO_KV_Q8_0) && n_pages >= 1 && kv_heads >= 1 && kv_heads <= 1024 &&
+         page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0 &&
+         (hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 256);
+}
+
+static int check_kv_cache(const draco_kv_cache* c, const char* fn, PagedView* view) {
+  if (!c) return fail(DRACO_ERR_ARG, "%s: null cache", fn);
+  if (c->type != DRACO_KV_BF16 && c->type != DRACO_KV_Q8_0)
+    return fail(DRACO_ERR_TYPE, "%s: cache type %d (supported: DRACO_KV_BF16, DRACO_KV_Q8_0)", fn, c->type);
+  if (!kv_shape_ok(c->type, c->n_pages, c->kv_heads, c->page_size, c->head_dim))
+    return fail(DRACO_ERR_SHAPE,
+                "%s: %d pages of %d positions, %d key/value heads of %d (pages: a power of two from 16 to 1024; "
+                "head_dim 32, 64, 96, 128 or 256; at most 1024 heads)",
+                fn, c->n_pages, c->page_size, c->kv_heads, c->head_dim);
+  if (c->n_seqs < 0 || c->max_pages < 1 || c->table_stride < 0 ||
+      (int64_t)c->max_pages * c->page_size > 0x7FFFFFFF)
+    return fail(DRACO_ERR_SHAPE, "%s: block table of %d sequences, %d pages each, stride %lld", fn, c->n_seqs,
+                c->max_pages, (long long)c->table_stride);
+  if (!c->k || !c->v || (c->n_seqs > 0 && !c->block_table)) return fail(DRACO_ERR_ARG, "%s: null cache pointer", fn);
+  if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15)
+    return fail(DRACO_ERR_ALIGN, "%s: cache buffers must be 16-byte aligned", fn);
+  if (reinterpret_cast<uintptr_t>(c->block_table) & 3)
+    return fail(DRACO_ERR_ALIGN, "%s: block_table not 4-byte aligned", fn);
+  view->k = static_cast<uint8_t*>(c->k);
+  view->v = static_cast<uint8_t*>(c->v);
+  view->table = c->block_table;
+  view->table_stride = c->table_stride;
+  view->block_bytes = paged_block_bytes(c->type, c->page_size, c->head_dim);
+  view->n_seqs = c->n_seqs;
+  view->max_pages = c->max_pages;
+  view->n_pages = c->n_pages;
+  view->kv_heads = c->kv_heads;
+  view->page_shift = __builtin_ctz((unsigned)c->page_size);
+  view->type = c->type;
+  return DRACO_OK;
+}
+
+static int check_dtype(int dtype, const char* fn) {
+  if (dtype != DRACO_DTYPE_F32 && dtype != DRACO_DTYPE_BF16) return fail(DRACO_ERR_TYPE, "%s: dtype %d", fn, dtype);
+  return DRACO_OK;
+}
+
+// rows of `width` elements at 16-byte boundaries
+static int check_rows(const void* p, int64_t ld, int64_t width, int dtype, const char* fn, const char* name) {
+  const int per = dtype == DRACO_DTYPE_F32 ? 4 : 8;
+  if (ld < width) return fail(DRACO_ERR_SHAPE, "%s: %s has token stride %lld for rows of %lld", fn, name, (long long)ld,
+                              (long long)width);
+  if ((reinterpret_cast<uintptr_t>(p) & 15) || ld % per)
+    return fail(DRACO_ERR_ALIGN, "%s: rows of %s must start on 16-byte boundaries", fn, name);
+  return DRACO_OK;
+}
+
+}  // namespace draco
+
+int64_t draco_kv_cache_bytes(int type, int n_pages, int kv_heads, int page_size, int head_dim) {
+  if (!kv_shape_ok(type, n_pages, kv_heads, page_size, head_dim)) return -1;
+  return (int64_t)n_pages * kv_heads * paged_block_bytes(type, page_size, head_dim);
+}
+
+int draco_kv_append(const draco_kv_cache* cache, const draco_kv_append_args* args, int dtype, void* stream) {
+  const char* fn = "kv_append";
+  PagedView c;
+  int rc = check_kv_cache(cache, fn, &c);
+  if (rc || (rc = check_dtype(dtype, fn))) return rc;
+  if (!args) return fail(DRACO_ERR_ARG, "%s: null arguments", fn);
+  draco_kv_append_args a = *args;
+  if (a.n < 0 || a.heads < 0) return fail(DRACO_ERR_SHAPE, "%s: %d tokens, %d heads", fn, a.n, a.heads);
+  if ((a.q == nullptr) != (a.q_out == nullptr)) return fail(DRACO_ERR_ARG, "%s: q and q_out come together", fn);
+  if ((a.cos_table == nullptr) != (a.sin_table == nullptr))
+    return fail(DRACO_ERR_ARG, "%s: cos and sin tables come together", fn);
+  if (a.n == 0) return ok();
+  if (!a.k || !a.v || !a.seq || !a.pos) return fail(DRACO_ERR_ARG, "%s: null pointer", fn);
+  if (a.q == nullptr) a.heads = 0;
+  if (a.heads > 65536) return fail(DRACO_ERR_SHAPE, "%s: %d heads", fn, a.heads);
+  const int64_t hd = cache->head_dim, kw = (int64_t)c.kv_heads * hd, qw = (int64_t)a.heads * hd;
+  if (a.heads > 0 && ((rc = check_rows(a.q, a.ldq, qw, dtype, fn, "q")) ||
+                      (rc = check_rows(a.q_out, a.ldqo, qw, dtype, fn, "q_out"))))
+    return rc;
+  if ((rc = check_rows(a.k, a.ldk, kw, dtype, fn, "k")) || (rc = check_rows(a.v, a.ldv, kw, dtype, fn, "v"))) return rc;
+  if (a.cos_table) {
+    if (a.max_positions < 1) return fail(DRACO_ERR_SHAPE, "%s: tables of no position", fn);
+    if ((reinterpret_cast<uintptr_t>(a.cos_table) | reinterpret_cast<uintptr_t>(a.sin_table)) & 15)
+      return fail(DRACO_ERR_ALIGN, "%s: cos and sin tables must be 16-byte aligned", fn);
+  }
+  if ((reinterpret_cast<uintptr_t>(a.seq) | reinterpret_cast<uintptr_t>(a.pos)) & 3)
+    return fail(DRACO_ERR_ALIGN, "%s: seq and pos not 4-byte aligned", fn);
+  const cudaError_t e = launch_kv_append(c, cache->head_dim, dtype, a, (cudaStream_t)stream);
+  return e == cudaSuccess ? ok() : cuda_fail(e, fn);
+}
+
+int draco_kv_read(const draco_kv_cache* cache, const int* seq, const int* pos, int n, void* k_out, void* v_out,
+                  int64_t ldk, int64_t ldv, int dtype, void* stream) {
+  const char* fn = "kv_read";
+  PagedView c;
+  int rc = check_kv_cache(cache, fn, &c);
+  if (rc || (rc = check_dtype(dtype, fn))) return rc;
+  if (n < 0) return fail(DRACO_ERR_SHAPE, "%s: %d rows", fn, n);
+  if (n == 0) return ok();
+  if (!seq || !pos || !k_out || !v_out) return fail(DRACO_ERR_ARG, "%s: null pointer", fn);
+  const int64_t kw = (int64_t)c.kv_heads * cache->head_dim;
+  if ((rc = check_rows(k_out, ldk, kw, dtype, fn, "k_out")) || (rc = check_rows(v_out, ldv, kw, dtype, fn, "v_out")))
+    return rc;
+  if ((reinterpret_cast<uintptr_t>(seq) | reinterpret_cast<uintptr_t>(pos)) & 3)
+    return fail(DRACO_ERR_ALIGN, "%s: seq and pos not 4-byte aligned", fn);
+  const cudaError_t e = launch_kv_read(c, cache->head_dim, dtype, seq, pos, n, k_out, v_out, ldk, ldv,
+                                       (cudaStream_t)stream);
+  return e == cudaSuccess ? ok() : cuda_fail(e, fn);
+}
+
+int draco_attention_paged(const draco_kv_cache* cache, const draco_attention_paged_args* args, int dtype,
+                          void* stream) {
+  const char* fn = "attention_paged";
+  PagedView c;
+  int rc = check_kv_cache(cache, fn, &c);
+  if (rc || (rc = check_dtype(dtype, fn))) return rc;
+  if (!args) return fail(DRACO_ERR_ARG, "%s: null arguments", fn);
+  const draco_attention_paged_args& a = *args;
+  if (a.n < 0 || a.heads < 1 || a.heads > 65536 || a.heads % c.kv_heads)
+    return fail(DRACO_ERR_SHAPE, "%s: %d tokens, %d heads over %d key/value heads", fn, a.n, a.heads, c.kv_heads);
+  if (a.max_q < 0 || a.max_kv < 0) return fail(DRACO_ERR_SHAPE, "%s: max_q %d, max_kv %d", fn, a.max_q, a.max_kv);
+  if (!(a.scale >= 0.f) || a.scale > 1e30f) return fail(DRACO_ERR_ARG, "%s: scale %g", fn, (double)a.scale);
+  if (a.n == 0 || c.n_seqs == 0) return ok();
+  if ((int64_t)a.n * (a.heads / c.kv_heads) > 0x7FFF0000) return fail(DRACO_ERR_SHAPE, "%s: %d tokens", fn, a.n);
+  if (!a.q || !a.out || !a.q_start || !a.kv_len) return fail(DRACO_ERR_ARG, "%s: null pointer", fn);
+  const int64_t qw = (int64_t)a.heads * cache->head_dim;
+  if ((rc = check_rows(a.q, a.ldq, qw, dtype, fn, "q")) || (rc = check_rows(a.out, a.ldo, qw, dtype, fn, "out")))
+    return rc;
+  if ((reinterpret_cast<uintptr_t>(a.q_start) | reinterpret_cast<uintptr_t>(a.kv_len)) & 3)
+    return fail(DRACO_ERR_ALIGN, "%s: q_start and kv_len not 4-byte aligned", fn);
+  PagedAttnArgs p = {};
+  p.c = c;
+  p.q = a.q;
+  p.out = a.out;
+  p.ldq = a.ldq;
+  p.ldo = a.ldo;
+  p.q_start = a.q_start;
+  p.kv_len = a.kv_len;
+  p.scale_log2 = (a.scale > 0.f ? a.scale : 1.f / sqrtf((float)cache->head_dim)) * 1.4426950408889634f;
+  p.n = a.n;
+  p.n_seqs = c.n_seqs;
+  p.heads = a.heads;
+  p.group = a.heads / c.kv_heads;
+  p.min_new = 0;
+  p.max_new = 0x7FFFFFFF;
+  char msg[200] = {0};
+  rc = paged_attn_launch(p, cache->head_dim, dtype, a.max_q, a.max_kv, a.workspace, a.workspace_bytes,
+                         (cudaStream_t)stream, msg, sizeof(msg));
+  return rc ? fail(rc, "%s", msg) : ok();
+}
+
+size_t draco_attention_paged_workspace_bytes(const draco_kv_cache* cache, int n, int heads, int max_q, int max_kv,
+                                             int dtype) {
+  PagedView c;
+  if (check_kv_cache(cache, "attention_paged_workspace_bytes", &c)) return 0;
+  if (check_dtype(dtype, "attention_paged_workspace_bytes") || n < 0 || heads < 1 || heads % c.kv_heads || max_q < 0 ||
+      max_kv < 0)
+    return 0;
+  return paged_attn_workspace_bytes(n, c.n_seqs, heads / c.kv_heads, c.kv_heads, cache->head_dim, max_q, max_kv,
+                                    c.type == DRACO_KV_Q8_0, dtype == DRACO_DTYPE_F32);
+}
+
+int draco_verify_drafts(const draco_verify_args* args, void* stream) {
+  const char* fn = "verify_drafts";
+  if (!args) return fail(DRACO_ERR_ARG, "%s: null arguments", fn);
+  const draco_verify_args& a = *args;
+  int rc = check_dtype(a.dtype, fn);
+  if (rc) return rc;
+  if (a.n < 0 || a.n_seqs < 0 || a.vocab < 1 || a.max_rows < 1 || a.n_seqs > (1 << 24) || a.vocab > (1 << 30))
+    return fail(DRACO_ERR_SHAPE, "%s: %d rows of %d, %d sequences of at most %d rows", fn, a.n, a.vocab, a.n_seqs,
+                a.max_rows);
+  if (!(a.temperature >= 0.f) || a.temperature > 1e30f)
+    return fail(DRACO_ERR_ARG, "%s: temperature %g", fn, (double)a.temperature);
+  if (a.n_seqs == 0) return ok();
+  if (!a.row_start || !a.accepted || !a.tokens || (a.n > 0 && (!a.logits || !a.drafts)) ||
+      (a.temperature > 0.f && (!a.accept_u || !a.sample_u)))
+    return fail(DRACO_ERR_ARG, "%s: null pointer", fn);
+  if (a.ld_logits < 0 || a.ld_tokens < a.max_rows || (a.draft_probs && a.ld_probs < 0))
+    return fail(DRACO_ERR_SHAPE, "%s: a negative row stride, or rows of tokens that overlap", fn);
+  const uintptr_t el = a.dtype == DRACO_DTYPE_F32 ? 3 : 1;
+  if ((reinterpret_cast<uintptr_t>(a.logits) & el) ||
+      ((reinterpret_cast<uintptr_t>(a.draft_probs) | reinterpret_cast<uintptr_t>(a.row_start) |
+        reinterpret_cast<uintptr_t>(a.drafts) | reinterpret_cast<uintptr_t>(a.accept_u) |
+        reinterpret_cast<uintptr_t>(a.sample_u) | reinterpret_cast<uintptr_t>(a.accepted) |
+        reinterpret_cast<uintptr_t>(a.tokens)) & 3))
+    return fail(DRACO_ERR_ALIGN, "%s: pointers must be aligned to their elements", fn);
+  char msg[200] = {0};
+  rc = verify_launch(a, (cudaStream_t)stream, msg, sizeof(msg));
+  return rc ? fail(rc, "%s", msg) : ok();
 }

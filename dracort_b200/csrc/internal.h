@@ -64,6 +64,18 @@ int attention_launch(int op, float* q, const float* k, const float* v, float* kc
 // 0..max_pos.
 size_t attention_workspace_bytes(int n, int heads, int hd, int max_pos);
 
+// Serving over a paged cache (paged_kv.cu, paged_attn.cu, verify.cu).
+struct PagedView;
+struct PagedAttnArgs;
+cudaError_t launch_kv_append(const PagedView& c, int hd, int dtype, const draco_kv_append_args& a, cudaStream_t st);
+cudaError_t launch_kv_read(const PagedView& c, int hd, int dtype, const int* seq, const int* pos, int n, void* k_out,
+                           void* v_out, int64_t ldk, int64_t ldv, cudaStream_t st);
+int paged_attn_launch(PagedAttnArgs a, int hd, int dtype, int max_q, int max_kv, void* ws, size_t ws_bytes,
+                      cudaStream_t st, char* msg, size_t ml);
+size_t paged_attn_workspace_bytes(int n, int n_seqs, int group, int kv_heads, int hd, int max_q, int max_kv, bool q8,
+                                  bool f32);
+int verify_launch(const draco_verify_args& v, cudaStream_t st, char* msg, size_t ml);
+
 // Number of SMs of the current device (cached per device).
 int device_sm_count();
 

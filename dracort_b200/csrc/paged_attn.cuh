@@ -1,0 +1,76 @@
+// paged_attn.cuh — what the two paged attention kernels share: the call's
+// arguments and the row tiles.
+#pragma once
+
+#include "paged.cuh"
+
+namespace draco {
+
+// One call.  The rows of sequence s are its new tokens' query heads of one
+// key/value head, ordered (token, head in group); a row tile takes `R`
+// consecutive rows.
+struct PagedAttnArgs {
+  PagedView c;
+  const void* q;
+  void* out;
+  int64_t ldq, ldo;
+  const int* q_start;
+  const int* kv_len;
+  float* recs;   // partial results of splits
+  int* counters;
+  float scale_log2;  // softmax scale * log2(e)
+  int n, n_seqs, heads, group, n_splits;
+  int min_new, max_new;  // this kernel takes the sequences with min_new <= new tokens < max_new
+};
+
+struct RowTile {
+  int s;         // sequence, -1: none
+  int start;     // its first token in q
+  int new_tok;   // its new tokens
+  int row0;      // first row of the tile
+  int rows;      // rows of the sequence (new_tok * group)
+  int kv;        // its cached keys
+};
+
+__device__ __forceinline__ int seq_begin(const PagedAttnArgs& a, int s) {
+  return min(max(__ldg(a.q_start + s), 0), a.n);
+}
+
+// Tile t of R rows.  Sequence s owns the tiles from floor(start_s * group / R)
+// + s on: enough for its rows whatever the other lengths are, so that no
+// prefix sum over the sequences is needed, and strictly increasing in s, so
+// that a warp finds s with a 32-ary search (one round of loads up to 32
+// sequences).  Tiles past a sequence's rows are empty.  All lanes of the warp
+// take part.
+__device__ __forceinline__ RowTile find_tile(const PagedAttnArgs& a, int t, int R) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, cnt = a.n_seqs;
+  while (cnt > 1) {
+    const int step = (cnt + 31) / 32;
+    const int s = lo + lane * step;
+    const bool le = s < lo + cnt && (int)((int64_t)seq_begin(a, s) * a.group / R) + s <= t;
+    const unsigned m = __ballot_sync(0xffffffffu, le);
+    const int k = max(__popc(m), 1) - 1;
+    cnt = min(step, cnt - k * step);
+    lo += k * step;
+  }
+  RowTile r;
+  r.s = -1;
+  r.start = seq_begin(a, lo);
+  const int end = max(seq_begin(a, lo + 1), r.start);
+  r.new_tok = end - r.start;
+  r.rows = r.new_tok * a.group;
+  r.row0 = (t - (int)((int64_t)r.start * a.group / R) - lo) * R;
+  const int64_t cap = (int64_t)a.c.max_pages << a.c.page_shift;
+  const int kv = __ldg(a.kv_len + lo);
+  r.kv = (int)(kv < 0 ? 0 : kv > cap ? cap : kv);
+  if (r.row0 >= 0 && r.row0 < r.rows && r.new_tok >= a.min_new && r.new_tok < a.max_new) r.s = lo;
+  return r;
+}
+
+// keys that row `row` of the tile's sequence sees (may be <= 0: none)
+__device__ __forceinline__ int row_limit(const PagedAttnArgs& a, const RowTile& t, int row) {
+  return t.kv - t.new_tok + row / a.group + 1;
+}
+
+}  // namespace draco

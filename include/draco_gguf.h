@@ -440,6 +440,166 @@ int draco_attention_decode(const float* q, const float* k, const float* v, float
  * for invalid arguments). */
 size_t draco_attention_workspace_bytes(int n, int heads, int head_dim, int max_pos);
 
+/* ---- serving over a paged key/value cache -------------------------------
+ * One layer's cache: `n_pages` pages of `page_size` positions, keys in `k` and
+ * values in `v`, each [n_pages][kv_heads][page_size] rows of head_dim values:
+ *   DRACO_KV_BF16: bf16 rows, rounded to nearest even;
+ *   DRACO_KV_Q8_0: per page and head page_size * head_dim int8 quants, then
+ *     page_size * (head_dim / 32) fp16 scales; value = scale * quant.  Blocks
+ *     of 32 values by the Q8_0 rule (scale = max|x| / 127, quant = rint(x /
+ *     scale), draco/format/gguf.py:300-303 decodes them); values beyond
+ *     +-65024 are clamped to it, a NaN makes its block NaN.
+ * draco_kv_cache_bytes() gives the bytes of k, and of v.
+ * Position p of sequence s lives in page block_table[s * table_stride + p /
+ * page_size] (device int32, max_pages entries per sequence; stride 0: one row
+ * for all), row p % page_size.  Sequences may share pages (a common prefix).  A position beyond
+ * the table, or whose entry is outside 0..n_pages - 1, is never accessed: it
+ * is not written, and reads as zeros.
+ * head_dim 32, 64, 96, 128 or 256; page_size a power of two from 16 to 1024;
+ * k and v 16-byte aligned.  The reference's paged attention and block manager
+ * (draco/attention/paged.py:26-269, draco/kv_cache/block.py:119-441) keep
+ * pages of 16- or 32-bit values in torch. */
+#define DRACO_KV_BF16 1
+#define DRACO_KV_Q8_0 8
+
+typedef struct draco_kv_cache {
+  int type; /* DRACO_KV_* */
+  int kv_heads;
+  int head_dim;
+  int page_size;
+  int n_pages;
+  int n_seqs;    /* rows of the block table */
+  int max_pages; /* entries of a sequence's row */
+  int64_t table_stride;
+  void* k;
+  void* v;
+  const int* block_table;
+} draco_kv_cache;
+
+/* Bytes of a cache's k (or v) buffer, -1 for unsupported arguments.  Host only. */
+int64_t draco_kv_cache_bytes(int type, int n_pages, int kv_heads, int page_size, int head_dim);
+
+/* New tokens for the cache.  Token i belongs to sequence seq[i] at absolute
+ * position pos[i] (device int32).
+ *   q, k, v : [n, heads | kv_heads, head_dim] of `dtype` (DRACO_DTYPE_F32 or
+ *             DRACO_DTYPE_BF16), token strides ldq / ldk / ldv elements (q/k/v
+ *             may be slices of one projection's output).  q may be NULL.
+ *   q_out   : the rotated q, token stride ldqo; may be q; NULL with q NULL
+ *   cos_table, sin_table : [max_positions, head_dim / 2] fp32
+ *             (draco/runtime/cpu/ops.py:77-83); both NULL: no rotation
+ * q and k are rotated as draco_rope_kv_append rotates them; the rotated key
+ * and the value are rounded to the cache's type.  Tokens of one call go to
+ * distinct rows: a row that two of them share holds no meaning afterwards.  A
+ * token whose sequence or position is outside the cache or the tables writes no
+ * key or value; its q is rotated if its position is inside the tables and
+ * copied otherwise. */
+typedef struct draco_kv_append_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  int64_t ldq, ldk, ldv, ldqo;
+  const float* cos_table;
+  const float* sin_table;
+  int64_t max_positions;
+  const int* seq;
+  const int* pos;
+  int n;
+  int heads;
+} draco_kv_append_args;
+int draco_kv_append(const draco_kv_cache* cache, const draco_kv_append_args* args, int dtype, void* stream);
+
+/* Rows of the cache as values: k_out and v_out [n, kv_heads, head_dim] of
+ * `dtype`, token strides ldk / ldv elements, row i the position pos[i] of
+ * sequence seq[i].  Exact in fp32; bf16 rounds once. */
+int draco_kv_read(const draco_kv_cache* cache, const int* seq, const int* pos, int n, void* k_out, void* v_out,
+                  int64_t ldk, int64_t ldv, int dtype, void* stream);
+
+/* Causal attention of new tokens over the paged cache, all sequences of a
+ * batch in one call: a decode step (one token each), drafted tokens, a chunk
+ * of a prompt, whole prompts, or a mixture.  Their keys and values are in the
+ * cache already (draco_kv_append).
+ *   q, out : [n, heads, head_dim] of `dtype`, token strides ldq / ldo elements;
+ *            16-byte aligned rows; out may be q
+ *   q_start: device int32 [n_seqs + 1], ascending: the tokens q_start[s] ..
+ *            q_start[s + 1] - 1 are sequence s's newest
+ *   kv_len : device int32 [n_seqs], the sequence's cached positions, its new
+ *            tokens included
+ * Token i (from 0) of a sequence's m new ones sees positions 0 .. kv_len - m +
+ * i: out = softmax(scale q K^T) V, query head h reading key/value head
+ * h / (heads / kv_heads).  A token that sees no position (kv_len < m) gets
+ * zeros; rows of out behind the last sequence stay as they are.  max_q and
+ * max_kv bound the sequences' new tokens and cached positions: they size the
+ * launch and the workspace and need not be tight (results do not depend on
+ * lengths beyond max_kv being wrong, only the speed does; a sequence of more
+ * than max_q new tokens is still computed).
+ * scale 0 means 1 / sqrt(head_dim).  m, l and the output are accumulated in
+ * fp32; fp32 activations keep fp32 accuracy, bf16 ones round the
+ * probabilities to 16 bits.
+ * Workspace: at least draco_attention_paged_workspace_bytes() bytes, 16-byte
+ * aligned, zeroed before its first use, left ready for the next call on the
+ * same stream; two calls that may overlap need two. */
+typedef struct draco_attention_paged_args {
+  const void* q;
+  void* out;
+  int64_t ldq, ldo;
+  const int* q_start;
+  const int* kv_len;
+  int n;
+  int heads;
+  int max_q;
+  int max_kv;
+  float scale;
+  void* workspace;
+  size_t workspace_bytes;
+} draco_attention_paged_args;
+int draco_attention_paged(const draco_kv_cache* cache, const draco_attention_paged_args* args, int dtype,
+                          void* stream);
+size_t draco_attention_paged_workspace_bytes(const draco_kv_cache* cache, int n, int heads, int max_q, int max_kv,
+                                             int dtype);
+
+/* Verification of drafted tokens (speculative sampling; the reference verifies
+ * n-gram drafts greedily, draco/runtime/cpu/speculative.py).  Sequence s owns
+ * rows row_start[s] .. row_start[s + 1] - 1 (device int32 [n_seqs + 1],
+ * ascending) of logits [n, vocab]: one row per draft and one more.
+ *   logits      : of `dtype`, row stride ld_logits (0: one row for all)
+ *   drafts      : device int32 [n]: the token proposed after row r (the entry
+ *                 of a sequence's last row is not read)
+ *   draft_probs : fp32 [n, vocab], row stride ld_probs: the drafter's
+ *                 probabilities, or NULL: each draft was certain
+ *   accept_u    : fp32 [n], sample_u fp32 [n_seqs]: uniform numbers in [0, 1)
+ *   temperature : p = softmax(logits / temperature); 0: greedy
+ * Draft x of row r is taken while accept_u[r] * q(x) < p(x) (greedy: x is the
+ * first index of the largest logit); at the first that is not, the next token
+ * is drawn from max(p - q, 0) (from p where that is zero everywhere), after the
+ * last draft from p: the first index whose cumulative weight exceeds
+ * sample_u[s] times the total, accumulated in fp64.
+ *   accepted : int32 [n_seqs], drafts taken
+ *   tokens   : int32 [n_seqs, max_rows], row stride ld_tokens: the drafts
+ *              taken, the next token, then -1
+ * One row and no draft is plain sampling.  A sequence of no rows gives 0
+ * and -1s.  NaN logits count as -infinity; a row of -infinity has no token
+ * (-1); a draft outside the vocabulary is not taken.  max_rows is the largest
+ * number of rows of a sequence: tokens past it are not stored. */
+typedef struct draco_verify_args {
+  const void* logits;
+  const float* draft_probs;
+  const int* row_start;
+  const int* drafts;
+  const float* accept_u;
+  const float* sample_u;
+  int* accepted;
+  int* tokens;
+  int64_t ld_logits, ld_probs, ld_tokens;
+  float temperature;
+  int dtype;
+  int n;
+  int n_seqs;
+  int vocab;
+  int max_rows;
+} draco_verify_args;
+int draco_verify_drafts(const draco_verify_args* args, void* stream);
+
 /* Single-weight convenience form of draco_gguf_gemv_grouped. */
 int draco_gguf_gemv(int qtype, const void* w_tiled, const float* x, float* y, const float* bias,
                     int batch, int64_t n_rows, int64_t k, void* workspace,
