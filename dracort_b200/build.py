@@ -29,7 +29,7 @@ STAMP_PATH = LIB_DIR / "build.stamp"
 INCLUDE = REPO_DIR / "include"
 
 SOURCES = ["capi.cu", "dequant.cu", "gemv.cu", "gemv_tc.cu", "gemm.cu", "act.cu", "tp.cu", "attn.cu", "paged_kv.cu",
-           "paged_attn.cu", "verify.cu"]
+           "paged_attn.cu", "paged_attn_tc.cu", "verify.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
 

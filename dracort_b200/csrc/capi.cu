@@ -608,8 +608,7 @@ size_t draco_attention_paged_workspace_bytes(const draco_kv_cache* cache, int n,
   if (check_dtype(dtype, "attention_paged_workspace_bytes") || n < 0 || heads < 1 || heads % c.kv_heads || max_q < 0 ||
       max_kv < 0)
     return 0;
-  return paged_attn_workspace_bytes(n, c.n_seqs, heads / c.kv_heads, c.kv_heads, cache->head_dim, max_q, max_kv,
-                                    c.type == DRACO_KV_Q8_0, dtype == DRACO_DTYPE_F32);
+  return paged_attn_workspace_bytes(c, n, heads / c.kv_heads, cache->head_dim, dtype, max_q, max_kv);
 }
 
 int draco_verify_drafts(const draco_verify_args* args, void* stream) {

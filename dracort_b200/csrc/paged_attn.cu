@@ -43,7 +43,6 @@
 namespace draco {
 
 constexpr int kPaThreads = 128;
-constexpr int kPaCounters = 2048;  // (row tile, kv head) pairs that may be split
 constexpr float kPaLazy = 8.f;
 constexpr int kPaMinSplit = 256;   // keys of a split at least (16 blocks per warp group at WM 1)
 
@@ -642,7 +641,7 @@ static int pick_wm(int max_q, int group, int hd, bool q8, bool f32) {
 // Splits of the keys: about three CTAs for each of the two that an SM holds, so
 // that sequences of different lengths even out, none shorter than kPaMinSplit.
 static int pick_splits(int64_t units, int max_kv) {
-  if (units > kPaCounters || units < 1) return 1;
+  if (units > kPagedCounters || units < 1) return 1;
   const int64_t want = 6LL * device_sm_count();
   int64_t s = std::min((want + units - 1) / units, ((int64_t)max_kv + kPaMinSplit - 1) / kPaMinSplit);
   return (int)std::max<int64_t>(1, std::min<int64_t>(s, 128));
@@ -650,23 +649,33 @@ static int pick_splits(int64_t units, int max_kv) {
 struct PaPlan {
   int wm, splits;
   int64_t tiles, units;
-  size_t bytes;
+  size_t bytes;  // of partial results
 };
-static PaPlan plan_of(int n, int n_seqs, int group, int kv_heads, int hd, int max_q, int max_kv, bool q8,
-                      bool f32) {
+static PaPlan plan_of(int n, int n_seqs, int group, int kv_heads, int hd, int max_q, int max_kv, bool q8, bool f32) {
   PaPlan p;
   p.wm = pick_wm(max_q, group, hd, q8, f32);
   p.tiles = (int64_t)n * group / (16 * p.wm) + n_seqs;
   p.units = p.tiles * kv_heads;
   p.splits = pick_splits(p.units, max_kv);
-  p.bytes = kPaCounters * sizeof(int);
-  if (p.splits > 1) p.bytes += (size_t)p.units * p.splits * 16 * p.wm * (hd + 2) * sizeof(float);
+  p.bytes = p.splits > 1 ? (size_t)p.units * p.splits * 16 * p.wm * (hd + 2) * sizeof(float) : 0;
   return p;
 }
 
-size_t paged_attn_workspace_bytes(int n, int n_seqs, int group, int kv_heads, int hd, int max_q, int max_kv, bool q8,
-                                  bool f32) {
-  return plan_of(n, n_seqs, group, kv_heads, hd, max_q, max_kv, q8, f32).bytes;
+// New tokens from which a sequence goes to the tensor-memory kernel, or 0: none
+// does.  Its CTA takes 256 rows at a time however few there are.
+constexpr int kTcMinRows = 64;
+static int tc_from(const PagedView& c, int hd, int dtype, int group, int max_q) {
+  if (!paged_attn_tc_takes(c, hd, dtype, group, 1 << c.page_shift)) return 0;
+  const int from = kTcMinRows / group + 1;
+  return max_q >= from ? from : 0;
+}
+
+size_t paged_attn_workspace_bytes(const PagedView& c, int n, int group, int hd, int dtype, int max_q, int max_kv) {
+  const bool q8 = c.type == DRACO_KV_Q8_0, f32 = dtype == DRACO_DTYPE_F32;
+  const int from = tc_from(c, hd, dtype, group, max_q);
+  size_t bytes = plan_of(n, c.n_seqs, group, c.kv_heads, hd, from ? from - 1 : max_q, max_kv, q8, f32).bytes;
+  if (from) bytes = std::max(bytes, paged_attn_tc_plan(n, c.n_seqs, group, c.kv_heads, hd, max_kv).bytes);
+  return kPagedHead + bytes;
 }
 
 template <int HD, bool Q8, bool F32, int WM>
@@ -716,13 +725,19 @@ static cudaError_t launch_hd(int hd, const PagedAttnArgs& a, const PaPlan& p, cu
 int paged_attn_launch(PagedAttnArgs a, int hd, int dtype, int max_q, int max_kv, void* ws, size_t ws_bytes,
                       cudaStream_t st, char* msg, size_t ml) {
   const bool q8 = a.c.type == DRACO_KV_Q8_0, f32 = dtype == DRACO_DTYPE_F32;
-  const PaPlan p = plan_of(a.n, a.n_seqs, a.group, a.c.kv_heads, hd, max_q, max_kv, q8, f32);
-  if (ws == nullptr || ws_bytes < p.bytes || (reinterpret_cast<uintptr_t>(ws) & 15)) {
-    snprintf(msg, ml, "attention_paged: workspace of %zu bytes given (16-byte aligned), %zu needed", ws_bytes, p.bytes);
+  const size_t need = paged_attn_workspace_bytes(a.c, a.n, a.group, hd, dtype, max_q, max_kv);
+  if (ws == nullptr || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 15)) {
+    snprintf(msg, ml, "attention_paged: workspace of %zu bytes given (16-byte aligned), %zu needed", ws_bytes, need);
     return DRACO_ERR_WORKSPACE;
   }
   a.counters = static_cast<int*>(ws);
-  a.recs = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kPaCounters * sizeof(int));
+  a.recs = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kPagedHead);
+  // long sequences to the tensor-memory kernel, the others (any that a batch
+  // holds beside them: the lengths are on the device) to the warp MMA
+  const int from = tc_from(a.c, hd, dtype, a.group, max_q);
+  a.min_new = 0;
+  a.max_new = from ? from : 0x7FFFFFFF;
+  const PaPlan p = plan_of(a.n, a.n_seqs, a.group, a.c.kv_heads, hd, from ? from - 1 : max_q, max_kv, q8, f32);
   a.n_splits = p.splits;
   const cudaError_t e = q8 ? (f32 ? launch_hd<true, true>(hd, a, p, st) : launch_hd<true, false>(hd, a, p, st))
                            : (f32 ? launch_hd<false, true>(hd, a, p, st) : launch_hd<false, false>(hd, a, p, st));
@@ -730,7 +745,11 @@ int paged_attn_launch(PagedAttnArgs a, int hd, int dtype, int max_q, int max_kv,
     snprintf(msg, ml, "attention_paged launch failed: %s", cudaGetErrorString(e));
     return DRACO_ERR_CUDA;
   }
-  return DRACO_OK;
+  if (!from) return DRACO_OK;
+  a.min_new = from;
+  a.max_new = 0x7FFFFFFF;
+  const TcPlan t = paged_attn_tc_plan(a.n, a.n_seqs, a.group, a.c.kv_heads, hd, max_kv);
+  return paged_attn_tc_launch(a, hd, t, a.counters + kPagedCounters, st, msg, ml);
 }
 
 }  // namespace draco

@@ -6,6 +6,10 @@
 
 namespace draco {
 
+constexpr int kPagedCounters = 2048;  // (row tile, kv head) pairs that may be split over CTAs
+// workspace: int32 counters [kPagedCounters], status word, padding to this; then partial results
+constexpr int kPagedHead = kPagedCounters * 4 + 64;
+
 // One call.  The rows of sequence s are its new tokens' query heads of one
 // key/value head, ordered (token, head in group); a row tile takes `R`
 // consecutive rows.
@@ -72,5 +76,16 @@ __device__ __forceinline__ RowTile find_tile(const PagedAttnArgs& a, int t, int 
 __device__ __forceinline__ int row_limit(const PagedAttnArgs& a, const RowTile& t, int row) {
   return t.kv - t.new_tok + row / a.group + 1;
 }
+
+// the tensor-memory kernel (paged_attn_tc.cu)
+struct TcPlan {
+  int rt, splits;
+  int64_t tiles, units;
+  size_t bytes;  // of partial results
+};
+bool paged_attn_tc_takes(const PagedView& c, int hd, int dtype, int group, int page_size);
+TcPlan paged_attn_tc_plan(int n, int n_seqs, int group, int kv_heads, int hd, int max_kv);
+int paged_attn_tc_launch(const PagedAttnArgs& a, int hd, const TcPlan& p, int* status, cudaStream_t st, char* msg,
+                         size_t ml);
 
 }  // namespace draco

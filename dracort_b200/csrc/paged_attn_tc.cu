@@ -1,0 +1,839 @@
+// paged_attn_tc.cu — causal attention of long chunks and prompts over the paged
+// cache on the 5th-generation tensor cores (tcgen05): bf16 activations,
+// head_dim up to 128, bf16 or Q8_0 pages (draco_attention_paged chooses).
+//
+// Mathematics as in paged_attn.cu: one pass over the keys, S = Q K^T, P =
+// exp2(c S - m), O += P V, the reference m raised (and O rescaled) only when
+// the row's maximum outgrows it by 2^8.
+//
+// What bounds it: the tensor cores and, at the same rate for head_dim 128, the
+// 16 exponentials per clock of an SM.  A CTA holds two tiles of 128 rows (a
+// row is a (token, query head) pair of one key/value head, so the heads of a
+// group share the key tiles) and keeps both units busy by turns: while one
+// tile's scores go through the softmax warps, the MMAs of the other run.
+//   warps 0-3, 4-7   softmax of tile 0 and 1: a thread owns a row: it reads the
+//                    row's 128 scores from tensor memory, forms P and stores it
+//                    over them as the A operand of the second product, so P
+//                    never goes through shared memory;
+//   warp 8           issues the MMAs: for each key tile j and row tile w, PV_w
+//                    of tile j, then S_w of tile j + 1 into the columns that P_w
+//                    leaves;
+//   bf16 pages:      warp 9 loads key and value tiles page by page with TMA
+//                    (128-byte swizzle; a bad page is loaded from past the
+//                    end: zeros), warps 10-11 clean the value tiles at the
+//                    causal edge (below);
+//   Q8_0 pages:      warps 12-19 load quants and scales, and write d * quant as
+//                    fp16 (11 bits of its 18) into the same swizzled tiles.
+// Tensor memory: two 128-column S / P tiles, two O tiles; shared memory: two
+// Q tiles, two stages of key and value tiles; one CTA per SM.  Key tiles are
+// read from the L2 by the CTAs of a head, whose row tiles run side by side.
+// Q8_0: operands are fp16, q is scaled per row by a power of two and P by 2^6,
+// as in paged_attn.cu.
+//
+// Rows that see no key of a tile multiply its values by P = 0, so values past
+// the end, and values that are not finite in tiles with masked pairs, are
+// replaced by zeros in shared memory; the latter are marked, and the rows that
+// do see them add their products at the end, element by element.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <cstdio>
+
+#include "internal.h"
+#include "paged_attn.cuh"
+
+namespace draco {
+
+constexpr int kTcRows = 128;            // rows of a tile (fewer when the group does not divide 128)
+constexpr int kTcKeys = 128;
+constexpr uint64_t kTcWaitNs = 2000000000ull;  // 2 s: far beyond any legitimate wait
+constexpr int kTcBadWords = 32;         // marks of 1024 keys from the first edge tile on
+
+struct __align__(64) TcParams {
+  CUtensorMap qmap, kmap, vmap;
+  PagedAttnArgs a;
+  int rt;        // rows of a row tile: group * (128 / group)
+  int hd;
+  int box_rows;  // rows of a TMA box: min(page_size, 128)
+  int page_rows; // rows in the key (or value) buffer: pages * kv_heads * page_size
+  int* status;
+};
+
+template <int HDP, bool Q8>
+struct TcCfg {
+  static constexpr int kBoxes = HDP / 64;
+  static constexpr int kHalf = 128 * 128;                 // 128 rows x 64 values
+  static constexpr int kTile = kBoxes * kHalf;            // 32 or 16 KB
+  static constexpr int kStages = 2;
+  static constexpr int kSmem = 1024 + 2 * kTile + kStages * 2 * kTile;
+  static constexpr int kThreads = Q8 ? 640 : 384;
+  static constexpr int kProducers = 8;                    // Q8_0: converting warps
+  // registers of a thread: softmax warpgroups, the MMA / load warpgroup, converting warpgroups
+  static constexpr int kRegsSoftmax = Q8 ? 168 : 208, kRegsOne = Q8 ? 32 : 80, kRegsConvert = 56;
+  static constexpr int kRegsBlock = 256 * kRegsSoftmax + 128 * kRegsOne + (kThreads - 384) * kRegsConvert;
+};
+
+__device__ __forceinline__ void tca_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tca_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tca_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tca_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+// Shared-memory operand with the 128-byte swizzle, rows of 64 values at 128
+// bytes, 8-row groups at 1024 (version 1, layout 2).  K-major: rows are M / N,
+// values K; MN-major: rows are K, values N, and `lbo` is the distance between
+// 64-value groups of N.
+__device__ __forceinline__ uint64_t tca_desc(uint32_t addr, uint32_t lbo) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// fp32 D; A and B bf16 (format 1) or fp16 (0); bit 16: B is MN-major
+__host__ __device__ constexpr uint32_t tca_idesc(bool bf16, int m, int n, bool b_mn) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void tca_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void tca_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void tca_ld32(uint32_t addr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+// waits for this thread's loads; ties 32 of the loaded registers to the wait
+__device__ __forceinline__ void tca_ld_wait(float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void tca_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tca_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tca_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tca_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ float tca_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+struct TcBars {
+  uint64_t q_full, q_ready;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], v_clean[2];
+  uint64_t s_full[2], p_full[2], o_full[2], drain;
+};
+
+template <int HDP, bool Q8>
+__global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
+    paged_attn_tc_kernel(const __grid_constant__ TcParams P) {
+  using C = TcCfg<HDP, Q8>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) TcBars bars;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort, s_last;
+  __shared__ uint32_t s_bad[kTcBadWords];
+  const PagedAttnArgs& a = P.a;
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t* q_s = smem;                       // [2] Q tiles
+  uint8_t* k_s = smem + 2 * C::kTile;        // [stage] key tiles
+  uint8_t* v_s = k_s + C::kStages * C::kTile;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grid_dependency_wait();
+  const int tile_id = gridDim.x - 1 - blockIdx.x;  // the tiles with the most keys first
+  const RowTile tile = find_tile(a, tile_id, 2 * P.rt);
+  if (tile.s < 0) return;
+  const int kvh = blockIdx.z, hd = P.hd;
+  const int rows = min(2 * P.rt, tile.rows - tile.row0);
+  const int kend = max(0, min(tile.kv, row_limit(a, tile, tile.row0 + rows - 1)));
+  int ck = (kend + a.n_splits - 1) / a.n_splits;
+  ck = max(kTcKeys, (ck + kTcKeys - 1) & ~(kTcKeys - 1));
+  const int active = max(1, (kend + ck - 1) / ck);
+  const int split = blockIdx.y;
+  if (split >= active) return;
+  const int kbeg = split * ck, kfin = min(kend, kbeg + ck);
+  const int nj = (kfin - kbeg + kTcKeys - 1) / kTcKeys;  // key tiles
+  // the first tile in which some row is masked (or keys end)
+  const int first_lim = max(0, min(tile.kv, row_limit(a, tile, tile.row0)));
+  const int jedge = max(0, min(nj, first_lim <= kbeg ? 0 : (first_lim - kbeg) / kTcKeys));
+
+  if (tid == 0) {
+    mbar_init(&bars.q_full, 1);
+    mbar_init(&bars.q_ready, 8);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.k_full[i], Q8 ? C::kProducers : 1);
+      mbar_init(&bars.v_full[i], Q8 ? C::kProducers : 1);
+      mbar_init(&bars.k_empty[i], 1);
+      mbar_init(&bars.v_empty[i], 1);
+      mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_full[i], 4);
+      mbar_init(&bars.o_full[i], 1);
+      mbar_init(&bars.v_clean[i], 2);
+    }
+    mbar_init(&bars.drain, 1);
+    fence_mbar_init();
+    s_abort = 0;
+  }
+  if (tid < kTcBadWords) s_bad[tid] = 0;
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tca_before();
+  __syncthreads();
+  tca_after();
+  const uint32_t tmem = s_tmem;
+
+  // a wait that gives up: the role leaves its loop, the others' waits run out
+  // too.  (Every barrier's next phase but one needs the waiting side to have
+  // passed, so a parity never stands for two phases.)
+  auto wait = [&](uint64_t* bar, int phase) -> bool {
+    if (mbar_wait_bounded(bar, (uint32_t)phase & 1u, kTcWaitNs)) return true;
+    s_abort = 1;
+    return false;
+  };
+  auto wait_warp = [&](uint64_t* bar, int phase) -> bool {
+    return __all_sync(0xffffffffu, wait(bar, phase));
+  };
+
+  // registers by warpgroup: the sums stay within what the block is launched with
+  if (warp < 8)
+    regs_up<C::kRegsSoftmax>();
+  else if (warp < 12)
+    regs_down<C::kRegsOne>();
+  else
+    regs_down<C::kRegsConvert>();
+
+  if (warp < 8) {
+    // ------------------------------------------------------------- softmax
+    const int w = warp >> 2, rw = 32 * (warp & 3) + lane;  // row of the tile
+    const int r = w * P.rt + rw;                           // row of the CTA
+    const bool valid = rw < P.rt && r < rows;
+    const int lim = valid ? max(0, min(tile.kv, row_limit(a, tile, tile.row0 + r))) : 0;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+    const uint32_t s_t = tmem + 128 * w + lanes, o_t = tmem + 256 + HDP * w + lanes;
+    float sc = a.scale_log2;
+    bool ok = true;
+    if constexpr (Q8) {
+      // q as fp16, scaled by a power of two to at most 1 per row
+      ok = nj == 0 || wait_warp(&bars.q_full, 0);
+      if (ok && nj > 0) {
+        uint8_t* row = q_s + w * C::kTile + rw * 128;
+        float m = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < HDP / 8; ++c) {
+          const uint4 u = *reinterpret_cast<const uint4*>(row + (c >> 3) * C::kHalf + (((c & 7) ^ (rw & 7)) << 4));
+          m = fmaxf(fmaxf(fmaxf(m, fmaxf(fabsf(bf16lo(u.x)), fabsf(bf16hi(u.x)))),
+                          fmaxf(fabsf(bf16lo(u.y)), fabsf(bf16hi(u.y)))),
+                    fmaxf(fmaxf(fabsf(bf16lo(u.z)), fabsf(bf16hi(u.z))),
+                          fmaxf(fabsf(bf16lo(u.w)), fabsf(bf16hi(u.w)))));
+        }
+        float s = 1.f;
+        if (m > 1e-30f && m < 1e38f) s = __int_as_float((__float_as_int(m) & 0x7F800000) + 0x00800000);
+        const float inv = 1.f / s;
+        sc *= s;
+#pragma unroll 1
+        for (int c = 0; c < HDP / 8; ++c) {
+          uint4* p = reinterpret_cast<uint4*>(row + (c >> 3) * C::kHalf + (((c & 7) ^ (rw & 7)) << 4));
+          const uint4 u = *p;
+          *p = make_uint4(pack_f16(bf16lo(u.x) * inv, bf16hi(u.x) * inv), pack_f16(bf16lo(u.y) * inv, bf16hi(u.y) * inv),
+                          pack_f16(bf16lo(u.z) * inv, bf16hi(u.z) * inv), pack_f16(bf16lo(u.w) * inv, bf16hi(u.w) * inv));
+        }
+        tca_proxy();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.q_ready);
+      }
+    }
+    constexpr float kShift = Q8 ? 6.f : 0.f;
+    float m = -INFINITY, l = 0.f;
+    for (int j = 0; j < nj && ok; ++j) {
+      if (!(ok = wait_warp(&bars.s_full[w], j))) break;
+      tca_after();
+      float s[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tca_ld32(s_t + 32 * c, s + 32 * c);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tca_ld_wait(s + 32 * c);
+      const int k0 = kbeg + j * kTcKeys;
+      if (__any_sync(0xffffffffu, k0 + kTcKeys > lim)) {
+        const int vis = lim - k0;
+#pragma unroll
+        for (int i = 0; i < 128; ++i) s[i] = i < vis ? s[i] : -INFINITY;
+      }
+      float x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3];
+#pragma unroll
+      for (int i = 4; i < 128; i += 4) {
+        x0 = fmaxf(x0, s[i]), x1 = fmaxf(x1, s[i + 1]), x2 = fmaxf(x2, s[i + 2]), x3 = fmaxf(x3, s[i + 3]);
+      }
+      const float mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * sc;
+      if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+        const float n = fmaxf(m, mx);
+        const float f = n == -INFINITY ? 1.f : tca_exp2(m - n);
+        m = n;
+        l *= f;
+        if (j > 0) {  // O of the tiles so far is complete: the scores of tile j came after it
+#pragma unroll 1
+          for (int c = 0; c < HDP / 32; ++c) {
+            float o[32];
+            tca_ld32(o_t + 32 * c, o);
+            tca_ld_wait(o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= f;
+            tca_st32(o_t + 32 * c, reinterpret_cast<uint32_t*>(o));
+          }
+        }
+      }
+      const float ref = m == -INFINITY ? 0.f : m - kShift;
+      float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t p[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float u = tca_exp2(fmaf(s[64 * c + 2 * i], sc, -ref)), v = tca_exp2(fmaf(s[64 * c + 2 * i + 1], sc, -ref));
+          l0 += u, l1 += v;
+          p[i] = Q8 ? pack_f16(u, v) : pack_bf16(u, v);
+        }
+        tca_st32(s_t + 32 * c, p);
+      }
+      l += l0 + l1;
+      tca_st_wait();
+      tca_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.p_full[w]);
+    }
+    if (ok && nj > 0) ok = wait_warp(&bars.o_full[w], 0);
+    tca_after();
+    // marked values: what the rows that see them add
+    uint32_t any_bad = 0;
+#pragma unroll 1
+    for (int i = 0; i < kTcBadWords; ++i) any_bad |= s_bad[i];
+    const int rr = tile.row0 + r;
+    const int64_t unit = (int64_t)tile_id * a.c.kv_heads + kvh;
+    float* rec = a.recs + (unit * a.n_splits + split) * (int64_t)(2 * P.rt) * (hd + 2);
+    __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(a.out) + (int64_t)(tile.start + rr / a.group) * a.ldo +
+                          (int64_t)(kvh * a.group + rr % a.group) * hd;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (ok) {
+#pragma unroll 1
+      for (int c = 0; c < HDP / 32 && 32 * c < hd; ++c) {
+        __syncwarp();
+        float o[32];
+        if (nj > 0) {
+          tca_ld32(o_t + 32 * c, o);
+          tca_ld_wait(o);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+        if (any_bad != 0 && valid) {
+          const uint8_t* qrow = q_s + w * C::kTile + rw * 128;
+#pragma unroll 1
+          for (int b = 0; b < kTcBadWords * 32; ++b) {
+            if (!((s_bad[b >> 5] >> (b & 31)) & 1u)) continue;
+            const int key = kbeg + jedge * kTcKeys + b;
+            if (key >= lim) break;
+            const int page = page_of(a.c, tile.s, key), off = key & ((1 << a.c.page_shift) - 1);
+            const int64_t at = ((int64_t)page * a.c.kv_heads + kvh) * a.c.block_bytes;
+            float dot = 0.f;
+#pragma unroll 1
+            for (int d = 0; d < hd; ++d) {
+              const uint16_t qb = *reinterpret_cast<const uint16_t*>(
+                  qrow + (d >> 6) * C::kHalf + ((((d >> 3) & 7) ^ (rw & 7)) << 4) + 2 * (d & 7));
+              float kv;
+              if constexpr (Q8)
+                kv = __half2float(reinterpret_cast<const __half*>(a.c.k + at + ((int64_t)hd << a.c.page_shift))
+                                      [off * (hd / 32) + d / 32]) *
+                     (float)reinterpret_cast<const int8_t*>(a.c.k + at)[off * hd + d];
+              else
+                kv = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.c.k + at)[off * hd + d]);
+              dot = fmaf(Q8 ? __half2float(__ushort_as_half(qb)) : __uint_as_float((uint32_t)qb << 16), kv, dot);
+            }
+            const float p = tca_exp2(fmaf(dot, sc, -(m == -INFINITY ? 0.f : m - kShift)));
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const int d = 32 * c + i;
+              float v;
+              if constexpr (Q8)
+                v = __half2float(reinterpret_cast<const __half*>(a.c.v + at + ((int64_t)hd << a.c.page_shift))
+                                     [off * (hd / 32) + d / 32]) *
+                    (float)reinterpret_cast<const int8_t*>(a.c.v + at)[off * hd + d];
+              else
+                v = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.c.v + at)[off * hd + d]);
+              if (!(fabsf(v) < INFINITY)) o[i] = fmaf(p, v, o[i]);
+            }
+          }
+        }
+        if (valid && active == 1) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = l == 0.f ? 0.f : o[i + e] * inv;
+            store8(orow + 32 * c + i, x);
+          }
+        } else if (valid) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            __stcg(reinterpret_cast<float4*>(rec + 4 * P.rt + (int64_t)r * hd + 32 * c + i),
+                   make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]));
+          if (c == 0) __stcg(reinterpret_cast<float2*>(rec + 2 * r), make_float2(m, l));
+        }
+      }
+    }
+    if (active > 1) {
+      __threadfence();  // this thread's record before the arrival
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (tid == 0) {
+        s_last = 0;
+        if (!s_abort) {
+          const int prev = atomicAdd(a.counters + unit, 1);
+          s_last = prev == active - 1;
+          if (s_last) {
+            atomicExch(a.counters + unit, 0);
+            __threadfence();
+          }
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      {
+        if (s_last && valid) {
+          const int64_t rsz = (int64_t)(2 * P.rt) * (hd + 2);
+          const float* recs = a.recs + unit * a.n_splits * rsz;
+          float M = -INFINITY, L = 0.f;
+          for (int sp = 0; sp < active; ++sp) M = fmaxf(M, __ldcg(recs + sp * rsz + 2 * r));
+          for (int sp = 0; sp < active; ++sp) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(recs + sp * rsz + 2 * r));
+            if (ml.x == -INFINITY && ml.y == ml.y) continue;
+            L = fmaf(ml.x == -INFINITY ? 0.f : tca_exp2(ml.x - M), ml.y, L);
+          }
+          const float iv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll 1
+          for (int d = 0; d < hd; d += 8) {
+            float x[8] = {};
+#pragma unroll 1
+            for (int sp = 0; sp < active; ++sp) {
+              const float* rc = recs + sp * rsz;
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(rc + 2 * r));
+              if (ml.x == -INFINITY && ml.y == ml.y) continue;
+              const float f = ml.x == -INFINITY ? 0.f : tca_exp2(ml.x - M);
+              const float4 u = __ldcg(reinterpret_cast<const float4*>(rc + 4 * P.rt + (int64_t)r * hd + d));
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(rc + 4 * P.rt + (int64_t)r * hd + d + 4));
+              x[0] = fmaf(f, u.x, x[0]), x[1] = fmaf(f, u.y, x[1]), x[2] = fmaf(f, u.z, x[2]), x[3] = fmaf(f, u.w, x[3]);
+              x[4] = fmaf(f, v.x, x[4]), x[5] = fmaf(f, v.y, x[5]), x[6] = fmaf(f, v.z, x[6]), x[7] = fmaf(f, v.w, x[7]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = L == 0.f ? 0.f : x[e] * iv;
+            store8(orow + d, x);
+          }
+        }
+      }
+    }
+    tca_before();
+  } else if (warp == 8) {
+    // ------------------------------------------------------------- MMA
+    if (lane == 0 && nj > 0) {
+      constexpr uint32_t ids = tca_idesc(!Q8, 128, 128, false), ido = tca_idesc(!Q8, 128, HDP, true);
+      const uint32_t q_u = smem_u32(q_s), k_u = smem_u32(k_s), v_u = smem_u32(v_s);
+      auto scores = [&](int w, int j) {
+        const uint32_t qa = q_u + w * C::kTile, ka = k_u + (j & 1) * C::kTile;
+#pragma unroll
+        for (int k = 0; k < HDP / 16; ++k) {
+          const uint32_t at = (k >> 2) * C::kHalf + (k & 3) * 32;
+          tca_mma_ss(tmem + 128 * w, tca_desc(qa + at, 16), tca_desc(ka + at, 16), ids, k > 0);
+        }
+        tca_commit(&bars.s_full[w]);
+      };
+      auto outputs = [&](int w, int j) {
+        const uint32_t va = v_u + (j & 1) * C::kTile;
+#pragma unroll
+        for (int k = 0; k < kTcKeys / 16; ++k)
+          tca_mma_ts(tmem + 256 + HDP * w, tmem + 128 * w + 8 * k, tca_desc(va + k * 2048, C::kHalf), ido,
+                     j > 0 || k > 0);
+      };
+      bool ok = wait(Q8 ? &bars.q_ready : &bars.q_full, 0);
+      ok = ok && wait(&bars.k_full[0], 0);
+      if (ok) {
+        tca_after();
+        scores(0, 0);
+        scores(1, 0);
+        tca_commit(&bars.k_empty[0]);
+      }
+      for (int j = 0; j < nj && ok; ++j) {
+#pragma unroll 1
+        for (int w = 0; w < 2 && ok; ++w) {
+          if (w == 0) {
+            ok = wait(Q8 ? &bars.v_full[j & 1] : &bars.v_clean[j & 1], j >> 1);
+          }
+          ok = ok && wait(&bars.p_full[w], j);
+          if (!ok) break;
+          tca_after();
+          outputs(w, j);
+          if (w == 1) tca_commit(&bars.v_empty[j & 1]);
+          if (j + 1 < nj) {
+            if (w == 0 && !(ok = wait(&bars.k_full[(j + 1) & 1], (j + 1) >> 1))) break;
+            tca_after();
+            scores(w, j + 1);
+            if (w == 1) tca_commit(&bars.k_empty[(j + 1) & 1]);
+          } else {
+            tca_commit(&bars.o_full[w]);
+          }
+        }
+      }
+      if (!ok) {
+        // the MMAs issued so far finish before shared and tensor memory are given up
+        tca_commit(&bars.drain);
+        mbar_wait_bounded(&bars.drain, 0, kTcWaitNs);
+      }
+    }
+    __syncwarp();
+    tca_before();
+  } else if (warp < 12) {
+    if (warp == 9) {
+      // ----------------------------------------------------------- loads
+      if (lane == 0 && nj > 0) {
+        mbar_arrive_expect_tx(&bars.q_full, 2 * C::kBoxes * P.rt * 128);
+        const int tok = tile.start + tile.row0 / a.group;
+        for (int w = 0; w < 2; ++w)
+          for (int b = 0; b < C::kBoxes; ++b)
+            tca_load_3d(q_s + w * C::kTile + b * C::kHalf, &P.qmap, 64 * b, kvh * a.group,
+                        tok + w * (P.rt / a.group), &bars.q_full);
+      }
+      if constexpr (!Q8) {
+        // lane i holds the page of the tile's i-th box
+        const int per = kTcKeys / P.box_rows;
+        bool ok = true;
+        int j = 0;
+        for (; j < nj; ++j) {
+          const int st = j & 1, k0 = kbeg + j * kTcKeys;
+          const int key = k0 + lane * P.box_rows;
+          int row = P.page_rows;  // past the end: zeros
+          if (lane < per && key < kfin) {
+            const int page = page_of(a.c, tile.s, key);
+            if (page >= 0)
+              row = ((page * a.c.kv_heads + kvh) << a.c.page_shift) + (key & ((1 << a.c.page_shift) - 1));
+          }
+          if (j >= 2) ok = wait_warp(&bars.k_empty[st], (j >> 1) - 1);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&bars.k_full[st], C::kTile);
+          __syncwarp();
+          if (lane < per)
+            for (int b = 0; b < C::kBoxes; ++b)
+              tca_load_2d(k_s + st * C::kTile + b * C::kHalf + lane * P.box_rows * 128, &P.kmap, 64 * b, row,
+                          &bars.k_full[st]);
+          if (j >= 2) ok = wait_warp(&bars.v_empty[st], (j >> 1) - 1);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&bars.v_full[st], C::kTile);
+          __syncwarp();
+          if (lane < per)
+            for (int b = 0; b < C::kBoxes; ++b)
+              tca_load_2d(v_s + st * C::kTile + b * C::kHalf + lane * P.box_rows * 128, &P.vmap, 64 * b, row,
+                          &bars.v_full[st]);
+        }
+        if (!ok && lane == 0) {  // copies in flight land before the CTA leaves
+          for (int jj = max(0, j - 1); jj <= j; ++jj) {
+            mbar_wait_bounded(&bars.k_full[jj & 1], (jj >> 1) & 1, kTcWaitNs);
+            if (jj < j) mbar_wait_bounded(&bars.v_full[jj & 1], (jj >> 1) & 1, kTcWaitNs);
+          }
+        }
+      }
+      __syncwarp();
+    } else if constexpr (!Q8) {
+      // ----------------------------------------------------------- value tiles at the edge
+      bool ok = true;
+      const int t = tid - 320;  // 64 threads: two rows each
+      for (int j = 0; j < nj && ok; ++j) {
+        if (!(ok = wait_warp(&bars.v_full[j & 1], j >> 1))) break;
+        if (j < jedge) {
+          if (lane == 0) mbar_arrive(&bars.v_clean[j & 1]);
+          continue;
+        }
+        const int k0 = kbeg + j * kTcKeys;
+        uint8_t* tile_s = v_s + (j & 1) * C::kTile;
+#pragma unroll 1
+        for (int rr = t; rr < kTcKeys; rr += 64) {
+          bool bad = false;
+#pragma unroll 1
+          for (int c = 0; c < HDP / 8; ++c) {
+            uint4* p = reinterpret_cast<uint4*>(tile_s + (c >> 3) * C::kHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
+            if (k0 + rr >= kfin) {
+              *p = make_uint4(0, 0, 0, 0);
+              continue;
+            }
+            uint4 u = *p;
+            bool hit = false;
+            auto clean = [&](uint32_t& x) {
+              if ((x & 0x7F80u) == 0x7F80u) x &= 0xFFFF0000u, hit = true;
+              if ((x & 0x7F800000u) == 0x7F800000u) x &= 0xFFFFu, hit = true;
+            };
+            clean(u.x), clean(u.y), clean(u.z), clean(u.w);
+            if (hit) *p = u, bad = true;
+          }
+          const int b = (j - jedge) * kTcKeys + rr;
+          if (bad && b < kTcBadWords * 32) atomicOr(&s_bad[b >> 5], 1u << (b & 31));
+        }
+        tca_proxy();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.v_clean[j & 1]);
+      }
+    }
+  } else {
+    // --------------------------------------------------------------- Q8_0 tiles
+    if constexpr (Q8) {
+      const int pt = tid - 384, row = pt & 127, half = pt >> 7;  // a key and 64 (or 32) of its values
+      constexpr int kVals = HDP / 2;             // values of a thread
+      constexpr int kVec = kVals / 16;           // 16-byte loads
+      const int d0 = half * kVals;
+      uint4 qv[kVec];
+      uint32_t sv[kVals / 32];
+      auto fetch = [&](const uint8_t* base, int j) {
+        const int key = kbeg + j * kTcKeys + row;
+        int page = -1;
+        if (j < nj && key < kfin) page = page_of(a.c, tile.s, key);
+        const int off = key & ((1 << a.c.page_shift) - 1);
+        const uint8_t* blk = base + ((int64_t)max(page, 0) * a.c.kv_heads + kvh) * a.c.block_bytes;
+        const uint8_t* sp = blk + ((int64_t)hd << a.c.page_shift);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          const bool on = page >= 0 && d0 + 16 * i < hd;
+          qv[i] = on ? __ldg(reinterpret_cast<const uint4*>(blk + (int64_t)off * hd + d0 + 16 * i))
+                     : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < kVals / 32; ++i) {
+          const bool on = page >= 0 && d0 + 32 * i < hd;
+          sv[i] = on ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(sp) + off * (hd / 32) + (d0 >> 5) + i) : 0u;
+        }
+      };
+      auto put = [&](uint8_t* tile_s) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          const uint32_t d = (sv[i / 2] & 0xFFFFu) * 0x10001u;
+          const __half2 d2 = *reinterpret_cast<const __half2*>(&d);
+          const uint32_t ws[4] = {qv[i].x ^ 0x80808080u, qv[i].y ^ 0x80808080u, qv[i].z ^ 0x80808080u,
+                                  qv[i].w ^ 0x80808080u};
+          uint32_t o[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t x = __byte_perm(ws[e >> 1], 0x64646464u, (e & 1) ? 0x4342 : 0x4140), c = 0x64806480u;
+            const __half2 h = __hmul2_rn(__hsub2_rn(*reinterpret_cast<const __half2*>(&x),
+                                                    *reinterpret_cast<const __half2*>(&c)), d2);
+            o[e] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          const int dd = d0 + 16 * i, c = (dd >> 3) & 7;
+          uint8_t* base = tile_s + (dd >> 6) * C::kHalf + row * 128;
+          *reinterpret_cast<uint4*>(base + ((c ^ (row & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(base + (((c + 1) ^ (row & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+      };
+      bool ok = true;
+      fetch(a.c.k, 0);
+      for (int j = 0; j < nj && ok; ++j) {
+        const int st = j & 1;
+        if (j >= 2 && !(ok = wait_warp(&bars.k_empty[st], (j >> 1) - 1))) break;
+        put(k_s + st * C::kTile);
+        fetch(a.c.v, j);
+        tca_proxy();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.k_full[st]);
+        if (j >= 2 && !(ok = wait_warp(&bars.v_empty[st], (j >> 1) - 1))) break;
+        if (j >= jedge) {
+          bool bad = false;
+#pragma unroll
+          for (int i = 0; i < kVals / 32; ++i)
+            if ((sv[i] & 0x7C00u) == 0x7C00u) sv[i] = 0, bad = true;
+          const int b = (j - jedge) * kTcKeys + row;
+          if (bad && b < kTcBadWords * 32) atomicOr(&s_bad[b >> 5], 1u << (b & 31));
+        }
+        put(v_s + st * C::kTile);
+        fetch(a.c.k, j + 1);
+        tca_proxy();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.v_full[st]);
+      }
+    }
+  }
+  __syncthreads();
+  if (s_abort && tid == 0) {
+    atomicExch(P.status, DRACO_ERR_TIMEOUT);
+    if (nj > 0) mbar_wait_bounded(&bars.q_full, 0, kTcWaitNs);
+  }
+  if (warp == 8) {
+    tca_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+static PFN_cuTensorMapEncodeTiled_v12000 tc_encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  if (!fn) {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }
+  return fn;
+}
+
+bool paged_attn_tc_takes(const PagedView& c, int hd, int dtype, int group, int page_size) {
+  if (dtype != DRACO_DTYPE_BF16 || hd > 128 || group > kTcRows) return false;
+  // TMA row coordinates are 32-bit
+  return c.type == DRACO_KV_Q8_0 || (int64_t)c.n_pages * c.kv_heads * page_size < 0x7FFFFF00ll;
+}
+
+TcPlan paged_attn_tc_plan(int n, int n_seqs, int group, int kv_heads, int hd, int max_kv) {
+  TcPlan p;
+  p.rt = group * (kTcRows / group);
+  p.tiles = (int64_t)n * group / (2 * p.rt) + n_seqs;
+  p.units = p.tiles * kv_heads;
+  // One CTA per SM: when the row tiles leave SMs idle, as many splits as fit
+  // one wave.  A split's partial rows cost a round trip through the L2, so a
+  // second wave of splits never pays.
+  const int64_t full = (int64_t)n * group / (2 * p.rt) * kv_heads;  // tiles that surely have rows
+  int64_t s = full > 0 ? device_sm_count() / full : 1;
+  s = std::min<int64_t>(s, ((int64_t)max_kv + 4 * kTcKeys - 1) / (4 * kTcKeys));
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(s, 32));
+  if (p.units > kPagedCounters) p.splits = 1;
+  p.bytes = p.splits > 1 ? (size_t)p.units * p.splits * (2 * p.rt) * (hd + 2) * sizeof(float) : 0;
+  return p;
+}
+
+template <int HDP, bool Q8>
+static cudaError_t tc_launch(const TcParams& P, const TcPlan& p, cudaStream_t st) {
+  using C = TcCfg<HDP, Q8>;
+  static int attr_set[64] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !attr_set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(paged_attn_tc_kernel<HDP, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         C::kSmem);
+    if (e != cudaSuccess) return e;
+    // the warpgroups' register counts are drawn from the block's: with fewer
+    // registers than that the increase would wait for good
+    cudaFuncAttributes fa;
+    e = cudaFuncGetAttributes(&fa, paged_attn_tc_kernel<HDP, Q8>);
+    if (e != cudaSuccess) return e;
+    if (fa.numRegs * C::kThreads < C::kRegsBlock) return cudaErrorInvalidConfiguration;
+    if (dev < 64) attr_set[dev] = 1;
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)p.tiles, (unsigned)p.splits, (unsigned)P.a.c.kv_heads);
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_attn_tc_kernel<HDP, Q8>, P);
+}
+
+int paged_attn_tc_launch(const PagedAttnArgs& a, int hd, const TcPlan& p, int* status, cudaStream_t st, char* msg,
+                         size_t ml) {
+  auto enc = tc_encode_fn();
+  if (!enc) {
+    snprintf(msg, ml, "attention_paged: cuTensorMapEncodeTiled unavailable");
+    return DRACO_ERR_CUDA;
+  }
+  TcParams P;
+  P.a = a;
+  P.a.n_splits = p.splits;
+  P.rt = p.rt;
+  P.hd = hd;
+  P.status = status;
+  const int page_size = 1 << a.c.page_shift;
+  P.box_rows = std::min(page_size, kTcKeys);
+  const bool q8 = a.c.type == DRACO_KV_Q8_0;
+  // q [n][heads][hd]: 64 values x the group's heads x the tile's tokens
+  cuuint64_t qdim[3] = {(cuuint64_t)hd, (cuuint64_t)a.heads, (cuuint64_t)a.n};
+  cuuint64_t qstr[2] = {(cuuint64_t)hd * 2, (cuuint64_t)a.ldq * 2};
+  cuuint32_t qbox[3] = {64, (cuuint32_t)a.group, (cuuint32_t)(p.rt / a.group)};
+  cuuint32_t one[3] = {1, 1, 1};
+  CUresult r = enc(&P.qmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a.q), qdim, qstr, qbox, one,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  P.page_rows = 0;
+  if (!q8 && r == CUDA_SUCCESS) {
+    P.page_rows = a.c.n_pages * a.c.kv_heads * page_size;
+    cuuint64_t dim[2] = {(cuuint64_t)hd, (cuuint64_t)P.page_rows};
+    cuuint64_t str[1] = {(cuuint64_t)hd * 2};
+    cuuint32_t box[2] = {64, (cuuint32_t)P.box_rows};
+    for (int i = 0; i < 2 && r == CUDA_SUCCESS; ++i)
+      r = enc(i ? &P.vmap : &P.kmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, i ? a.c.v : a.c.k, dim, str, box, one,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  } else {
+    P.kmap = P.qmap;
+    P.vmap = P.qmap;
+  }
+  if (r != CUDA_SUCCESS) {
+    snprintf(msg, ml, "attention_paged: cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return DRACO_ERR_ARG;
+  }
+  const cudaError_t e = hd <= 64 ? (q8 ? tc_launch<64, true>(P, p, st) : tc_launch<64, false>(P, p, st))
+                                 : (q8 ? tc_launch<128, true>(P, p, st) : tc_launch<128, false>(P, p, st));
+  if (e != cudaSuccess) {
+    snprintf(msg, ml, "attention_paged launch failed: %s", cudaGetErrorString(e));
+    return DRACO_ERR_CUDA;
+  }
+  return DRACO_OK;
+}
+
+}  // namespace draco
