@@ -8,24 +8,34 @@
 // and sum l, O rescaled when m grows (by more than 8 in the exponent's log2:
 // up to there the old reference only makes the summands larger).
 //
-// What bounds it: few rows share a key, so bytes: every key and value is read
-// once per row tile.  The query heads of a key/value head and the new tokens
-// are the rows of one MMA (m16n8k16), so that a key's fragment serves all of
-// them, and the keys go through 16 at a time: a group of WM warps (one row tile
-// of 16 rows each) fills its own ring of 16 * WM keys per stage with
-// cp.async and never waits for the other groups.  4 / WM groups of a CTA take
-// the key blocks of the CTA's key range in turn and merge in shared memory;
-// long ranges are split over CTAs (blockIdx.y) and merged, in split order, by
-// the last CTA to arrive.
+// What bounds it: few rows share a key, so bytes, and for Q8_0 the conversion
+// of its quants.  Both products have the keys (and values) as the MMA's A
+// operand and the rows as its 8-column B operand, S^T = K Q^T and O^T = V^T
+// P^T (m16n8k16): a decode step's rows (the heads of a group) fill 8 columns
+// where they would leave 16 rows half empty, S and O take half the registers,
+// and a converted fragment serves all NN column tiles of the warp.  P^T comes
+// out of the first product as a C fragment and goes into the second as a B
+// fragment through two 8x8 transposes (movmatrix).
+// A warp takes the 16-key blocks of the CTA's key range in turn with the three
+// others, fills its own ring with cp.async and waits for nobody; the warps
+// merge in shared memory.  Long ranges are split over CTAs (blockIdx.y) and
+// merged, in split order, by the last CTA to arrive.
 //
 // Precision.  fp32 activations keep 22-24 bits: operands go into the MMAs as
-// sums of 16-bit terms.
+// sums of 16-bit terms, and products go through accumulators of their own of
+// at most 32 dims or 16 keys, added in fp32 (the tensor core's accumulation
+// truncates).
 //   bf16 cache: keys and values are bf16 already.  q and P are one bf16 each
 //     for bf16 activations, or three (8 + 8 + 8 bits) for fp32.
-//   Q8_0 cache: d * quant has 18 bits, and fp16 takes 11 of them: one fp16 for
-//     bf16 activations (relative error 2^-12, against 2^-9 of the output), or
-//     two, exact, for fp32, with q and P as two fp16 (22 bits) and the
-//     smallest cross product left out.  A row of q is scaled by a power of
+//   Q8_0 cache, keys: the quants are exact in fp16; the products of a block of
+//     32 are scaled by its scale in fp32.  A byte quant + 128 in the low half
+//     of a word is the fp16 subnormal (quant + 128) 2^-24, as it stands; the
+//     2^24 goes into the row's scale, the 128 sum(q) into the accumulator's
+//     start (fp32 activations subtract it beforehand, exactly).
+//     Values: scale * quant has 18 bits, and fp16 takes 11 of them: one fp16 for
+//     bf16 activations (relative error 2^-11, against 2^-8 of the output), or
+//     two, exact, for fp32.  q and P are one fp16, or two (22 bits); the
+//     smallest cross product is left out.  A row of q is scaled by a power of
 //     two to at most 1 and P to at most 2^14, so that fp16's range does not cut
 //     either.
 // m, l, O and the scores are fp32.
@@ -33,7 +43,7 @@
 // A key or value outside [0, kv_len) and a row of a page outside the cache is
 // zero-filled in shared memory, never read.  A NaN or infinity in a value row
 // that some rows of the tile do not see (a later token of the same chunk)
-// must not reach them as 0 * NaN: such a step multiplies row by row.
+// must not reach them as 0 * NaN: such a step multiplies key by key.
 #include <algorithm>
 #include <cstdio>
 
@@ -44,7 +54,7 @@ namespace draco {
 
 constexpr int kPaThreads = 128;
 constexpr float kPaLazy = 8.f;
-constexpr int kPaMinSplit = 256;   // keys of a split at least (16 blocks per warp group at WM 1)
+constexpr int kPaMinSplit = 256;  // keys of a split at least: 4 blocks of each warp
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;  // 0: the 16 bytes are filled with zeros and src is not read
@@ -93,6 +103,11 @@ __device__ __forceinline__ uint32_t hsub2_(uint32_t a, uint32_t b) {
   const __half2 r = __hsub2_rn(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 // a * b - c
 __device__ __forceinline__ uint32_t hfms2_(uint32_t a, uint32_t b, uint32_t c) {
   const __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b),
@@ -121,59 +136,63 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t (&t)[NT]) {
 // ---------------------------------------------------------------------------
 // geometry
 // ---------------------------------------------------------------------------
-template <int HD, bool Q8, bool F32, int WM>
+template <int HD, bool Q8, bool F32, int NN>
 struct PaCfg {
   static constexpr int kTerms = F32 ? (Q8 ? 2 : 3) : 1;   // 16-bit terms of q and P
-  static constexpr int kGroups = 4 / WM;                  // warp groups of the CTA
-  static constexpr int kKeys = 16 * WM;                   // keys of a stage
-  static constexpr int kRowsTile = 16 * WM;
+  static constexpr int kRows = 8 * NN;                    // rows of a tile
+  static constexpr int kWarps = kPaThreads / 32;
   static constexpr int kRowBytes = Q8 ? HD : HD * 2;
   // row strides in shared memory without bank conflicts: ldmatrix wants the 8
   // rows of a matrix 16 bytes apart (mod 128), the Q8_0 loads want 4 rows 32
   // or 96 bytes apart
   static constexpr int kStride = Q8 ? HD + (HD % 64 == 0 ? 32 : 0) : HD * 2 + 16;
-  static constexpr int kScale = Q8 ? HD / 16 : 0;         // scale bytes of a row
-  static constexpr int kTile = kKeys * (kStride + kScale);  // keys, or values, of a stage
+  static constexpr int kScale = Q8 ? HD / 16 : 0;           // scale bytes of a row
+  static constexpr int kTile = 16 * (kStride + kScale);     // 16 keys, or values
   static constexpr int kStage = 2 * kTile;
-  static constexpr int kQBytes = kTerms * (HD / 16) * 32 * 16 * WM;
-  static constexpr int kMerge = kGroups * kRowsTile * HD * 4;  // partial O of the groups
+  static constexpr int kQBytes = kTerms * (HD / 32) * NN * 512;
+  static constexpr int kInit = Q8 && !F32 ? (HD / 32) * kRows * 4 : 0;  // -128 sum(q) of every block
+  static constexpr int kHead = kQBytes + kInit;
+  static constexpr int kMerge = kWarps * kRows * HD * 4;    // partial O of the warps
+  // three CTAs per SM for Q8_0, whose warps compute, two for bf16, whose
+  // stages are larger, where that leaves two stages
   static constexpr int stages() {
-    int s = (104 * 1024 - kQBytes) / (kStage * kGroups);  // two CTAs per SM where that leaves two stages
+    int s = ((Q8 ? 74 : 110) * 1024 - kHead) / (kStage * kWarps);
     return s < 2 ? 2 : s > 6 ? 6 : s;
   }
   static constexpr int kStages = stages();
-  static constexpr int kRing = kStages * kStage * kGroups;
-  static constexpr int smem() { return kQBytes + (kRing > kMerge ? kRing : kMerge); }
-  static_assert(kRowBytes % 16 == 0 && kStride % 16 == 0 && (kKeys * kScale) % 16 == 0, "16-byte copies");
+  static constexpr int kRing = kStages * kStage * kWarps;
+  static constexpr int smem() { return kHead + (kRing > kMerge ? kRing : kMerge); }
+  static_assert(kRowBytes % 16 == 0 && kStride % 16 == 0 && (16 * kScale) % 16 == 0, "16-byte copies");
+  static_assert(smem() <= 220 * 1024, "shared memory");
 };
 
-// the key (0..7) of an 8-key MMA tile behind the tile's column n: for Q8_0 an
-// order in which both the key loads (lanes n = 0..3 and 4..7 together) and the
-// value loads (n even, n odd) touch rows that differ mod 4
+// the key (0..7) behind row n of an 8-key MMA half: for Q8_0 an order in which
+// both the key loads (rows 0..3 and 4..7 together) and the value loads (n even,
+// n odd) touch rows that differ mod 4
 template <bool Q8>
-__device__ __forceinline__ int key_of_col(int n) {
+__device__ __forceinline__ int key_of(int n) {
   if constexpr (!Q8) return n;
   return (0x57463120 >> (4 * n)) & 0xF;
 }
 
-template <int HD, bool Q8, bool F32, int WM>
+template <int HD, bool Q8, bool F32, int NN>
 __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
-  using C = PaCfg<HD, Q8, F32, WM>;
+  using C = PaCfg<HD, Q8, F32, NN>;
   using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
-  constexpr int NT = C::kTerms, KS = C::kStride;
+  constexpr int NT = C::kTerms, KS = C::kStride, NB = HD / 32, W = C::kWarps;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float row_scale[C::kRowsTile];
-  __shared__ float gm[C::kGroups][C::kRowsTile], gl[C::kGroups][C::kRowsTile];
+  __shared__ float row_scale[C::kRows];
+  __shared__ float gm[W][C::kRows], gl[W][C::kRows];
   __shared__ int last_flag;
   grid_dependency_wait();
   grid_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   // the last tiles of a prompt see the most keys: they start first
   const int tile_id = gridDim.x - 1 - blockIdx.x;
-  const RowTile tile = find_tile(a, tile_id, C::kRowsTile);
+  const RowTile tile = find_tile(a, tile_id, C::kRows);
   if (tile.s < 0) return;
   const int kvh = blockIdx.z;
-  const int rows = min(C::kRowsTile, tile.rows - tile.row0);
+  const int rows = min(C::kRows, tile.rows - tile.row0);
   // keys that the tile's last row sees, and this CTA's share of them
   const int kend = max(0, min(tile.kv, row_limit(a, tile, tile.row0 + rows - 1)));
   int ck = (kend + a.n_splits - 1) / a.n_splits;
@@ -183,47 +202,37 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
   if (split >= active) return;
   const int kbeg = split * ck, kfin = min(kend, kbeg + ck);
 
-  const int grp = warp / WM, wrow = (warp % WM) * 16, gt = tid % (32 * WM);
-  uint8_t* ring = smem + C::kQBytes + grp * (C::kStages * C::kStage);
+  // --- the warp's ring: 16-key blocks, warp w takes every W-th (a block lies in one page)
+  uint8_t* ring = smem + C::kHead + warp * (C::kStages * C::kStage);
   const uint32_t ring_u = smem_u32(ring);
-
-  // --- the group's loader: blocks of kKeys keys, group `grp` takes every kGroups-th
-  const int n_blocks = (kfin - kbeg + C::kKeys - 1) / C::kKeys;
-  const int my_blocks = n_blocks > grp ? (n_blocks - grp + C::kGroups - 1) / C::kGroups : 0;
-  auto block_page = [&](int b) -> int {  // lane j < WM: the page of the block's j-th 16 keys
-    const int key = kbeg + (grp + b * C::kGroups) * C::kKeys + 16 * (lane % WM);
-    return b < my_blocks && key < kfin ? page_of(a.c, tile.s, key) : -1;
-  };
-  auto load_block = [&](int b, int stage, int page_l) {
-    const int key0 = kbeg + (grp + b * C::kGroups) * C::kKeys;
-    constexpr int CPR = C::kRowBytes / 16;                 // 16-byte chunks of a row
-    constexpr int N = C::kKeys * CPR / (32 * WM);          // chunks of a thread
+  const int n_blocks = (kfin - kbeg + 15) / 16;
+  const int my_blocks = n_blocks > warp ? (n_blocks - warp + W - 1) / W : 0;
+  const int page_mask = (1 << a.c.page_shift) - 1;
+  auto block_key = [&](int b) { return kbeg + (warp + b * W) * 16; };
+  auto block_page = [&](int b) { return b < my_blocks ? page_of(a.c, tile.s, block_key(b)) : -1; };
+  auto load_block = [&](int b, int stage, int page) {
+    constexpr int CPR = C::kRowBytes / 16;  // 16-byte chunks of a row
+    constexpr int N = 16 * CPR / 32;        // chunks of a lane
+    const int key0 = block_key(b);
+    const int have = page >= 0 ? min(16, kfin - key0) : 0;
+    const int64_t at = ((int64_t)max(page, 0) * a.c.kv_heads + kvh) * a.c.block_bytes;
+    const int off = key0 & page_mask;
+    const uint8_t* kp = a.c.k + at + (int64_t)off * C::kRowBytes + 16 * lane;
+    const uint8_t* vp = a.c.v + at + (int64_t)off * C::kRowBytes + 16 * lane;
     const uint32_t dst0 = ring_u + stage * C::kStage;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int idx = i * (32 * WM) + gt, r = idx / CPR, ch = idx % CPR;
-      const int page = __shfl_sync(0xffffffffu, page_l, r >> 4);
-      const int key = key0 + r;
-      const bool on = page >= 0 && key < kfin;
-      const int64_t at = ((int64_t)(on ? page : 0) * a.c.kv_heads + kvh) * a.c.block_bytes +
-                         (int64_t)(on ? key & ((1 << a.c.page_shift) - 1) : 0) * C::kRowBytes + 16 * ch;
-      cp_async16(dst0 + r * KS + 16 * ch, a.c.k + at, on);
-      cp_async16(dst0 + C::kTile + r * KS + 16 * ch, a.c.v + at, on);
+      const int idx = i * 32 + lane, r = idx / CPR, ch = idx % CPR;
+      const uint32_t dst = dst0 + r * KS + 16 * ch;
+      cp_async16(dst, kp + 512 * i, r < have);
+      cp_async16(dst + C::kTile, vp + 512 * i, r < have);
     }
-    if constexpr (Q8) {
-      // scales: 16 keys' are HD / 16 chunks of 16 bytes, contiguous in the page
-      constexpr int SN = WM * (HD / 16);
-      const int sub = gt / (HD / 16), ch = gt % (HD / 16);
-      const int page = __shfl_sync(0xffffffffu, page_l, sub < WM ? sub : 0);
-      if (gt < SN) {
-        const int key = key0 + 16 * sub;
-        const bool on = page >= 0 && key < kfin;
-        const int64_t at = ((int64_t)(on ? page : 0) * a.c.kv_heads + kvh) * a.c.block_bytes +
-                           ((int64_t)HD << a.c.page_shift) +
-                           (int64_t)(on ? key & ((1 << a.c.page_shift) - 1) : 0) * C::kScale + 16 * ch;
-        const uint32_t d = dst0 + C::kKeys * KS + sub * 16 * C::kScale + 16 * ch;
-        cp_async16(d, a.c.k + at, on);
-        cp_async16(d + C::kTile, a.c.v + at, on);
+    if constexpr (Q8) {  // the scales of 16 keys: HD / 16 chunks, contiguous in the page
+      if (lane < HD / 16) {
+        const int64_t sc = ((int64_t)HD << a.c.page_shift) - (int64_t)off * C::kRowBytes + (int64_t)off * C::kScale;
+        const uint32_t dst = dst0 + 16 * KS + 16 * lane;
+        cp_async16(dst, kp + sc, have > 0);
+        cp_async16(dst + C::kTile, vp + sc, have > 0);
       }
     }
   };
@@ -236,16 +245,16 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     cp_async_commit();
   }
 
-  // --- q as MMA fragments in shared memory: [term][16 dims][row tile][lane]
+  // --- q as B fragments in shared memory: [term][32 dims][column tile][lane] of two MMA steps
   const T* qbase = static_cast<const T*>(a.q);
   auto q_row = [&](int r) -> const T* {  // row r of the tile
     const int rr = tile.row0 + r;
     return qbase + (int64_t)(tile.start + rr / a.group) * a.ldq + (int64_t)(kvh * a.group + rr % a.group) * HD;
   };
   if constexpr (Q8) {  // the row's power-of-two scale
-    constexpr int TPR = kPaThreads / C::kRowsTile;  // 8, 4 or 2 threads of a row
-    const int r = tid / TPR;
+    constexpr int TPR = kPaThreads / C::kRows < 16 ? kPaThreads / C::kRows : 16;  // threads of a row
     float m = 0.f;
+    const int r = tid / TPR;
     if (r < rows) {
       const T* p = q_row(r);
       for (int j = tid % TPR; j < HD / 8; j += TPR) {
@@ -260,277 +269,332 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     // 2^(exponent + 1) > m; rows of zeros, infinities and NaN keep scale 1
     float s = 1.f;
     if (m > 1e-30f && m < 1e38f) s = __int_as_float((__float_as_int(m) & 0x7F800000) + 0x00800000);
-    if (tid % TPR == 0) row_scale[r] = s;
+    if (tid % TPR == 0 && r < C::kRows) row_scale[r] = s;
     __syncthreads();
   }
-  for (int idx = tid; idx < (HD / 16) * WM * 32; idx += kPaThreads) {
-    const int ln = idx & 31, w = (idx >> 5) % WM, step = (idx >> 5) / WM;
-    const int lg = ln >> 2, lt = ln & 3;
-    // the step's dims behind fragment columns (2t, 2t+1) and (2t+8, 2t+9)
-    const int d0 = Q8 ? 32 * (step >> 1) + 8 * lt + 4 * (step & 1) : 16 * step + 2 * lt;
-    const int d1 = Q8 ? d0 + 2 : d0 + 8;
-    uint32_t f[NT][4];
+  float* init = reinterpret_cast<float*>(smem + C::kQBytes);  // [32 dims][row]
+  for (int idx = tid; idx < NB * NN * 32; idx += kPaThreads) {
+    const int ln = idx & 31, nt = (idx >> 5) % NN, blk = (idx >> 5) / NN;
+    const int lg = ln >> 2, lt = ln & 3, r = 8 * nt + lg;
+    // the dims behind (2t, 2t+1) and (2t+8, 2t+9) of the block's two steps
+    float x[8] = {};
+    if (r < rows) {
+      const T* p = q_row(r) + 32 * blk;
+      if constexpr (Q8) {
+        load8(p + 8 * lt, x);
+        const float inv = 1.f / row_scale[r];  // a power of two: exact
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {  // rows lg, lg + 8
-      const int r = 16 * w + lg + 8 * h;
-      float x[4] = {0.f, 0.f, 0.f, 0.f};
-      if (r < rows) {
-        const T* p = q_row(r);
-        if constexpr (F32) {
-          const float2 u = *reinterpret_cast<const float2*>(p + d0), v = *reinterpret_cast<const float2*>(p + d1);
-          x[0] = u.x, x[1] = u.y, x[2] = v.x, x[3] = v.y;
-        } else {
-          const uint32_t u = *reinterpret_cast<const uint32_t*>(p + d0), v = *reinterpret_cast<const uint32_t*>(p + d1);
-          x[0] = bf16lo(u), x[1] = bf16hi(u), x[2] = bf16lo(v), x[3] = bf16hi(v);
-        }
-        if constexpr (Q8) {
-          const float inv = 1.f / row_scale[r];  // a power of two: exact
+        for (int e = 0; e < 8; ++e) x[e] *= inv;
+      } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] *= inv;
+        for (int e = 0; e < 4; ++e) {
+          const int d = 16 * (e >> 1) + 8 * (e & 1) + 2 * lt;
+          if constexpr (F32) {
+            const float2 u = *reinterpret_cast<const float2*>(p + d);
+            x[2 * e] = u.x, x[2 * e + 1] = u.y;
+          } else {
+            const uint32_t u = *reinterpret_cast<const uint32_t*>(p + d);
+            x[2 * e] = bf16lo(u), x[2 * e + 1] = bf16hi(u);
+          }
         }
       }
-      uint32_t lo[NT], hi[NT];
-      split2<Q8, NT>(x[0], x[1], lo);
-      split2<Q8, NT>(x[2], x[3], hi);
-#pragma unroll
-      for (int e = 0; e < NT; ++e) f[e][h] = lo[e], f[e][h + 2] = hi[e];
     }
+    uint32_t f[4][NT];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split2<Q8, NT>(x[2 * e], x[2 * e + 1], f[e]);
 #pragma unroll
     for (int e = 0; e < NT; ++e)
-      *reinterpret_cast<uint4*>(smem + (((e * (HD / 16) + step) * WM + w) * 32 + ln) * 16) =
-          make_uint4(f[e][0], f[e][1], f[e][2], f[e][3]);
+      *reinterpret_cast<uint4*>(smem + (((e * NB + blk) * NN + nt) * 32 + ln) * 16) =
+          make_uint4(f[0][e], f[1][e], f[2][e], f[3][e]);
+    if constexpr (C::kInit > 0) {
+      float q = 0.f;  // of the fp16 values
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 u = __half22float2(*reinterpret_cast<__half2*>(&f[e][0]));
+        q += u.x + u.y;
+      }
+      q += __shfl_xor_sync(0xffffffffu, q, 1);
+      q += __shfl_xor_sync(0xffffffffu, q, 2);
+      if (lt == 0) init[blk * C::kRows + r] = q * (-128.f / 16777216.f);
+    }
   }
   __syncthreads();
 
-  // --- this thread's rows
-  const int r0 = wrow + g, r1 = r0 + 8;
-  const int lim0 = r0 < rows ? min(tile.kv, row_limit(a, tile, tile.row0 + r0)) : 0;
-  const int lim1 = r1 < rows ? min(tile.kv, row_limit(a, tile, tile.row0 + r1)) : 0;
-  const int wfirst = min(tile.kv, row_limit(a, tile, tile.row0 + wrow));  // the warp's first row sees the fewest
-  const int wlast = wrow < rows ? min(tile.kv, row_limit(a, tile, tile.row0 + min(wrow + 15, rows - 1))) : 0;
-  float sc0 = a.scale_log2, sc1 = a.scale_log2;
-  if constexpr (Q8) sc0 *= row_scale[r0], sc1 *= row_scale[r1];
-  const int kc0 = key_of_col<Q8>(2 * t), kc1 = key_of_col<Q8>(2 * t + 1), krow = key_of_col<Q8>(g);
-  constexpr float kShift = Q8 ? 6.f : 0.f;  // fp16 P: 2^6 at the reference, at most 2^14
-  float acc[HD / 8][4];
+  // --- this thread's columns: rows 8 nt + 2t, + 1; its keys: key_of(g), 8 + key_of(g) of a block
+  int lim[NN][2];
+  float sc[NN][2];
+  const int first = min(tile.kv, row_limit(a, tile, tile.row0));  // the first row sees the fewest keys
 #pragma unroll
-  for (int i = 0; i < HD / 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-  // dims of accumulator i behind its columns 2t and 2t + 1
-  auto dim_of = [&](int i, int e) -> int {
-    return Q8 ? 32 * (i >> 2) + 4 * (2 * t + e) + (i & 3) : 8 * i + 2 * t + e;
-  };
+  for (int n = 0; n < NN; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 8 * n + 2 * t + e;
+      // (columns behind the last row hold q = 0 and are not stored)
+      lim[n][e] = min(tile.kv, row_limit(a, tile, tile.row0 + min(r, rows - 1)));
+      sc[n][e] = a.scale_log2;
+      if constexpr (Q8) sc[n][e] *= row_scale[r] * (F32 ? 1.f : 16777216.f);
+    }
+  const int kg = key_of<Q8>(g), kc0 = key_of<Q8>(2 * t), kc1 = key_of<Q8>(2 * t + 1);
+  constexpr float kShift = Q8 ? 6.f : 0.f;  // fp16 P: 2^6 at the reference, at most 2^14
+  float acc[HD / 16][NN][4];
+#pragma unroll
+  for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+    for (int n = 0; n < NN; ++n) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.f;
+  float m[NN][2], l[NN][2];
+#pragma unroll
+  for (int n = 0; n < NN; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
+  // dim behind accumulator i, elements 0/1 (h = 0) or 2/3 (h = 1)
+  auto dim_of = [&](int i, int h) -> int { return Q8 ? 32 * (i >> 1) + 4 * g + 2 * (i & 1) + h : 16 * i + g + 8 * h; };
 
+#pragma unroll 1
   for (int b = 0; b < my_blocks; ++b) {
     cp_async_wait<C::kStages - 2>();
-    if constexpr (WM == 1)
-      __syncwarp();
-    else
-      asm volatile("bar.sync %0, %1;" ::"r"(grp + 1), "n"(32 * WM) : "memory");
-    // the next block into the stage that block b - 1 has left
+    __syncwarp();  // everybody's copies are there, and block b - 1 has been read
     {
       const int nb = b + C::kStages - 1, pg = page_next;
       page_next = block_page(nb + 1);
       if (nb < my_blocks) load_block(nb, nb % C::kStages, pg);
       cp_async_commit();
     }
-    const int key0 = kbeg + (grp + b * C::kGroups) * C::kKeys;
-    const uint8_t* kt = ring + (b % C::kStages) * C::kStage;
-    const uint32_t kt_u = ring_u + (b % C::kStages) * C::kStage;
-#pragma unroll 1
-    for (int u = 0; u < WM; ++u) {  // 16 keys at a time
-      const int k16 = key0 + 16 * u;
-      if (k16 >= kfin || k16 >= wlast) break;
-      const uint8_t* k_s = kt + 16 * u * KS;
-      const uint8_t* v_s = k_s + C::kTile;
-      const uint32_t k_u = kt_u + 16 * u * KS;
-      const uint8_t* ks_s = kt + C::kKeys * KS + 16 * u * C::kScale;  // scales
-      const uint8_t* vs_s = ks_s + C::kTile;
-      if constexpr (Q8) {
-        // scales came 16 keys at a time: those of values past the end become
-        // zero (stale ones may be NaN); their scores are masked
-        if (k16 + 16 > kfin) {
-          for (int j = lane; j < 16 * (HD / 32); j += 32)
-            if (k16 + j / (HD / 32) >= kfin) reinterpret_cast<uint16_t*>(const_cast<uint8_t*>(vs_s))[j] = 0;
-          __syncwarp();
-        }
+    const int k16 = block_key(b);
+    const int at = (b % C::kStages) * C::kStage;
+    const uint8_t* k_s = ring + at;
+    const uint8_t* v_s = k_s + C::kTile;
+    const uint32_t k_u = ring_u + at;
+    const uint8_t* ks_s = k_s + 16 * KS;  // scales
+    const uint8_t* vs_s = ks_s + C::kTile;
+    if constexpr (Q8) {
+      // scales came 16 keys at a time: those of values past the end become
+      // zero (stale ones may be NaN); their scores are masked
+      if (k16 + 16 > kfin) {
+        for (int j = lane; j < 16 * NB; j += 32)
+          if (k16 + j / NB >= kfin) reinterpret_cast<uint16_t*>(const_cast<uint8_t*>(vs_s))[j] = 0;
+        __syncwarp();
       }
-      float s[2][4] = {};
+    }
+    float s[NN][4];
 #pragma unroll
-      for (int kk = 0; kk < HD / 32; ++kk) {
-        uint32_t qf[NT][2][4];
+    for (int n = 0; n < NN; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    // scales of keys g and g + 8, all blocks
+    uint32_t dk[2][(NB + 1) / 2];
+    if constexpr (Q8) {
 #pragma unroll
-        for (int e = 0; e < NT; ++e)
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* p = ks_s + (kg + 8 * h) * C::kScale;
+        if constexpr (NB == 1)
+          dk[h][0] = *reinterpret_cast<const uint16_t*>(p);
+        else if constexpr (NB == 3)
+          dk[h][0] = *reinterpret_cast<const uint16_t*>(p) | ((uint32_t)*reinterpret_cast<const uint16_t*>(p + 2) << 16),
+          dk[h][1] = *reinterpret_cast<const uint16_t*>(p + 4);
+        else
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint4 w = *reinterpret_cast<const uint4*>(
-                smem + (((e * (HD / 16) + 2 * kk + h) * WM + warp % WM) * 32 + lane) * 16);
-            qf[e][h][0] = w.x, qf[e][h][1] = w.y, qf[e][h][2] = w.z, qf[e][h][3] = w.w;
-          }
+          for (int e = 0; e < NB / 2; ++e) dk[h][e] = *reinterpret_cast<const uint32_t*>(p + 4 * e);
+      }
+    }
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          if constexpr (!Q8) {
-            uint32_t kf[4];
-            ldsm4(kf, k_u + (8 * n + (lane & 7)) * KS + (4 * kk + (lane >> 3)) * 16);
+    for (int blk = 0; blk < NB; ++blk) {
+      uint32_t kf[2][4];  // two steps of 16 dims: (key g, key g + 8) x (dims 2t, dims 2t + 8)
+      if constexpr (!Q8) {
+        const uint32_t p = k_u + ((lane & 7) + 8 * ((lane >> 3) & 1)) * KS + (4 * blk + (lane >> 4)) * 16;
+        ldsm4(kf[0], p);
+        ldsm4(kf[1], p + 32);
+      } else {
 #pragma unroll
-            for (int e = 0; e < NT; ++e) {
-              mma_acc<Q8>(s[n], qf[e][0], kf[0], kf[1]);
-              mma_acc<Q8>(s[n], qf[e][1], kf[2], kf[3]);
-            }
-          } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(k_s + (8 * n + krow) * KS + 32 * kk + 8 * t);
-            const uint32_t d1 = *reinterpret_cast<const uint16_t*>(ks_s + (8 * n + krow) * C::kScale + 2 * kk);
-            const uint32_t dd = d1 * 0x10001u;
-            uint32_t hi[4], lo[4];
+        for (int h = 0; h < 2; ++h) {
+          const uint2 w = *reinterpret_cast<const uint2*>(k_s + (kg + 8 * h) * KS + 32 * blk + 8 * t);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t x = (h ? w.y : w.x) ^ 0x80808080u;  // quant + 128
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                // fp16 1024 + byte, minus 1152: the quant
-                const uint32_t i2 = hsub2_(__byte_perm(x, 0x64646464u, j ? 0x4342 : 0x4140), 0x64806480u);
-                hi[2 * h + j] = hmul2_(i2, dd);
-                if constexpr (F32) lo[2 * h + j] = hfms2_(i2, dd, hi[2 * h + j]);
-              }
-            }
-            mma_acc<Q8>(s[n], qf[0][0], hi[0], hi[1]);
-            mma_acc<Q8>(s[n], qf[0][1], hi[2], hi[3]);
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t x = (e ? w.y : w.x) ^ 0x80808080u;  // quant + 128
             if constexpr (F32) {
-              mma_acc<Q8>(s[n], qf[1][0], hi[0], hi[1]);
-              mma_acc<Q8>(s[n], qf[1][1], hi[2], hi[3]);
-              mma_acc<Q8>(s[n], qf[0][0], lo[0], lo[1]);
-              mma_acc<Q8>(s[n], qf[0][1], lo[2], lo[3]);
+              // fp16 1024 + byte, minus 1152: the quant
+              kf[e][h] = hsub2_(__byte_perm(x, 0x64646464u, 0x4140), 0x64806480u);
+              kf[e][h + 2] = hsub2_(__byte_perm(x, 0x64646464u, 0x4342), 0x64806480u);
+            } else {
+              kf[e][h] = __byte_perm(x, 0u, 0x4140);
+              kf[e][h + 2] = __byte_perm(x, 0u, 0x4342);
             }
           }
         }
       }
-      // scores in log2, masked
-      const bool edge = k16 + 16 > wfirst;
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        s[n][0] *= sc0, s[n][1] *= sc0, s[n][2] *= sc1, s[n][3] *= sc1;
-        if (edge) {
-          const int ka = k16 + 8 * n + kc0, kb = k16 + 8 * n + kc1;
-          if (ka >= lim0) s[n][0] = -INFINITY;
-          if (kb >= lim0) s[n][1] = -INFINITY;
-          if (ka >= lim1) s[n][2] = -INFINITY;
-          if (kb >= lim1) s[n][3] = -INFINITY;
-        }
+      float d0 = 1.f, d1 = 1.f;
+      if constexpr (Q8) {
+        d0 = f16_bits_to_f32(dk[0][blk / 2] >> (16 * (blk & 1)));
+        d1 = f16_bits_to_f32(dk[1][blk / 2] >> (16 * (blk & 1)));
       }
-      float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-      float x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-      if (__any_sync(0xffffffffu, x0 > m0 + kPaLazy || x1 > m1 + kPaLazy)) {
 #pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-          x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
-          x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
-        }
-        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-        const float f0 = n0 == -INFINITY ? 1.f : fast_exp2(m0 - n0), f1 = n1 == -INFINITY ? 1.f : fast_exp2(m1 - n1);
-        m0 = n0, m1 = n1, l0 *= f0, l1 *= f1;
-#pragma unroll
-        for (int i = 0; i < HD / 8; ++i) acc[i][0] *= f0, acc[i][1] *= f0, acc[i][2] *= f1, acc[i][3] *= f1;
-      }
-      const float ref0 = m0 == -INFINITY ? 0.f : m0 - kShift, ref1 = m1 == -INFINITY ? 0.f : m1 - kShift;
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        s[n][0] = fast_exp2(s[n][0] - ref0), s[n][1] = fast_exp2(s[n][1] - ref0);
-        s[n][2] = fast_exp2(s[n][2] - ref1), s[n][3] = fast_exp2(s[n][3] - ref1);
-        l0 += s[n][0] + s[n][1], l1 += s[n][2] + s[n][3];
-      }
-      if (edge) {
-        // values that are not finite and that some rows of the warp do not see
-        bool bad = false;
-        if constexpr (Q8) {
-          for (int j = lane; j < 16 * (HD / 32); j += 32)
-            bad |= (reinterpret_cast<const uint16_t*>(vs_s)[j] & 0x7C00u) == 0x7C00u;
+      for (int n = 0; n < NN; ++n) {
+        if constexpr (!Q8 && !F32) {
+          const uint4 w = *reinterpret_cast<const uint4*>(smem + ((blk * NN + n) * 32 + lane) * 16);
+          mma_acc<Q8>(s[n], kf[0], w.x, w.y);
+          mma_acc<Q8>(s[n], kf[1], w.z, w.w);
         } else {
-          for (int j = lane; j < 16 * (HD / 2); j += 32) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(v_s + (j / (HD / 2)) * KS + 4 * (j % (HD / 2)));
-            bad |= (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+          float u[4] = {0.f, 0.f, 0.f, 0.f};
+          if constexpr (C::kInit > 0) {
+            const float2 i2 = *reinterpret_cast<const float2*>(init + blk * C::kRows + 8 * n + 2 * t);
+            u[0] = u[2] = i2.x, u[1] = u[3] = i2.y;
+          }
+#pragma unroll
+          for (int e = NT - 1; e >= 0; --e) {  // the smallest terms first
+            const uint4 w = *reinterpret_cast<const uint4*>(smem + (((e * NB + blk) * NN + n) * 32 + lane) * 16);
+            mma_acc<Q8>(u, kf[0], w.x, w.y);
+            mma_acc<Q8>(u, kf[1], w.z, w.w);
+          }
+          if constexpr (Q8) {
+            s[n][0] = fmaf(u[0], d0, s[n][0]), s[n][1] = fmaf(u[1], d0, s[n][1]);
+            s[n][2] = fmaf(u[2], d1, s[n][2]), s[n][3] = fmaf(u[3], d1, s[n][3]);
+          } else {
+            s[n][0] += u[0], s[n][1] += u[1], s[n][2] += u[2], s[n][3] += u[3];
           }
         }
-        if (__any_sync(0xffffffffu, bad)) {
+      }
+    }
+    const bool edge = k16 + 16 > first;
+    bool grow = false;
+#pragma unroll
+    for (int n = 0; n < NN; ++n) {
+      if (edge) {
+        const int ka = k16 + kg, kb = ka + 8;
+        if (ka >= lim[n][0]) s[n][0] = -INFINITY;
+        if (ka >= lim[n][1]) s[n][1] = -INFINITY;
+        if (kb >= lim[n][0]) s[n][2] = -INFINITY;
+        if (kb >= lim[n][1]) s[n][3] = -INFINITY;
+      }
+      grow |= fmaxf(s[n][0], s[n][2]) * sc[n][0] > m[n][0] + kPaLazy;
+      grow |= fmaxf(s[n][1], s[n][3]) * sc[n][1] > m[n][1] + kPaLazy;
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int n = 0; n < NN; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(s[n][e], s[n][e + 2]) * sc[n][e];
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          const float nm = fmaxf(m[n][e], x);
+          const float f = nm == -INFINITY ? 1.f : fast_exp2(m[n][e] - nm);
+          m[n][e] = nm, l[n][e] *= f;
+#pragma unroll
+          for (int i = 0; i < HD / 16; ++i) acc[i][n][e] *= f, acc[i][n][e + 2] *= f;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NN; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float ref = m[n][e] == -INFINITY ? 0.f : m[n][e] - kShift;
+        s[n][e] = fast_exp2(fmaf(s[n][e], sc[n][e], -ref));
+        s[n][e + 2] = fast_exp2(fmaf(s[n][e + 2], sc[n][e], -ref));
+        l[n][e] += s[n][e] + s[n][e + 2];
+      }
+    if (edge) {
+      // values that are not finite and that some rows of the tile do not see
+      bool bad = false;
+      if constexpr (Q8) {
+        for (int j = lane; j < 16 * NB; j += 32)
+          bad |= (reinterpret_cast<const uint16_t*>(vs_s)[j] & 0x7C00u) == 0x7C00u;
+      } else {
+        for (int j = lane; j < 16 * (HD / 2); j += 32) {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(v_s + (j / (HD / 2)) * KS + 4 * (j % (HD / 2)));
+          bad |= (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+        }
+      }
+      if (__any_sync(0xffffffffu, bad)) {
 #pragma unroll 1
-          for (int j = 0; j < 16; ++j) {
-            // P of key j: column c of tile j / 8, held by lane c / 2 of the quad
-            int c = 0;
-            for (int n = 0; n < 8; ++n)
-              if (key_of_col<Q8>(n) == (j & 7)) c = n;
-            const int src = (lane & ~3) | (c >> 1);
-            const float pa = j < 8 ? (c & 1 ? s[0][1] : s[0][0]) : (c & 1 ? s[1][1] : s[1][0]);
-            const float pb = j < 8 ? (c & 1 ? s[0][3] : s[0][2]) : (c & 1 ? s[1][3] : s[1][2]);
-            const float p0 = __shfl_sync(0xffffffffu, pa, src), p1 = __shfl_sync(0xffffffffu, pb, src);
-            const bool on0 = k16 + j < lim0, on1 = k16 + j < lim1;
+        for (int j = 0; j < 16; ++j) {
+          int src = 0;  // the quad that holds P of key j
+          for (int n = 0; n < 8; ++n)
+            if (key_of<Q8>(n) == (j & 7)) src = n;
+          src = 4 * src + t;
 #pragma unroll
-            for (int i = 0; i < HD / 8; ++i)
+          for (int n = 0; n < NN; ++n) {
+            const float p0 = __shfl_sync(0xffffffffu, j < 8 ? s[n][0] : s[n][2], src);
+            const float p1 = __shfl_sync(0xffffffffu, j < 8 ? s[n][1] : s[n][3], src);
+            const bool on0 = k16 + j < lim[n][0], on1 = k16 + j < lim[n][1];
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int d = dim_of(i, e);
+            for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int d = dim_of(i, h);
                 float v;
                 if constexpr (Q8)
                   v = __half2float(reinterpret_cast<const __half*>(vs_s + j * C::kScale)[d >> 5]) *
                       (float)reinterpret_cast<const int8_t*>(v_s + j * KS)[d];
                 else
                   v = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(v_s + j * KS)[d]);
-                if (on0) acc[i][e] = fmaf(p0, v, acc[i][e]);
-                if (on1) acc[i][e + 2] = fmaf(p1, v, acc[i][e + 2]);
+                if (on0) acc[i][n][2 * h] = fmaf(p0, v, acc[i][n][2 * h]);
+                if (on1) acc[i][n][2 * h + 1] = fmaf(p1, v, acc[i][n][2 * h + 1]);
               }
           }
-          continue;
         }
+        continue;
       }
-      // P as the A operand: (row g, keys of columns 2t, 2t+1), (row g+8, same), then tile 1
-      uint32_t pf[NT][4];
-      {
+    }
+    // P^T as B operands: (keys of rows 2t, 2t+1; column g), (the same + 8)
+    uint32_t pf[NN][NT][2];
+#pragma unroll
+    for (int n = 0; n < NN; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
         uint32_t x[NT];
+        split2<Q8, NT>(s[n][2 * h], s[n][2 * h + 1], x);
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            split2<Q8, NT>(s[n][2 * h], s[n][2 * h + 1], x);
-#pragma unroll
-            for (int e = 0; e < NT; ++e) pf[e][2 * n + h] = x[e];
-          }
+        for (int e = 0; e < NT; ++e) pf[n][e][h] = transpose8x8(x[e]);
       }
-      if constexpr (!Q8) {
+    if constexpr (!Q8) {
 #pragma unroll
-        for (int i = 0; i < HD / 8; i += 2) {
-          uint32_t vf[4];  // dims 8i..8i+7: keys 0-7, 8-15; dims 8i+8..: keys 0-7, 8-15
-          ldsm4t(vf, k_u + C::kTile + (lane & 15) * KS + (8 * i + 8 * (lane >> 4)) * 2);
+      for (int i = 0; i < HD / 16; ++i) {
+        uint32_t vf[4];  // (dim g, dim g + 8) x (keys 2t, keys 2t + 8)
+        ldsm4t(vf, k_u + C::kTile + ((lane & 7) + 8 * (lane >> 4)) * KS + (2 * i + ((lane >> 3) & 1)) * 16);
 #pragma unroll
-          for (int e = 0; e < NT; ++e) {
-            mma_acc<Q8>(acc[i], pf[e], vf[0], vf[1]);
-            mma_acc<Q8>(acc[i + 1], pf[e], vf[2], vf[3]);
+        for (int n = 0; n < NN; ++n) {
+          if constexpr (!F32) {
+            mma_acc<Q8>(acc[i][n], vf, pf[n][0][0], pf[n][0][1]);
+          } else {
+            float u[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = NT - 1; e >= 0; --e) mma_acc<Q8>(u, vf, pf[n][e][0], pf[n][e][1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][n][e] += u[e];
           }
         }
-      } else {
+      }
+    } else {
 #pragma unroll
-        for (int blk = 0; blk < HD / 32; ++blk) {
-          uint32_t hi[2][4], lo[2][4];  // [keys 0-7 / 8-15][dim 4g + j of the block]
+      for (int blk = 0; blk < NB; ++blk) {
+        uint32_t hi[2][4], lo[2][4];  // [keys 2t.. / 2t + 8..][dim 4g + j of the block]
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const int ka = 8 * n + kc0, kb = 8 * n + kc1;
-            const uint32_t wa = *reinterpret_cast<const uint32_t*>(v_s + ka * KS + 32 * blk + 4 * g) ^ 0x80808080u;
-            const uint32_t wb = *reinterpret_cast<const uint32_t*>(v_s + kb * KS + 32 * blk + 4 * g) ^ 0x80808080u;
-            const uint32_t da = *reinterpret_cast<const uint16_t*>(vs_s + ka * C::kScale + 2 * blk);
-            const uint32_t db = *reinterpret_cast<const uint16_t*>(vs_s + kb * C::kScale + 2 * blk);
-            const uint32_t dd = da | (db << 16);
-            const uint32_t ab[2] = {__byte_perm(wa, wb, 0x5140), __byte_perm(wa, wb, 0x7362)};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t i2 =
-                  hsub2_(__byte_perm(ab[j >> 1], 0x64646464u, (j & 1) ? 0x4342 : 0x4140), 0x64806480u);
-              hi[n][j] = hmul2_(i2, dd);
-              if constexpr (F32) lo[n][j] = hfms2_(i2, dd, hi[n][j]);
-            }
-          }
+        for (int h = 0; h < 2; ++h) {
+          const int ka = 8 * h + kc0, kb = 8 * h + kc1;
+          const uint32_t wa = *reinterpret_cast<const uint32_t*>(v_s + ka * KS + 32 * blk + 4 * g) ^ 0x80808080u;
+          const uint32_t wb = *reinterpret_cast<const uint32_t*>(v_s + kb * KS + 32 * blk + 4 * g) ^ 0x80808080u;
+          const uint32_t da = *reinterpret_cast<const uint16_t*>(vs_s + ka * C::kScale + 2 * blk);
+          const uint32_t db = *reinterpret_cast<const uint16_t*>(vs_s + kb * C::kScale + 2 * blk);
+          const uint32_t dd = da | (db << 16);
+          const uint32_t ab[2] = {__byte_perm(wa, wb, 0x5140), __byte_perm(wa, wb, 0x7362)};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            mma_acc<Q8>(acc[4 * blk + j], pf[0], hi[0][j], hi[1][j]);
-            if constexpr (F32) {
-              mma_acc<Q8>(acc[4 * blk + j], pf[NT - 1], hi[0][j], hi[1][j]);
-              mma_acc<Q8>(acc[4 * blk + j], pf[0], lo[0][j], lo[1][j]);
+            const uint32_t i2 = hsub2_(__byte_perm(ab[j >> 1], 0x64646464u, (j & 1) ? 0x4342 : 0x4140), 0x64806480u);
+            hi[h][j] = hmul2_(i2, dd);
+            if constexpr (F32) lo[h][j] = hfms2_(i2, dd, hi[h][j]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t vh[4] = {hi[0][2 * i], hi[0][2 * i + 1], hi[1][2 * i], hi[1][2 * i + 1]};
+#pragma unroll
+          for (int n = 0; n < NN; ++n) {
+            if constexpr (!F32) {
+              mma_acc<Q8>(acc[2 * blk + i][n], vh, pf[n][0][0], pf[n][0][1]);
+            } else {
+              const uint32_t vl[4] = {lo[0][2 * i], lo[0][2 * i + 1], lo[1][2 * i], lo[1][2 * i + 1]};
+              float u[4] = {0.f, 0.f, 0.f, 0.f};
+              mma_acc<Q8>(u, vl, pf[n][0][0], pf[n][0][1]);
+              mma_acc<Q8>(u, vh, pf[n][NT - 1][0], pf[n][NT - 1][1]);
+              mma_acc<Q8>(u, vh, pf[n][0][0], pf[n][0][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[2 * blk + i][n][e] += u[e];
             }
           }
         }
@@ -539,24 +603,36 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
   }
   cp_async_wait<0>();
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, o);
-  }
-  __syncthreads();  // the ring is free: partial O of the groups go over it
-  if (t == 0) gm[grp][r0] = m0, gm[grp][r1] = m1, gl[grp][r0] = l0, gl[grp][r1] = l1;
-  float* part = reinterpret_cast<float*>(smem + C::kQBytes);  // [group][row][HD]
+  for (int n = 0; n < NN; ++n)
 #pragma unroll
-  for (int i = 0; i < HD / 8; ++i)
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
+  __syncthreads();  // the rings are free: partial O of the warps go over them
+  float* part = reinterpret_cast<float*>(smem + C::kHead);  // [warp][row][HD]
+#pragma unroll
+  for (int n = 0; n < NN; ++n) {
+    if (g == 0) {
+      *reinterpret_cast<float2*>(&gm[warp][8 * n + 2 * t]) = make_float2(m[n][0], m[n][1]);
+      *reinterpret_cast<float2*>(&gl[warp][8 * n + 2 * t]) = make_float2(l[n][0], l[n][1]);
+    }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int d = dim_of(i, e);
-      part[(grp * C::kRowsTile + r0) * HD + d] = acc[i][e];
-      part[(grp * C::kRowsTile + r1) * HD + d] = acc[i][e + 2];
+      float* p = part + (warp * C::kRows + 8 * n + 2 * t + e) * HD;
+      if constexpr (Q8) {
+#pragma unroll
+        for (int i = 0; i < HD / 16; i += 2)
+          *reinterpret_cast<float4*>(p + dim_of(i, 0)) =
+              make_float4(acc[i][n][e], acc[i][n][e + 2], acc[i + 1][n][e], acc[i + 1][n][e + 2]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) p[dim_of(i, 0)] = acc[i][n][e], p[dim_of(i, 1)] = acc[i][n][e + 2];
+      }
     }
+  }
   __syncthreads();
-  // merge the groups; one split: normalise and write
-  constexpr int kRec = C::kRowsTile * (HD + 2);
+  // merge the warps; one split: normalise and write
+  constexpr int kRec = C::kRows * (HD + 2);
   const int64_t unit = (int64_t)tile_id * a.c.kv_heads + kvh;
   float* rec = active > 1 ? a.recs + (unit * a.n_splits + split) * kRec : nullptr;
   T* obase = static_cast<T*>(a.out);
@@ -568,14 +644,14 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     const int r = idx / (HD / 8), d = 8 * (idx % (HD / 8));
     float M = gm[0][r], L = 0.f, o[8] = {};
 #pragma unroll
-    for (int w = 1; w < C::kGroups; ++w) M = fmaxf(M, gm[w][r]);
+    for (int w = 1; w < W; ++w) M = fmaxf(M, gm[w][r]);
 #pragma unroll
-    for (int w = 0; w < C::kGroups; ++w) {
+    for (int w = 0; w < W; ++w) {
+      if (gm[w][r] == -INFINITY && gl[w][r] == gl[w][r]) continue;  // no key seen by this warp
       const float f = gm[w][r] == -INFINITY ? 0.f : fast_exp2(gm[w][r] - M);
-      if (gm[w][r] == -INFINITY && !(gl[w][r] != gl[w][r])) continue;  // no key seen by this group
       L = fmaf(f, gl[w][r], L);
-      const float4 p0 = *reinterpret_cast<const float4*>(part + (w * C::kRowsTile + r) * HD + d);
-      const float4 p1 = *reinterpret_cast<const float4*>(part + (w * C::kRowsTile + r) * HD + d + 4);
+      const float4 p0 = *reinterpret_cast<const float4*>(part + (w * C::kRows + r) * HD + d);
+      const float4 p1 = *reinterpret_cast<const float4*>(part + (w * C::kRows + r) * HD + d + 4);
       o[0] = fmaf(f, p0.x, o[0]), o[1] = fmaf(f, p0.y, o[1]), o[2] = fmaf(f, p0.z, o[2]), o[3] = fmaf(f, p0.w, o[3]);
       o[4] = fmaf(f, p1.x, o[4]), o[5] = fmaf(f, p1.y, o[5]), o[6] = fmaf(f, p1.z, o[6]), o[7] = fmaf(f, p1.w, o[7]);
     }
@@ -585,8 +661,8 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
       for (int e = 0; e < 8; ++e) o[e] = L == 0.f ? 0.f : o[e] * inv;
       store8(out_row(r) + d, o);
     } else {
-      __stcg(reinterpret_cast<float4*>(rec + 2 * C::kRowsTile + r * HD + d), make_float4(o[0], o[1], o[2], o[3]));
-      __stcg(reinterpret_cast<float4*>(rec + 2 * C::kRowsTile + r * HD + d + 4), make_float4(o[4], o[5], o[6], o[7]));
+      __stcg(reinterpret_cast<float4*>(rec + 2 * C::kRows + r * HD + d), make_float4(o[0], o[1], o[2], o[3]));
+      __stcg(reinterpret_cast<float4*>(rec + 2 * C::kRows + r * HD + d + 4), make_float4(o[4], o[5], o[6], o[7]));
       if (d == 0) __stcg(reinterpret_cast<float2*>(rec + 2 * r), make_float2(M, L));
     }
   }
@@ -609,12 +685,12 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     float M = -INFINITY;
     for (int sp = 0; sp < active; ++sp) M = fmaxf(M, __ldcg(recs + (int64_t)sp * kRec + 2 * r));
     float L = 0.f, o[8] = {};
-#pragma unroll 2
+#pragma unroll 4
     for (int sp = 0; sp < active; ++sp) {
       const float* rc = recs + (int64_t)sp * kRec;
       const float2 ml = __ldcg(reinterpret_cast<const float2*>(rc + 2 * r));
-      const float4 p0 = __ldcg(reinterpret_cast<const float4*>(rc + 2 * C::kRowsTile + r * HD + d));
-      const float4 p1 = __ldcg(reinterpret_cast<const float4*>(rc + 2 * C::kRowsTile + r * HD + d + 4));
+      const float4 p0 = __ldcg(reinterpret_cast<const float4*>(rc + 2 * C::kRows + r * HD + d));
+      const float4 p1 = __ldcg(reinterpret_cast<const float4*>(rc + 2 * C::kRows + r * HD + d + 4));
       if (ml.x == -INFINITY && ml.y == ml.y) continue;
       const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
       L = fmaf(f, ml.y, L);
@@ -631,12 +707,15 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-// Row tiles of 16, 32 or 64 rows (WM 1, 2, 4): the smallest that holds the rows
-// of the longest chunk, since a sequence's keys are read once per row tile.
-// (fp32 rows of 256 over a bf16 cache stop at 32: 64 do not fit shared memory).
-static int pick_wm(int max_q, int group, int hd, bool q8, bool f32) {
+// Column tiles of a warp (NN: 1, 2, 4 or 8): the fewest that hold the rows of
+// the longest chunk, since a sequence's keys are read and converted once per
+// row tile; as far as O's HD * NN / 4 registers go.
+static int pick_nn(int max_q, int group, int hd) {
   const int64_t rows = (int64_t)max_q * group;
-  return rows <= 16 ? 1 : rows <= 32 || (hd == 256 && f32 && !q8) ? 2 : 4;
+  const int most = hd <= 64 ? 8 : hd <= 128 ? 4 : 2;
+  int nn = 1;
+  while (nn < most && rows > 8 * nn) nn *= 2;
+  return nn;
 }
 // Splits of the keys: about three CTAs for each of the two that an SM holds, so
 // that sequences of different lengths even out, none shorter than kPaMinSplit.
@@ -647,17 +726,17 @@ static int pick_splits(int64_t units, int max_kv) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(s, 128));
 }
 struct PaPlan {
-  int wm, splits;
+  int nn, splits;
   int64_t tiles, units;
   size_t bytes;  // of partial results
 };
-static PaPlan plan_of(int n, int n_seqs, int group, int kv_heads, int hd, int max_q, int max_kv, bool q8, bool f32) {
+static PaPlan plan_of(int n, int n_seqs, int group, int kv_heads, int hd, int max_q, int max_kv) {
   PaPlan p;
-  p.wm = pick_wm(max_q, group, hd, q8, f32);
-  p.tiles = (int64_t)n * group / (16 * p.wm) + n_seqs;
+  p.nn = pick_nn(max_q, group, hd);
+  p.tiles = (int64_t)n * group / (8 * p.nn) + n_seqs;
   p.units = p.tiles * kv_heads;
   p.splits = pick_splits(p.units, max_kv);
-  p.bytes = p.splits > 1 ? (size_t)p.units * p.splits * 16 * p.wm * (hd + 2) * sizeof(float) : 0;
+  p.bytes = p.splits > 1 ? (size_t)p.units * p.splits * 8 * p.nn * (hd + 2) * sizeof(float) : 0;
   return p;
 }
 
@@ -671,21 +750,20 @@ static int tc_from(const PagedView& c, int hd, int dtype, int group, int max_q) 
 }
 
 size_t paged_attn_workspace_bytes(const PagedView& c, int n, int group, int hd, int dtype, int max_q, int max_kv) {
-  const bool q8 = c.type == DRACO_KV_Q8_0, f32 = dtype == DRACO_DTYPE_F32;
   const int from = tc_from(c, hd, dtype, group, max_q);
-  size_t bytes = plan_of(n, c.n_seqs, group, c.kv_heads, hd, from ? from - 1 : max_q, max_kv, q8, f32).bytes;
+  size_t bytes = plan_of(n, c.n_seqs, group, c.kv_heads, hd, from ? from - 1 : max_q, max_kv).bytes;
   if (from) bytes = std::max(bytes, paged_attn_tc_plan(n, c.n_seqs, group, c.kv_heads, hd, max_kv).bytes);
   return kPagedHead + bytes;
 }
 
-template <int HD, bool Q8, bool F32, int WM>
+template <int HD, bool Q8, bool F32, int NN>
 static cudaError_t launch_t(const PagedAttnArgs& a, const PaPlan& p, cudaStream_t st) {
-  using C = PaCfg<HD, Q8, F32, WM>;
+  using C = PaCfg<HD, Q8, F32, NN>;
   static int attr_set[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 64 || !attr_set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<HD, Q8, F32, WM>,
+    cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<HD, Q8, F32, NN>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem());
     if (e != cudaSuccess) return e;
     if (dev < 64) attr_set[dev] = 1;
@@ -700,25 +778,26 @@ static cudaError_t launch_t(const PagedAttnArgs& a, const PaPlan& p, cudaStream_
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_attn_kernel<HD, Q8, F32, WM>, a);
+  return cudaLaunchKernelEx(&cfg, paged_attn_kernel<HD, Q8, F32, NN>, a);
 }
 template <int HD, bool Q8, bool F32>
-static cudaError_t launch_wm(const PagedAttnArgs& a, const PaPlan& p, cudaStream_t st) {
-  if (p.wm == 1) return launch_t<HD, Q8, F32, 1>(a, p, st);
-  if (p.wm == 2) return launch_t<HD, Q8, F32, 2>(a, p, st);
-  if constexpr (HD == 256 && F32 && !Q8)
-    return cudaErrorInvalidValue;  // pick_wm never asks for it
-  else
-    return launch_t<HD, Q8, F32, 4>(a, p, st);
+static cudaError_t launch_nn(const PagedAttnArgs& a, const PaPlan& p, cudaStream_t st) {
+  if (p.nn == 1) return launch_t<HD, Q8, F32, 1>(a, p, st);
+  if (p.nn == 2) return launch_t<HD, Q8, F32, 2>(a, p, st);
+  if constexpr (HD <= 64) {
+    if (p.nn == 8) return launch_t<HD, Q8, F32, 8>(a, p, st);
+  }
+  if constexpr (HD <= 128) return launch_t<HD, Q8, F32, 4>(a, p, st);
+  return cudaErrorInvalidValue;  // pick_nn gives no more
 }
 template <bool Q8, bool F32>
 static cudaError_t launch_hd(int hd, const PagedAttnArgs& a, const PaPlan& p, cudaStream_t st) {
   switch (hd) {
-    case 32: return launch_wm<32, Q8, F32>(a, p, st);
-    case 64: return launch_wm<64, Q8, F32>(a, p, st);
-    case 96: return launch_wm<96, Q8, F32>(a, p, st);
-    case 128: return launch_wm<128, Q8, F32>(a, p, st);
-    default: return launch_wm<256, Q8, F32>(a, p, st);
+    case 32: return launch_nn<32, Q8, F32>(a, p, st);
+    case 64: return launch_nn<64, Q8, F32>(a, p, st);
+    case 96: return launch_nn<96, Q8, F32>(a, p, st);
+    case 128: return launch_nn<128, Q8, F32>(a, p, st);
+    default: return launch_nn<256, Q8, F32>(a, p, st);
   }
 }
 
@@ -737,7 +816,7 @@ int paged_attn_launch(PagedAttnArgs a, int hd, int dtype, int max_q, int max_kv,
   const int from = tc_from(a.c, hd, dtype, a.group, max_q);
   a.min_new = 0;
   a.max_new = from ? from : 0x7FFFFFFF;
-  const PaPlan p = plan_of(a.n, a.n_seqs, a.group, a.c.kv_heads, hd, from ? from - 1 : max_q, max_kv, q8, f32);
+  const PaPlan p = plan_of(a.n, a.n_seqs, a.group, a.c.kv_heads, hd, from ? from - 1 : max_q, max_kv);
   a.n_splits = p.splits;
   const cudaError_t e = q8 ? (f32 ? launch_hd<true, true>(hd, a, p, st) : launch_hd<true, false>(hd, a, p, st))
                            : (f32 ? launch_hd<false, true>(hd, a, p, st) : launch_hd<false, false>(hd, a, p, st));

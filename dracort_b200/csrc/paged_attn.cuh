@@ -9,6 +9,7 @@ namespace draco {
 constexpr int kPagedCounters = 2048;  // (row tile, kv head) pairs that may be split over CTAs
 // workspace: int32 counters [kPagedCounters], status word, padding to this; then partial results
 constexpr int kPagedHead = kPagedCounters * 4 + 64;
+static_assert(kPagedHead == DRACO_PAGED_WORKSPACE_HEAD && kPagedCounters * 4 == DRACO_PAGED_WORKSPACE_STATUS, "header");
 
 // One call.  The rows of sequence s are its new tokens' query heads of one
 // key/value head, ordered (token, head in group); a row tile takes `R`

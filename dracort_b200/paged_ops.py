@@ -215,7 +215,9 @@ _workspaces: Dict[Tuple[int, int], torch.Tensor] = {}
 
 def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[:N.PAGED_WORKSPACE_HEAD].zero_()  # counters and status; the rest is written before it is read
+        return ws
     key = (device.index, stream)
     with _ws_lock:
         ws = _workspaces.get(key)

@@ -537,8 +537,13 @@ int draco_kv_read(const draco_kv_cache* cache, const int* seq, const int* pos, i
  * fp32; fp32 activations keep fp32 accuracy, bf16 ones round the
  * probabilities to 16 bits.
  * Workspace: at least draco_attention_paged_workspace_bytes() bytes, 16-byte
- * aligned, zeroed before its first use, left ready for the next call on the
- * same stream; two calls that may overlap need two. */
+ * aligned, its first DRACO_PAGED_WORKSPACE_HEAD bytes zeroed before its first
+ * use, left ready for the next call on the same stream; two calls that may
+ * overlap need two.  The int32 at DRACO_PAGED_WORKSPACE_STATUS is nonzero
+ * (DRACO_ERR_TIMEOUT) after a bounded device wait ran out, the outputs of that
+ * call then being invalid; zero the head again before reusing it. */
+#define DRACO_PAGED_WORKSPACE_STATUS 8192
+#define DRACO_PAGED_WORKSPACE_HEAD 8256
 typedef struct draco_attention_paged_args {
   const void* q;
   void* out;
