@@ -726,14 +726,19 @@ static int pick_splits(int64_t units, int max_kv) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(s, 128));
 }
 struct PaPlan {
-  int nn, splits;
+  int nn, splits, per_seq;
   int64_t tiles, units;
   size_t bytes;  // of partial results
 };
 static PaPlan plan_of(int n, int n_seqs, int group, int kv_heads, int hd, int max_q, int max_kv) {
   PaPlan p;
   p.nn = pick_nn(max_q, group, hd);
-  p.tiles = (int64_t)n * group / (8 * p.nn) + n_seqs;
+  const int R = 8 * p.nn;
+  p.tiles = (int64_t)n * group / R + n_seqs;
+  // short chunks: as many tiles for every sequence
+  const int64_t per = ((int64_t)max_q * group + R - 1) / R;
+  p.per_seq = per > 0 && per * n_seqs <= p.tiles ? (int)per : 0;
+  if (p.per_seq) p.tiles = per * n_seqs;
   p.units = p.tiles * kv_heads;
   p.splits = pick_splits(p.units, max_kv);
   p.bytes = p.splits > 1 ? (size_t)p.units * p.splits * 8 * p.nn * (hd + 2) * sizeof(float) : 0;
@@ -818,6 +823,7 @@ int paged_attn_launch(PagedAttnArgs a, int hd, int dtype, int max_q, int max_kv,
   a.max_new = from ? from : 0x7FFFFFFF;
   const PaPlan p = plan_of(a.n, a.n_seqs, a.group, a.c.kv_heads, hd, from ? from - 1 : max_q, max_kv);
   a.n_splits = p.splits;
+  a.per_seq = p.per_seq;
   const cudaError_t e = q8 ? (f32 ? launch_hd<true, true>(hd, a, p, st) : launch_hd<true, false>(hd, a, p, st))
                            : (f32 ? launch_hd<false, true>(hd, a, p, st) : launch_hd<false, false>(hd, a, p, st));
   if (e != cudaSuccess) {
@@ -825,6 +831,7 @@ int paged_attn_launch(PagedAttnArgs a, int hd, int dtype, int max_q, int max_kv,
     return DRACO_ERR_CUDA;
   }
   if (!from) return DRACO_OK;
+  a.per_seq = 0;
   a.min_new = from;
   a.max_new = 0x7FFFFFFF;
   const TcPlan t = paged_attn_tc_plan(a.n, a.n_seqs, a.group, a.c.kv_heads, hd, max_kv);

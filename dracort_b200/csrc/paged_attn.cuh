@@ -26,6 +26,7 @@ struct PagedAttnArgs {
   float scale_log2;  // softmax scale * log2(e)
   int n, n_seqs, heads, group, n_splits;
   int min_new, max_new;  // this kernel takes the sequences with min_new <= new tokens < max_new
+  int per_seq;           // row tiles of every sequence, or 0: tiles by the tokens' places
 };
 
 struct RowTile {
@@ -41,7 +42,9 @@ __device__ __forceinline__ int seq_begin(const PagedAttnArgs& a, int s) {
   return min(max(__ldg(a.q_start + s), 0), a.n);
 }
 
-// Tile t of R rows.  Sequence s owns the tiles from floor(start_s * group / R)
+// Tile t of R rows.  With per_seq the sequences own that many tiles each (short
+// chunks: a decode step finds its sequence without a search).  Otherwise
+// sequence s owns the tiles from floor(start_s * group / R)
 // + s on: enough for its rows whatever the other lengths are, so that no
 // prefix sum over the sequences is needed, and strictly increasing in s, so
 // that a warp finds s with a 32-ary search (one round of loads up to 32
@@ -50,6 +53,7 @@ __device__ __forceinline__ int seq_begin(const PagedAttnArgs& a, int s) {
 __device__ __forceinline__ RowTile find_tile(const PagedAttnArgs& a, int t, int R) {
   const int lane = threadIdx.x & 31;
   int lo = 0, cnt = a.n_seqs;
+  if (a.per_seq) lo = t / a.per_seq, cnt = 1;
   while (cnt > 1) {
     const int step = (cnt + 31) / 32;
     const int s = lo + lane * step;
@@ -65,7 +69,7 @@ __device__ __forceinline__ RowTile find_tile(const PagedAttnArgs& a, int t, int 
   const int end = max(seq_begin(a, lo + 1), r.start);
   r.new_tok = end - r.start;
   r.rows = r.new_tok * a.group;
-  r.row0 = (t - (int)((int64_t)r.start * a.group / R) - lo) * R;
+  r.row0 = (a.per_seq ? t % a.per_seq : t - (int)((int64_t)r.start * a.group / R) - lo) * R;
   const int64_t cap = (int64_t)a.c.max_pages << a.c.page_shift;
   const int kv = __ldg(a.kv_len + lo);
   r.kv = (int)(kv < 0 ? 0 : kv > cap ? cap : kv);

@@ -46,7 +46,9 @@
 namespace draco {
 
 constexpr int kTcRows = 128;            // rows of a tile (fewer when the group does not divide 128)
-constexpr int kTcKeys = 128;
+constexpr int kTcKeys = 128;            // keys of a shared-memory tile
+constexpr int kTcStep = 64;             // keys of a step: scores, P, second product
+constexpr int kTcPoly = 2;
 constexpr uint64_t kTcWaitNs = 2000000000ull;  // 2 s: far beyond any legitimate wait
 constexpr int kTcBadWords = 32;         // marks of 1024 keys from the first edge tile on
 
@@ -70,16 +72,19 @@ struct TcCfg {
   static constexpr int kThreads = Q8 ? 640 : 384;
   static constexpr int kProducers = 8;                    // Q8_0: converting warps
   // registers of a thread: softmax warpgroups, the MMA / load warpgroup, converting warpgroups
-  static constexpr int kRegsSoftmax = Q8 ? 168 : 208, kRegsOne = Q8 ? 32 : 80, kRegsConvert = 56;
+  static constexpr int kRegsSoftmax = Q8 ? 144 : 208, kRegsOne = Q8 ? 64 : 80, kRegsConvert = 64;
   static constexpr int kRegsBlock = 256 * kRegsSoftmax + 128 * kRegsOne + (kThreads - 384) * kRegsConvert;
 };
 
 __device__ __forceinline__ void tca_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tca_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tca_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tca_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+__device__ __forceinline__ void tca_commit(uint32_t one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(one)
+      : "memory");
 }
 // Shared-memory operand with the 128-byte swizzle, rows of 64 values at 128
 // bytes, 8-row groups at 1024 (version 1, layout 2).  K-major: rows are M / N,
@@ -89,23 +94,31 @@ __device__ __forceinline__ uint64_t tca_desc(uint32_t addr, uint32_t lbo) {
   return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
+// the descriptor behind its low word (tca_desc's high word is constant)
+__device__ __forceinline__ uint64_t tca_desc_of(uint32_t lo) {
+  constexpr uint32_t hi = (1024 >> 4) | (1u << 14) | (2u << 29);
+  return ((uint64_t)hi << 32) | lo;
+}
 // fp32 D; A and B bf16 (format 1) or fp16 (0); bit 16: B is MN-major
 __host__ __device__ constexpr uint32_t tca_idesc(bool bf16, int m, int n, bool b_mn) {
   return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
          ((uint32_t)(m >> 4) << 24);
 }
-__device__ __forceinline__ void tca_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// (`one`: the lane that issues.  The predicate sits on the instruction, not on a
+// branch: in warp-uniform code the operands are computed in uniform registers,
+// where a branch of one lane would move each there; 55 clocks an MMA.)
+__device__ __forceinline__ void tca_mma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one)
       : "memory");
 }
-__device__ __forceinline__ void tca_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void tca_mma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one)
       : "memory");
 }
 __device__ __forceinline__ void tca_ld32(uint32_t addr, float* v) {
@@ -159,6 +172,51 @@ __device__ __forceinline__ float tca_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ void tca_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(
+          r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t x;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(x));
+  return x;
+}
+// maximum that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// pairs of fp32 values in one register pair
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  return ((uint64_t)__float_as_uint(b) << 32) | __float_as_uint(a);
+}
+__device__ __forceinline__ float lo_2(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float hi_2(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t fma_2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+// 2^x on the FMA pipe: x = n + f with n the nearest integer (added to 1.5 * 2^23
+// it sits in the low bits), 2^f by a cubic fitted to |f| <= 1/2 for the least
+// relative error (7.5e-5; P keeps 8 or 11 bits), n added to the exponent (the
+// argument reduction of Cody and Waite).  x is raised to -126 at least; not
+// for NaN.
+constexpr float kP0 = 0.99992806f, kP1 = 0.69326097f, kP2 = 0.24261115f, kP3 = 0.05517165f;
+__device__ __forceinline__ float exp2_poly(float x) {
+  x = fmaxf(x, -126.f);
+  const float n = x + 12582912.f;
+  const float f = x - (n - 12582912.f);
+  float p = fmaf(kP3, f, kP2);
+  p = fmaf(p, f, kP1);
+  p = fmaf(p, f, kP0);
+  return __uint_as_float(__float_as_uint(p) + (__float_as_uint(n) << 23));
+}
 template <int N>
 __device__ __forceinline__ void regs_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -171,7 +229,7 @@ __device__ __forceinline__ void regs_down() {
 struct TcBars {
   uint64_t q_full, q_ready;
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], v_clean[2];
-  uint64_t s_full[2], p_full[2], o_full[2], drain;
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], o_full[2], drain;  // [row tile][step & 1]
 };
 
 template <int HDP, bool Q8>
@@ -188,21 +246,24 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
   uint8_t* q_s = smem;                       // [2] Q tiles
   uint8_t* k_s = smem + 2 * C::kTile;        // [stage] key tiles
   uint8_t* v_s = k_s + C::kStages * C::kTile;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // (lane 0's values: the compiler sees that the warp shares them)
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   grid_dependency_wait();
-  const int tile_id = gridDim.x - 1 - blockIdx.x;  // the tiles with the most keys first
+  // the tiles with the most keys first, of all heads
+  const int tile_id = gridDim.y - 1 - blockIdx.y;
   const RowTile tile = find_tile(a, tile_id, 2 * P.rt);
   if (tile.s < 0) return;
-  const int kvh = blockIdx.z, hd = P.hd;
+  const int kvh = blockIdx.x % a.c.kv_heads, hd = P.hd;
   const int rows = min(2 * P.rt, tile.rows - tile.row0);
   const int kend = max(0, min(tile.kv, row_limit(a, tile, tile.row0 + rows - 1)));
   int ck = (kend + a.n_splits - 1) / a.n_splits;
   ck = max(kTcKeys, (ck + kTcKeys - 1) & ~(kTcKeys - 1));
   const int active = max(1, (kend + ck - 1) / ck);
-  const int split = blockIdx.y;
+  const int split = blockIdx.x / a.c.kv_heads;
   if (split >= active) return;
   const int kbeg = split * ck, kfin = min(kend, kbeg + ck);
-  const int nj = (kfin - kbeg + kTcKeys - 1) / kTcKeys;  // key tiles
+  const int nj = __shfl_sync(0xffffffffu, (kfin - kbeg + kTcKeys - 1) / kTcKeys, 0);  // key tiles
+  const int ns = __shfl_sync(0xffffffffu, (kfin - kbeg + kTcStep - 1) / kTcStep, 0);  // steps
   // the first tile in which some row is masked (or keys end)
   const int first_lim = max(0, min(tile.kv, row_limit(a, tile, tile.row0)));
   const int jedge = max(0, min(nj, first_lim <= kbeg ? 0 : (first_lim - kbeg) / kTcKeys));
@@ -215,8 +276,11 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
       mbar_init(&bars.v_full[i], Q8 ? C::kProducers : 1);
       mbar_init(&bars.k_empty[i], 1);
       mbar_init(&bars.v_empty[i], 1);
-      mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_full[i], 4);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&bars.s_full[i][h], 1);
+        mbar_init(&bars.p_full[i][h], 4);
+        mbar_init(&bars.pv_done[i][h], 1);
+      }
       mbar_init(&bars.o_full[i], 1);
       mbar_init(&bars.v_clean[i], 2);
     }
@@ -234,15 +298,20 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
   tca_before();
   __syncthreads();
   tca_after();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
 
   // a wait that gives up: the role leaves its loop, the others' waits run out
-  // too.  (Every barrier's next phase but one needs the waiting side to have
-  // passed, so a parity never stands for two phases.)
+  // too.  (A wait names a phase by its parity: no barrier completes two phases
+  // more before the waiting side has passed.)
   auto wait = [&](uint64_t* bar, int phase) -> bool {
     if (mbar_wait_bounded(bar, (uint32_t)phase & 1u, kTcWaitNs)) return true;
     s_abort = 1;
     return false;
+  };
+  auto wait_fast = [&](uint64_t* bar, int phase) -> bool {  // the whole warp; one vote when the phase is over
+    const bool done = mbar_try_wait(bar, (uint32_t)phase & 1u);
+    if (__all_sync(0xffffffffu, done)) return true;
+    return __all_sync(0xffffffffu, wait(bar, phase));
   };
   auto wait_warp = [&](uint64_t* bar, int phase) -> bool {
     return __all_sync(0xffffffffu, wait(bar, phase));
@@ -298,63 +367,77 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
     }
     constexpr float kShift = Q8 ? 6.f : 0.f;
     float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < nj && ok; ++j) {
-      if (!(ok = wait_warp(&bars.s_full[w], j))) break;
+    for (int i = 0; i < ns && ok; ++i) {
+      if (!(ok = wait_warp(&bars.s_full[w][i & 1], i >> 1))) break;
       tca_after();
-      float s[128];
+      const uint32_t s_i = s_t + kTcStep * (i & 1);
+      const int vis = lim - (kbeg + i * kTcStep);  // columns that the row sees
+      float s[kTcStep];
+      tca_ld32(s_i, s);
+      tca_ld32(s_i + 32, s + 32);
+      tca_ld_wait(s);
+      tca_ld_wait(s + 32);
+      const bool edge = __any_sync(0xffffffffu, vis < kTcStep);
+      if (edge) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tca_ld32(s_t + 32 * c, s + 32 * c);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tca_ld_wait(s + 32 * c);
-      const int k0 = kbeg + j * kTcKeys;
-      if (__any_sync(0xffffffffu, k0 + kTcKeys > lim)) {
-        const int vis = lim - k0;
-#pragma unroll
-        for (int i = 0; i < 128; ++i) s[i] = i < vis ? s[i] : -INFINITY;
+        for (int e = 0; e < kTcStep; ++e) s[e] = e < vis ? s[e] : -INFINITY;
       }
-      float x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3];
+      float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
-      for (int i = 4; i < 128; i += 4) {
-        x0 = fmaxf(x0, s[i]), x1 = fmaxf(x1, s[i + 1]), x2 = fmaxf(x2, s[i + 2]), x3 = fmaxf(x3, s[i + 3]);
+      for (int e = 0; e < kTcStep; e += 4) {
+        x0 = max_nan(x0, max_nan(s[e], s[e + 1]));
+        x1 = max_nan(x1, max_nan(s[e + 2], s[e + 3]));
       }
-      const float mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * sc;
-      if (__any_sync(0xffffffffu, mx > m + 8.f)) {
-        const float n = fmaxf(m, mx);
+      const float mx = max_nan(x0, x1) * sc;
+      if (__any_sync(0xffffffffu, !(mx <= m + 8.f))) {
+        const float n = max_nan(m, mx);
         const float f = n == -INFINITY ? 1.f : tca_exp2(m - n);
         m = n;
         l *= f;
-        if (j > 0) {  // O of the tiles so far is complete: the scores of tile j came after it
+        if (i > 0) {  // O of the steps so far, once their products are done
+          if (!(ok = wait_warp(&bars.pv_done[w][(i - 1) & 1], (i - 1) >> 1))) break;
+          tca_after();
 #pragma unroll 1
           for (int c = 0; c < HDP / 32; ++c) {
             float o[32];
             tca_ld32(o_t + 32 * c, o);
             tca_ld_wait(o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= f;
+            for (int e = 0; e < 32; ++e) o[e] *= f;
             tca_st32(o_t + 32 * c, reinterpret_cast<uint32_t*>(o));
           }
         }
       }
-      const float ref = m == -INFINITY ? 0.f : m - kShift;
+      // (a row with an infinite score is NaN, as inf - inf)
+      const float ref = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7FC00000) : m - kShift;
+      const uint64_t sc2 = pair2(sc, sc), ref2 = pair2(-ref, -ref);
       float l0 = 0.f, l1 = 0.f;
+      auto form = [&](auto poly) {  // P, every kTcPoly-th pair's second exponential on the FMA pipe
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t p[32];
+        for (int c = 0; c < kTcStep / 32; ++c) {
+          uint32_t p[16];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float u = tca_exp2(fmaf(s[64 * c + 2 * i], sc, -ref)), v = tca_exp2(fmaf(s[64 * c + 2 * i + 1], sc, -ref));
-          l0 += u, l1 += v;
-          p[i] = Q8 ? pack_f16(u, v) : pack_bf16(u, v);
+          for (int e = 0; e < 16; ++e) {
+            const uint64_t x = fma_2(pair2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), sc2, ref2);
+            const float u = tca_exp2(lo_2(x));
+            const float v = decltype(poly)::value && e % kTcPoly == 1 ? exp2_poly(hi_2(x)) : tca_exp2(hi_2(x));
+            l0 += u, l1 += v;
+            p[e] = Q8 ? pack_f16(u, v) : pack_bf16(u, v);
+          }
+          tca_st16(s_i + 16 * c, p);
         }
-        tca_st32(s_t + 32 * c, p);
-      }
+      };
+      if (edge)
+        form(std::false_type());
+      else
+        form(std::true_type());
       l += l0 + l1;
       tca_st_wait();
       tca_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.p_full[w]);
+      if (lane == 0) mbar_arrive(&bars.p_full[w][i & 1]);
     }
-    if (ok && nj > 0) ok = wait_warp(&bars.o_full[w], 0);
+    if (ok && ns > 0) ok = wait_warp(&bars.o_full[w], 0);
     tca_after();
     // marked values: what the rows that see them add
     uint32_t any_bad = 0;
@@ -484,57 +567,71 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
     tca_before();
   } else if (warp == 8) {
     // ------------------------------------------------------------- MMA
-    if (lane == 0 && nj > 0) {
-      constexpr uint32_t ids = tca_idesc(!Q8, 128, 128, false), ido = tca_idesc(!Q8, 128, HDP, true);
-      const uint32_t q_u = smem_u32(q_s), k_u = smem_u32(k_s), v_u = smem_u32(v_s);
-      auto scores = [&](int w, int j) {
-        const uint32_t qa = q_u + w * C::kTile, ka = k_u + (j & 1) * C::kTile;
+    // the whole warp runs the loop, one lane issues: operands stay warp-uniform
+    // (a lane of its own would move each to a uniform register first)
+    if (nj > 0) {
+      const uint32_t one = elect_one();
+      constexpr uint32_t ids = tca_idesc(!Q8, 128, kTcStep, false), ido = tca_idesc(!Q8, 128, HDP, true);
+      // low words of the operand descriptors (address / 16 and the leading offset);
+      // the high word is the same for all
+      const uint32_t q_d = (uint32_t)tca_desc(smem_u32(q_s), 16), k_d = (uint32_t)tca_desc(smem_u32(k_s), 16),
+                     v_d = (uint32_t)tca_desc(smem_u32(v_s), C::kHalf);
+      constexpr uint32_t kTile16 = C::kTile >> 4, kStep16 = kTcStep * 128 >> 4;
+      // The loop is written out by step parity and row tile: what a step needs
+      // beside its MMAs is a dozen instructions, since this one warp's
+      // instruction latency would otherwise be what the tensor core waits for.
+      auto scores = [&](auto wc, auto hc, int j, bool last) {  // half h of key tile j
+        constexpr int w = decltype(wc)::value, h = decltype(hc)::value;
+        const uint32_t ka = k_d + (j & 1) * kTile16 + h * kStep16;
 #pragma unroll
         for (int k = 0; k < HDP / 16; ++k) {
-          const uint32_t at = (k >> 2) * C::kHalf + (k & 3) * 32;
-          tca_mma_ss(tmem + 128 * w, tca_desc(qa + at, 16), tca_desc(ka + at, 16), ids, k > 0);
+          const uint32_t at = ((k >> 2) * C::kHalf + (k & 3) * 32) >> 4;
+          tca_mma_ss(one, tmem + 128 * w + kTcStep * h, tca_desc_of(q_d + w * kTile16 + at), tca_desc_of(ka + at), ids,
+                     k > 0);
         }
-        tca_commit(&bars.s_full[w]);
+        tca_commit(one, &bars.s_full[w][h]);
+        if (w == 1 && (h == 1 || last)) tca_commit(one, &bars.k_empty[j & 1]);
       };
-      auto outputs = [&](int w, int j) {
-        const uint32_t va = v_u + (j & 1) * C::kTile;
+      auto outputs = [&](auto wc, auto hc, int j, bool last) {
+        constexpr int w = decltype(wc)::value, h = decltype(hc)::value;
+        const uint32_t va = v_d + (j & 1) * kTile16 + h * kStep16;
 #pragma unroll
-        for (int k = 0; k < kTcKeys / 16; ++k)
-          tca_mma_ts(tmem + 256 + HDP * w, tmem + 128 * w + 8 * k, tca_desc(va + k * 2048, C::kHalf), ido,
-                     j > 0 || k > 0);
+        for (int k = 0; k < kTcStep / 16; ++k)
+          tca_mma_ts(one, tmem + 256 + HDP * w, tmem + 128 * w + kTcStep * h + 8 * k, tca_desc_of(va + k * (2048 >> 4)),
+                     ido, h > 0 || k > 0 || j > 0);
+        tca_commit(one, &bars.pv_done[w][h]);
+        if (last) tca_commit(one, &bars.o_full[w]);
+        if (w == 1 && (h == 1 || last)) tca_commit(one, &bars.v_empty[j & 1]);
       };
-      bool ok = wait(Q8 ? &bars.q_ready : &bars.q_full, 0);
-      ok = ok && wait(&bars.k_full[0], 0);
+      using I0 = std::integral_constant<int, 0>;
+      using I1 = std::integral_constant<int, 1>;
+      bool ok = wait_fast(Q8 ? &bars.q_ready : &bars.q_full, 0) && wait_fast(&bars.k_full[0], 0);
       if (ok) {
         tca_after();
-        scores(0, 0);
-        scores(1, 0);
-        tca_commit(&bars.k_empty[0]);
+        scores(I0(), I0(), 0, ns == 1), scores(I1(), I0(), 0, ns == 1);
+        if (ns > 1) scores(I0(), I1(), 0, false), scores(I1(), I1(), 0, false);
       }
-      for (int j = 0; j < nj && ok; ++j) {
-#pragma unroll 1
-        for (int w = 0; w < 2 && ok; ++w) {
-          if (w == 0) {
-            ok = wait(Q8 ? &bars.v_full[j & 1] : &bars.v_clean[j & 1], j >> 1);
-          }
-          ok = ok && wait(&bars.p_full[w], j);
-          if (!ok) break;
-          tca_after();
-          outputs(w, j);
-          if (w == 1) tca_commit(&bars.v_empty[j & 1]);
-          if (j + 1 < nj) {
-            if (w == 0 && !(ok = wait(&bars.k_full[(j + 1) & 1], (j + 1) >> 1))) break;
-            tca_after();
-            scores(w, j + 1);
-            if (w == 1) tca_commit(&bars.k_empty[(j + 1) & 1]);
-          } else {
-            tca_commit(&bars.o_full[w]);
-          }
+      auto step = [&](auto wc, auto hc, int j) -> bool {
+        constexpr int w = decltype(wc)::value, h = decltype(hc)::value;
+        const int i = 2 * j + h;
+        if (!wait_fast(&bars.p_full[w][h], j)) return false;
+        tca_after();
+        outputs(wc, hc, j, i == ns - 1);
+        if (i + 2 < ns) {
+          if (w == 0 && h == 0 && !wait_fast(&bars.k_full[(j + 1) & 1], (j + 1) >> 1)) return false;
+          scores(wc, hc, j + 1, i + 2 == ns - 1);
         }
+        return true;
+      };
+#pragma unroll 1
+      for (int j = 0; j < nj && ok; ++j) {
+        ok = wait_fast(Q8 ? &bars.v_full[j & 1] : &bars.v_clean[j & 1], j >> 1) && step(I0(), I0(), j) &&
+             step(I1(), I0(), j);
+        if (ok && 2 * j + 1 < ns) ok = step(I0(), I1(), j) && step(I1(), I1(), j);
       }
       if (!ok) {
         // the MMAs issued so far finish before shared and tensor memory are given up
-        tca_commit(&bars.drain);
+        tca_commit(one, &bars.drain);
         mbar_wait_bounded(&bars.drain, 0, kTcWaitNs);
       }
     }
@@ -632,35 +729,37 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
   } else {
     // --------------------------------------------------------------- Q8_0 tiles
     if constexpr (Q8) {
-      const int pt = tid - 384, row = pt & 127, half = pt >> 7;  // a key and 64 (or 32) of its values
-      constexpr int kVals = HDP / 2;             // values of a thread
-      constexpr int kVec = kVals / 16;           // 16-byte loads
-      const int d0 = half * kVals;
-      uint4 qv[kVec];
-      uint32_t sv[kVals / 32];
+      // 16 values of a key per lane, the lanes of a warp on contiguous keys: 16-byte
+      // loads of whole lines, and 16-byte stores of which eight lanes cover all
+      // banks (a lane's two chunks go in the order that its place asks for)
+      constexpr int kPer = HDP / 16;               // lanes of a key
+      constexpr int kKeysPass = 256 / kPer;        // keys that the 8 warps take at a time
+      constexpr int kPass = kTcKeys / kKeysPass;   // 4 or 2
+      const int pt = tid - 384, piece = pt % kPer, d0 = 16 * piece, key_l = pt / kPer;
+      const bool on_d = d0 < hd;
+      uint4 qv[kPass];
+      uint32_t sv[kPass];
       auto fetch = [&](const uint8_t* base, int j) {
-        const int key = kbeg + j * kTcKeys + row;
-        int page = -1;
-        if (j < nj && key < kfin) page = page_of(a.c, tile.s, key);
-        const int off = key & ((1 << a.c.page_shift) - 1);
-        const uint8_t* blk = base + ((int64_t)max(page, 0) * a.c.kv_heads + kvh) * a.c.block_bytes;
-        const uint8_t* sp = blk + ((int64_t)hd << a.c.page_shift);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          const bool on = page >= 0 && d0 + 16 * i < hd;
-          qv[i] = on ? __ldg(reinterpret_cast<const uint4*>(blk + (int64_t)off * hd + d0 + 16 * i))
-                     : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < kVals / 32; ++i) {
-          const bool on = page >= 0 && d0 + 32 * i < hd;
-          sv[i] = on ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(sp) + off * (hd / 32) + (d0 >> 5) + i) : 0u;
+        for (int i = 0; i < kPass; ++i) {
+          const int key = kbeg + j * kTcKeys + i * kKeysPass + key_l;
+          int page = -1;
+          if (on_d && j < nj && key < kfin) page = page_of(a.c, tile.s, key);
+          qv[i] = make_uint4(0, 0, 0, 0);
+          sv[i] = 0;
+          if (page >= 0) {
+            const int off = key & ((1 << a.c.page_shift) - 1);
+            const uint8_t* blk = base + ((int64_t)page * a.c.kv_heads + kvh) * a.c.block_bytes;
+            qv[i] = __ldg(reinterpret_cast<const uint4*>(blk + off * hd + d0));
+            sv[i] = __ldg(reinterpret_cast<const uint16_t*>(blk + (hd << a.c.page_shift)) + off * (hd / 32) + (d0 >> 5));
+          }
         }
       };
       auto put = [&](uint8_t* tile_s) {
+        const int c0 = (d0 >> 3) & 7, flip = (piece ^ (piece >> 2)) & 1;
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          const uint32_t d = (sv[i / 2] & 0xFFFFu) * 0x10001u;
+        for (int i = 0; i < kPass; ++i) {
+          const uint32_t d = sv[i] * 0x10001u;
           const __half2 d2 = *reinterpret_cast<const __half2*>(&d);
           const uint32_t ws[4] = {qv[i].x ^ 0x80808080u, qv[i].y ^ 0x80808080u, qv[i].z ^ 0x80808080u,
                                   qv[i].w ^ 0x80808080u};
@@ -672,10 +771,14 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
                                                     *reinterpret_cast<const __half2*>(&c)), d2);
             o[e] = *reinterpret_cast<const uint32_t*>(&h);
           }
-          const int dd = d0 + 16 * i, c = (dd >> 3) & 7;
-          uint8_t* base = tile_s + (dd >> 6) * C::kHalf + row * 128;
-          *reinterpret_cast<uint4*>(base + ((c ^ (row & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<uint4*>(base + (((c + 1) ^ (row & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+          const int row = i * kKeysPass + key_l;
+          uint8_t* base = tile_s + (d0 >> 6) * C::kHalf + row * 128;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int second = e ^ flip;
+            *reinterpret_cast<uint4*>(base + (((c0 + second) ^ (row & 7)) << 4)) =
+                second ? make_uint4(o[4], o[5], o[6], o[7]) : make_uint4(o[0], o[1], o[2], o[3]);
+          }
         }
       };
       bool ok = true;
@@ -690,12 +793,14 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
         if (lane == 0) mbar_arrive(&bars.k_full[st]);
         if (j >= 2 && !(ok = wait_warp(&bars.v_empty[st], (j >> 1) - 1))) break;
         if (j >= jedge) {
-          bool bad = false;
 #pragma unroll
-          for (int i = 0; i < kVals / 32; ++i)
-            if ((sv[i] & 0x7C00u) == 0x7C00u) sv[i] = 0, bad = true;
-          const int b = (j - jedge) * kTcKeys + row;
-          if (bad && b < kTcBadWords * 32) atomicOr(&s_bad[b >> 5], 1u << (b & 31));
+          for (int i = 0; i < kPass; ++i) {
+            const int b = (j - jedge) * kTcKeys + i * kKeysPass + key_l;
+            if ((sv[i] & 0x7C00u) == 0x7C00u) {
+              sv[i] = 0;
+              if (b < kTcBadWords * 32) atomicOr(&s_bad[b >> 5], 1u << (b & 31));
+            }
+          }
         }
         put(v_s + st * C::kTile);
         fetch(a.c.k, j + 1);
@@ -776,7 +881,7 @@ static cudaError_t tc_launch(const TcParams& P, const TcPlan& p, cudaStream_t st
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.tiles, (unsigned)p.splits, (unsigned)P.a.c.kv_heads);
+  cfg.gridDim = dim3((unsigned)(P.a.c.kv_heads * p.splits), (unsigned)p.tiles);
   cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = st;

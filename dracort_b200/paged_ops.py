@@ -240,9 +240,9 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     h // (heads // kv_heads).  Returns out, shaped like q; tokens that see
     nothing get zeros, rows behind the last sequence are left as they are.
 
-    max_q, max_kv bound the tokens and positions of a sequence (default: all
-    tokens; the whole block table); they choose the kernel and size the launch,
-    so tight bounds are faster.  scale defaults to 1 / sqrt(head_dim).
+    max_q, max_kv are upper bounds of a sequence's tokens and positions (default:
+    all tokens; the whole block table); they choose the kernels and size the
+    launch, so tight bounds are faster (tokens past max_q may be left out).  scale defaults to 1 / sqrt(head_dim).
     workspace: a zeroed uint8 tensor of attention_paged_workspace_nbytes that
     the caller keeps (one per call that may overlap another); by default one
     per stream is kept here, and a captured call gets its own."""

@@ -529,10 +529,9 @@ int draco_kv_read(const draco_kv_cache* cache, const int* seq, const int* pos, i
  * i: out = softmax(scale q K^T) V, query head h reading key/value head
  * h / (heads / kv_heads).  A token that sees no position (kv_len < m) gets
  * zeros; rows of out behind the last sequence stay as they are.  max_q and
- * max_kv bound the sequences' new tokens and cached positions: they size the
- * launch and the workspace and need not be tight (results do not depend on
- * lengths beyond max_kv being wrong, only the speed does; a sequence of more
- * than max_q new tokens is still computed).
+ * max_kv are upper bounds of the sequences' new tokens and cached positions.
+ * They choose the kernels and size the launch and the workspace: tight ones
+ * are faster; tokens of a sequence past max_q may be left out.
  * scale 0 means 1 / sqrt(head_dim).  m, l and the output are accumulated in
  * fp32; fp32 activations keep fp32 accuracy, bf16 ones round the
  * probabilities to 16 bits.
