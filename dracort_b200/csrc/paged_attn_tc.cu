@@ -186,9 +186,9 @@ __device__ __forceinline__ uint32_t elect_one() {
   return x;
 }
 // maximum that keeps a NaN
-__device__ __forceinline__ float max_nan(float a, float b) {
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 // pairs of fp32 values in one register pair
@@ -385,12 +385,12 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
       float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
       for (int e = 0; e < kTcStep; e += 4) {
-        x0 = max_nan(x0, max_nan(s[e], s[e + 1]));
-        x1 = max_nan(x1, max_nan(s[e + 2], s[e + 3]));
+        x0 = max_nan(x0, s[e], s[e + 1]);
+        x1 = max_nan(x1, s[e + 2], s[e + 3]);
       }
-      const float mx = max_nan(x0, x1) * sc;
+      const float mx = max_nan(x0, x1, x1) * sc;
       if (__any_sync(0xffffffffu, !(mx <= m + 8.f))) {
-        const float n = max_nan(m, mx);
+        const float n = max_nan(m, mx, mx);
         const float f = n == -INFINITY ? 1.f : tca_exp2(m - n);
         m = n;
         l *= f;

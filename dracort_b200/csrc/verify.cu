@@ -47,13 +47,19 @@ struct VerifyArgs {
   int n, vocab, max_rows, greedy;
 };
 
-// running maximum, sum of exp2((x - m) c) and first index of the maximum
+// A row's maximum, the sum of exp2((x - m) c) and, for greedy, the first index
+// of the maximum.
 struct RowStat {
   float m, s;
   int i;
 };
+__device__ __forceinline__ float fast_exp2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float weight32(float x, float m, float c) {
-  return x == m ? 1.f : exp2f((x - m) * c);  // (inf - inf) is not taken
+  return x == m ? 1.f : fast_exp2f((x - m) * c);  // (inf - inf) is not taken
 }
 __device__ __forceinline__ RowStat join(RowStat a, RowStat b, float c) {
   RowStat r;
@@ -71,124 +77,205 @@ __device__ __forceinline__ float logit(const T* p) {
     x = __bfloat162float(*p);
   return x == x ? x : -INFINITY;  // a NaN logit is never drawn
 }
-__device__ __forceinline__ double weight64(float x, float m, double inv_t) {
-  return x == m ? 1.0 : x == -INFINITY ? 0.0 : exp((double)(x - m) * inv_t);
+
+// 2^(t / 256) for t <= 0 in fp64 (a few units in the last place), by P. T. P.
+// Tang's table-driven method: t = 256 k + j + f with |f| <= 1/2, the value is
+// 2^k 2^(j/256) e^r, r = f ln2 / 256, e^r by its Taylor series to r^4 (r^5 / 120 <
+// 4e-17).  Half the fp64 instructions of exp(), which bound the drawing.
+constexpr double kTangScale = 369.3299304675746;  // 256 / ln2
+constexpr int kTable = 256;
+__device__ __forceinline__ double exp2_256(double t, const double* table) {
+  const double kd = t + 6755399441055744.0;  // 1.5 * 2^52: the nearest integer in the low bits
+  const int n = __double2loint(kd);
+  const double r = (t - (kd - 6755399441055744.0)) * 0.0027076061740622863;  // ln2 / 256
+  double p = fma(r, 1.0 / 24.0, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  p *= table[n & (kTable - 1)];
+  const double v = __hiloint2double(__double2hiint(p) + ((n >> 8) << 20), __double2loint(p));
+  return t > -256000.0 ? v : 0.0;  // below 2^-1000 (and for -infinity): nothing
+}
+// exp((x - m) / T); t256 = 256 / (T ln2)
+__device__ __forceinline__ double weight64(float x, double m, double t256, const double* table) {
+  const double xd = (double)x;
+  return xd == m ? 1.0 : exp2_256((xd - m) * t256, table);
 }
 
-template <typename T>
+// 16 bytes of logits as fp32
+template <typename T, int V>
+__device__ __forceinline__ void unpack16(const uint4& w, float (&x)[V]) {
+  if constexpr (V == 4) {
+    x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y), x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
+  } else {
+    x[0] = bf16lo(w.x), x[1] = bf16hi(w.x), x[2] = bf16lo(w.y), x[3] = bf16hi(w.y);
+    x[4] = bf16lo(w.z), x[5] = bf16hi(w.z), x[6] = bf16lo(w.w), x[7] = bf16hi(w.w);
+  }
+}
+
+template <typename T, bool kGreedy>
 __global__ void __cluster_dims__(kVfCtas, 1, 1) __launch_bounds__(kVfThreads) verify_kernel(const VerifyArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
-  __shared__ RowStat wstat[kVfRows][kVfWarps];
-  __shared__ RowStat stat[kVfRows];      // this CTA's range
-  __shared__ RowStat full[kVfRows];      // the whole row
-  __shared__ double wsum[2][kVfWarps];   // weights of the warps' ranges: of p, and of what is drawn from
-  __shared__ double csum[2];
+  __shared__ RowStat wstat[kVfRows][kVfWarps];     // this CTA's range, by warp
+  __shared__ RowStat stat[kVfRows][kVfCtas];       // every CTA's range (each writes its column everywhere)
+  __shared__ RowStat full[kVfRows];                // the whole row
+  __shared__ double zsum[kVfCtas][kVfWarps];       // weights of p, by CTA and warp
+  __shared__ double rsum[kVfCtas][kVfWarps];       // what is drawn from
+  __shared__ double table[kGreedy ? 1 : kTable];   // 2^(j / 256)
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (!kGreedy && tid < kTable) table[tid] = exp2((double)tid / kTable);
   grid_dependency_wait();
   grid_launch_dependents();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = (int)cluster.block_rank(), b = blockIdx.x / kVfCtas;
   const T* logits = static_cast<const T*>(a.logits);
   const int begin = min(max(a.row_start[b], 0), a.n);
   const int rows = max(0, min(max(a.row_start[b + 1], 0), a.n) - begin);
-  // ranges: CTA, then warp, in vocabulary order, in units of 8 values
+  // the CTA's range of the vocabulary, in units of 8 values
   const int units = (a.vocab + 7) / 8, per_cta = (units + kVfCtas - 1) / kVfCtas;
-  const int per_warp = (per_cta + kVfWarps - 1) / kVfWarps;
-  const int w0 = min(a.vocab, 8 * min((rank + 1) * per_cta, rank * per_cta + warp * per_warp));
-  const int w1 = min(a.vocab, 8 * min((rank + 1) * per_cta, rank * per_cta + (warp + 1) * per_warp));
+  const int u0 = min(units, rank * per_cta), u1 = min(units, u0 + per_cta);
+  const float c = a.inv_t_log2;
 
   int count = 0;        // drafts taken
   bool decided = rows == 0;
   RowStat at = {-INFINITY, 0.f, 0};  // statistics of the row that the next token comes from
   for (int r0 = 0; r0 < rows && !decided; r0 += kVfRows) {
     const int nr = min(kVfRows, rows - r0);
-    for (int r = 0; r < nr; ++r) {
-      const T* row = logits + (int64_t)(begin + r0 + r) * a.ld_logits;
-      RowStat st = {-INFINITY, 0.f, 0x7FFFFFFF};
-      constexpr int V = 16 / (int)sizeof(T);
-      // from the first 16-byte boundary on in 16-byte loads
-      const int head = min(w1, w0 + (int)(((16 - (reinterpret_cast<uintptr_t>(row + w0) & 15)) & 15) / sizeof(T)));
-      const int vecs = (w1 - head) / V;
-      auto take = [&](float x, int i) {
-        x = x == x ? x : -INFINITY;
-        if (x > st.m) {
-          st.s = (st.m == -INFINITY ? 0.f : st.s * weight32(st.m, x, a.inv_t_log2)) + 1.f;
-          st.m = x, st.i = i;
-        } else if (x != -INFINITY) {
-          st.s += weight32(x, st.m, a.inv_t_log2);
-        }
+    // Rows side by side, 16 / nr warps each (a warp takes a row's whole share
+    // of the range when there are more): few long streams instead of many short
+    // ones whose latencies would add up.
+    const int side = min(nr, kVfWarps), wpr = kVfWarps / side, sub = warp % wpr;
+    const int per_sub = (u1 - u0 + wpr - 1) / wpr;
+    const int w0 = min(a.vocab, 8 * min(u1, u0 + sub * per_sub)), w1 = min(a.vocab, 8 * min(u1, u0 + (sub + 1) * per_sub));
+    for (int r = warp / wpr; r < nr && warp < side * wpr; r += side) {
+      constexpr int V = 16 / (int)sizeof(T), B = 32 / V;  // values of a load, loads in flight: 32 values of a lane
+      const T* row = logits + (int64_t)(begin + r0 + r) * a.ld_logits + w0;
+      const int len = w1 - w0;
+      // values before the first 16-byte boundary
+      const int h = min(len, (int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T)));
+      const int vecs = (len - h) / V;
+      const uint4* vp = reinterpret_cast<const uint4*>(row + h);
+      uint4 buf[B];
+      auto fetch = [&](int v0) {
+#pragma unroll
+        for (int e = 0; e < B; ++e)
+          if (v0 + 32 * e + lane < vecs) buf[e] = __ldg(vp + v0 + 32 * e + lane);
       };
-      if (w0 + lane < head) take(logit(row + w0 + lane), w0 + lane);
-      for (int v = lane; v < vecs; v += 32) {
-        const int i = head + v * V;
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(row + i));
-        float x[V];
-        if constexpr (V == 4) {
-          x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y), x[2] = __uint_as_float(w.z),
-          x[3] = __uint_as_float(w.w);
-        } else {
-          x[0] = bf16lo(w.x), x[1] = bf16hi(w.x), x[2] = bf16lo(w.y), x[3] = bf16hi(w.y);
-          x[4] = bf16lo(w.z), x[5] = bf16hi(w.z), x[6] = bf16lo(w.w), x[7] = bf16hi(w.w);
+      fetch(0);
+      RowStat st = {-INFINITY, 0.f, 0x7FFFFFFF};
+      // values before and after the vectors
+      const int odd = lane < h ? lane : h + vecs * V + (lane - h);
+      const float xo = odd < len ? logit(row + odd) : -INFINITY;
+      if (xo > -INFINITY) st.m = xo, st.s = 1.f, st.i = w0 + odd;
+      for (int v0 = 0; v0 < vecs; v0 += 32 * B) {
+        float x[B][V];
+#pragma unroll
+        for (int e = 0; e < B; ++e) {
+          unpack16<T, V>(buf[e], x[e]);
+          const bool on = v0 + 32 * e + lane < vecs;
+#pragma unroll
+          for (int k = 0; k < V; ++k) x[e][k] = on ? x[e][k] : -INFINITY;
         }
+        if (v0 + 32 * B < vecs) fetch(v0 + 32 * B);
+        float mx = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < V; ++e) take(x[e], i + e);
-      }
-      const int tail = head + vecs * V + lane;
-      if (tail < w1) take(logit(row + tail), tail);
+        for (int e = 0; e < B; ++e)
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        RowStat x;
-        x.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-        x.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-        x.i = __shfl_xor_sync(0xffffffffu, st.i, o);
-        st = join(st, x, a.inv_t_log2);
+          for (int k = 0; k < V; ++k) mx = fmaxf(mx, x[e][k]);  // (passes over a NaN)
+        if constexpr (kGreedy) {
+          if (mx >= st.m && mx > -INFINITY) {
+            int first = 0x7FFFFFFF;
+#pragma unroll
+            for (int e = B - 1; e >= 0; --e)
+#pragma unroll
+              for (int k = V - 1; k >= 0; --k)
+                if (x[e][k] == mx) first = w0 + h + (v0 + 32 * e + lane) * V + k;
+            st.i = mx > st.m ? first : min(st.i, first);
+            st.m = mx;
+          }
+        } else if (mx > -INFINITY) {
+          if (mx > st.m) {
+            st.s = st.m == -INFINITY ? 0.f : st.s * weight32(st.m, mx, c);
+            st.m = mx;
+          }
+          if (st.m < INFINITY) {
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int e = 0; e < B; ++e)
+#pragma unroll
+              for (int k = 0; k < V; k += 2) {
+                const float u = fast_exp2f((x[e][k] - st.m) * c), v = fast_exp2f((x[e][k + 1] - st.m) * c);
+                s0 += u == u ? u : 0.f, s1 += v == v ? v : 0.f;
+              }
+            st.s += s0 + s1;
+          } else {  // an infinite logit has all the weight
+#pragma unroll
+            for (int e = 0; e < B; ++e)
+#pragma unroll
+              for (int k = 0; k < V; ++k) st.s += x[e][k] == INFINITY ? 1.f : 0.f;
+          }
+        }
       }
-      if (lane == 0) wstat[r][warp] = st;
+      // the warp's maximum, then sums relative to it (or the first index of it)
+      RowStat wst = st;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) wst.m = fmaxf(wst.m, __shfl_xor_sync(0xffffffffu, wst.m, o));
+      if constexpr (kGreedy) {
+        wst.i = __reduce_min_sync(0xffffffffu, st.m == wst.m ? st.i : 0x7FFFFFFF);
+      } else {
+        wst.s = st.m == -INFINITY ? 0.f : st.s * weight32(st.m, wst.m, c);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) wst.s += __shfl_xor_sync(0xffffffffu, wst.s, o);
+      }
+      if (lane == 0) wstat[r][sub] = wst;
     }
     __syncthreads();
-    if (tid < nr) {
-      RowStat st = wstat[tid][0];
-      for (int w = 1; w < kVfWarps; ++w) st = join(st, wstat[tid][w], a.inv_t_log2);
-      stat[tid] = st;
+    if (r0 > 0) cluster.sync();  // everybody has read the last rows' statistics
+    for (int idx = tid; idx < nr * kVfCtas; idx += kVfThreads) {  // a thread per (row, CTA to tell)
+      RowStat st = wstat[idx / kVfCtas][0];
+      for (int w = 1; w < wpr; ++w) st = join(st, wstat[idx / kVfCtas][w], c);
+      *cluster.map_shared_rank(&stat[idx / kVfCtas][rank], idx % kVfCtas) = st;
     }
     cluster.sync();
     if (tid < nr) {
-      RowStat st = *cluster.map_shared_rank(&stat[tid], 0);
-      for (int c = 1; c < kVfCtas; ++c) st = join(st, *cluster.map_shared_rank(&stat[tid], c), a.inv_t_log2);
+      RowStat st = stat[tid][0];
+#pragma unroll
+      for (int k = 1; k < kVfCtas; ++k) st = join(st, stat[tid][k], c);
       full[tid] = st;
     }
-    cluster.sync();  // also: the ranges' statistics have been read
-    for (int r = 0; r < nr; ++r) {
-      const RowStat st = full[r];
-      at = st;
-      const int rr = begin + r0 + r;
-      if (r0 + r == rows - 1) {
-        decided = true;
-        break;
-      }
-      const int x = a.drafts[rr];
+    __syncthreads();
+    // the accept decisions, a row to a lane
+    for (int rb = 0; rb < nr && !decided; rb += 32) {
+      const int r = rb + lane;
       bool take = false;
-      if (x >= 0 && x < a.vocab && st.m > -INFINITY) {
-        if (a.greedy) {
-          take = x == st.i;
-        } else {
-          const float lx = logit(logits + (int64_t)rr * a.ld_logits + x);
-          const float qx = a.probs ? a.probs[(int64_t)rr * a.ld_probs + x] : 1.f;
-          const float wx = lx == -INFINITY ? 0.f : weight32(lx, st.m, a.inv_t_log2);
-          take = (double)a.accept_u[rr] * qx * st.s < wx;
+      if (r < nr && r0 + r < rows - 1) {
+        const int rr = begin + r0 + r, x = a.drafts[rr];
+        const RowStat st = full[r];
+        if (x >= 0 && x < a.vocab && st.m > -INFINITY) {
+          if constexpr (kGreedy) {
+            take = x == st.i;
+          } else {
+            const float lx = logit(logits + (int64_t)rr * a.ld_logits + x);
+            const float qx = a.probs ? a.probs[(int64_t)rr * a.ld_probs + x] : 1.f;
+            const float wx = lx == -INFINITY ? 0.f : lx == st.m ? 1.f : exp2f((lx - st.m) * c);
+            take = (double)a.accept_u[rr] * qx * st.s < wx;
+          }
         }
       }
-      if (!take) {
+      const unsigned stop = __ballot_sync(0xffffffffu, !take);
+      const int k = stop ? __ffs(stop) - 1 : 32;  // the first row that is not taken (or is the last)
+      const int n = min(k, nr - rb);
+      count += n;
+      if (n < nr - rb && n < 32) {
         decided = true;
-        break;
+        at = full[rb + n];
       }
-      ++count;
     }
     __syncthreads();  // full is written again for the next rows
   }
 
   int last = -1;
   if (rows > 0 && at.m > -INFINITY) {
-    if (a.greedy) {
+    if constexpr (kGreedy) {
       last = at.i;
     } else {
       const int rr = begin + count;
@@ -196,109 +283,150 @@ __global__ void __cluster_dims__(kVfCtas, 1, 1) __launch_bounds__(kVfThreads) ve
       const T* row = logits + (int64_t)rr * a.ld_logits;
       const int x = rejected && a.probs == nullptr ? a.drafts[rr] : -1;  // a point mass is taken out
       const float* q = rejected && a.probs != nullptr ? a.probs + (int64_t)rr * a.ld_probs : nullptr;
-      // weights of p by warp, and, without q, of what is drawn from
-      double sp = 0.0, sd = 0.0, z = 1.0;
-      for (int i = w0 + lane; i < w1; i += 32) {
-        const double w = weight64(logit(row + i), at.m, a.inv_t);
-        sp += w;
-        if (i != x) sd += w;
-      }
+      const double m64 = (double)at.m, t256 = a.inv_t * kTangScale;
+      // The warp's range in vocabulary order, in blocks of 32 values a lane: value
+      // k of lane L is base + 32 k + L.  Up to 2^17 entries a warp has one block,
+      // whose weights stay in registers from the first sum to the draw.
+      constexpr int K = 32;
+      const int per_warp = (per_cta + kVfWarps - 1) / kVfWarps;
+      const int w0 = min(a.vocab, 8 * min(u1, u0 + warp * per_warp));
+      const int w1 = min(a.vocab, 8 * min(u1, u0 + (warp + 1) * per_warp));
+      const int blocks = max(1, (w1 - w0 + 32 * K - 1) / (32 * K));
+      double w[K];
       auto warp_sum = [](double v) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         return v;
       };
-      auto share = [&](double p, double d) {  // warps' sums to shared memory, CTAs' sums to the cluster
-        p = warp_sum(p), d = warp_sum(d);
-        if (lane == 0) wsum[0][warp] = p, wsum[1][warp] = d;
-        __syncthreads();
-        if (tid < 2) {
-          double s = 0.0;
-          for (int w = 0; w < kVfWarps; ++w) s += wsum[tid][w];
-          csum[tid] = s;
-        }
-        cluster.sync();
-      };
-      auto total = [&](int which) {
-        double s = 0.0;
-        for (int c = 0; c < kVfCtas; ++c) s += *cluster.map_shared_rank(&csum[which], c);
-        return s;
-      };
-      auto rest = [&](int i) -> double {  // what index i may still be drawn with
-        const double w = weight64(logit(row + i), at.m, a.inv_t);
-        if (q == nullptr) return i == x ? 0.0 : w;
-        const double d = w / z - (double)q[i];
-        return d > 0.0 ? d : 0.0;
-      };
-      share(sp, sd);
-      if (q != nullptr) {
-        z = total(0);
-        sd = 0.0;
-        for (int i = w0 + lane; i < w1; i += 32) sd += rest(i);
-        cluster.sync();  // the sums have been read
-        share(sp, sd);
-      }
-      int which = 1;
-      double sum = total(1);
-      if (!(sum > 0.0)) which = 0, sum = total(0);  // p <= q everywhere: p itself
-      double before = 0.0;
-      for (int c = 0; c < rank; ++c) before += *cluster.map_shared_rank(&csum[which], c);
-      double mine = 0.0;
-      for (int w = 0; w < warp; ++w) before += wsum[which][w];
-      mine = wsum[which][warp];
-      const double goal = (double)a.sample_u[b] * sum;
-      // the first warp in order whose range passes the goal; rounding may leave
-      // the goal beyond all of them: the last range with weight then
-      __shared__ int found[kVfWarps], some[kVfWarps];
-      if (lane == 0) found[warp] = before + mine > goal && mine > 0.0, some[warp] = mine > 0.0;
-      cluster.sync();
-      int owner = -1, fallback = -1;
-      for (int w = lane; w < kVfCtas * kVfWarps; w += 32) {
-        if (*cluster.map_shared_rank(&found[w % kVfWarps], w / kVfWarps) && owner < 0) owner = w;
-        if (*cluster.map_shared_rank(&some[w % kVfWarps], w / kVfWarps)) fallback = w;
-      }
-      owner = owner < 0 ? 0x7FFFFFFF : owner;
+      auto lane_sum = [&]() {
+        double s0 = 0.0, s1 = 0.0;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        owner = min(owner, __shfl_xor_sync(0xffffffffu, owner, o));
-        fallback = max(fallback, __shfl_xor_sync(0xffffffffu, fallback, o));
-      }
-      if (owner == 0x7FFFFFFF) owner = fallback;
-      if (owner == rank * kVfWarps + warp) {
-        // this warp's range in 32 contiguous pieces, then the piece itself
-        auto weight = [&](int i) { return which ? rest(i) : weight64(logit(row + i), at.m, a.inv_t); };
-        auto scan = [&](double v) {
+        for (int k = 0; k < K; k += 2) s0 += w[k], s1 += w[k + 1];
+        return s0 + s1;
+      };
+      auto weights = [&](int blk) {  // of p
+        const int i0 = w0 + blk * 32 * K + lane;
+        float v[K];
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double u = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += u;
+        for (int k = 0; k < K; ++k) v[k] = i0 + 32 * k < w1 ? logit(row + i0 + 32 * k) : -INFINITY;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          w[k] = i0 + 32 * (k & ~7) - lane >= w1 ? 0.0 : i0 + 32 * k < w1 ? weight64(v[k], m64, t256, table) : 0.0;
+      };
+      double inv_z = 1.0;
+      auto left = [&](int blk) {  // what may still be drawn, from the weights of p
+        const int i0 = w0 + blk * 32 * K + lane;
+        if (q == nullptr) {
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+            if (i0 + 32 * k == x) w[k] = 0.0;
+        } else {
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            const double d = i0 + 32 * k < w1 ? w[k] * inv_z - (double)__ldg(q + i0 + 32 * k) : 0.0;
+            w[k] = d > 0.0 ? d : 0.0;
           }
-          return v;
-        };
-        int lo = w0, hi = w1;
-        double base = before;
-        while (hi - lo > 0) {
-          const int piece = (hi - lo + 31) / 32;
-          const int i0 = min(hi, lo + lane * piece), i1 = min(hi, i0 + piece);
-          double s = 0.0;
-          for (int i = i0; i < i1; ++i) s += weight(i);
-          const double upto = base + scan(s);
-          const unsigned over = __ballot_sync(0xffffffffu, s > 0.0 && upto > goal);
-          const unsigned any = __ballot_sync(0xffffffffu, s > 0.0);
-          const int k = over ? __ffs(over) - 1 : 31 - __clz(any | 1u);
-          base = __shfl_sync(0xffffffffu, upto - s, k);
-          lo = __shfl_sync(0xffffffffu, i0, k);
-          hi = __shfl_sync(0xffffffffu, i1, k);
-          if (piece == 1) break;
         }
-        if (lane == 0 && count < a.max_rows) a.tokens[(int64_t)b * a.ld_tokens + count] = lo;
+      };
+      auto tell = [&](double (*sums)[kVfWarps], double v) {  // this warp's sum to every CTA
+        v = warp_sum(v);
+        if (lane < kVfCtas) *cluster.map_shared_rank(&sums[rank][warp], lane) = v;
+      };
+      auto total = [&](double (*sums)[kVfWarps]) {  // in one order, so that all warps have the same
+        double v = 0.0;
+#pragma unroll
+        for (int k = 0; k < kVfCtas * kVfWarps / 32; ++k) v += (&sums[0][0])[32 * k + lane];
+        return warp_sum(v);
+      };
+      double sp = 0.0, sd = 0.0;
+      for (int blk = 0; blk < blocks; ++blk) {
+        weights(blk);
+        sp += lane_sum();
+        if (q == nullptr) {
+          left(blk);
+          sd += lane_sum();
+        }
       }
-      cluster.sync();  // nobody leaves while others read its shared memory
+      tell(zsum, sp);
+      if (q != nullptr) {
+        cluster.sync();
+        inv_z = 1.0 / total(zsum);
+        for (int blk = 0; blk < blocks; ++blk) {
+          if (blocks > 1) weights(blk);
+          left(blk);
+          sd += lane_sum();
+        }
+      }
+      tell(rsum, sd);
+      cluster.sync();
+      const bool any = total(rsum) > 0.0;  // not so: p <= q everywhere, p itself is drawn from
+      const double(*sums)[kVfWarps] = any ? rsum : zsum;
+      const double goal = (double)a.sample_u[b] * total(const_cast<double(*)[kVfWarps]>(sums));
+      // every warp finds the range that passes the goal: the first in order;
+      // rounding may leave the goal beyond all of them: the last with weight then
+      constexpr int P = kVfCtas * kVfWarps / 32;  // ranges of a lane
+      double mine[P], before = 0.0;
+#pragma unroll
+      for (int k = 0; k < P; ++k) mine[k] = (&sums[0][0])[P * lane + k], before += mine[k];
+      {
+        const double own = before;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double v = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += v;
+        }
+        before -= own;
+      }
+      int owner = 0x7FFFFFFF, fallback = -1;
+      double base = 0.0, base_last = 0.0;
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        if (mine[k] > 0.0) {
+          fallback = P * lane + k, base_last = before;
+          if (owner == 0x7FFFFFFF && before + mine[k] > goal) owner = P * lane + k, base = before;
+        }
+        before += mine[k];
+      }
+      const int first = __reduce_min_sync(0xffffffffu, owner), end = __reduce_max_sync(0xffffffffu, fallback);
+      const int chosen = first == 0x7FFFFFFF ? end : first;
+      base = __shfl_sync(0xffffffffu, first == 0x7FFFFFFF ? base_last : base, max(chosen, 0) / P);
+      if (chosen == rank * kVfWarps + warp) {
+        int token = -1, token_last = w0;
+        for (int blk = 0; blk < blocks && token < 0; ++blk) {
+          if (blocks > 1 || !any) {
+            weights(blk);
+            if (any) left(blk);
+          }
+          // sums of 32 consecutive values; the group and the value that pass the goal
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            const double s = warp_sum(w[k]);
+            if (token < 0 && s > 0.0) {
+              const int i = w0 + blk * 32 * K + 32 * k;
+              const unsigned some = __ballot_sync(0xffffffffu, w[k] > 0.0);
+              token_last = i + 31 - __clz(some);
+              if (base + s > goal) {
+                double v = w[k];
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                  const double u = __shfl_up_sync(0xffffffffu, v, o);
+                  if (lane >= o) v += u;
+                }
+                const unsigned over = __ballot_sync(0xffffffffu, w[k] > 0.0 && base + v > goal);
+                token = over ? i + __ffs(over) - 1 : token_last;
+              }
+              base += s;
+            }
+          }
+        }
+        if (token < 0) token = token_last;
+        if (lane == 0 && count < a.max_rows) a.tokens[(int64_t)b * a.ld_tokens + count] = token;
+      }
     }
   }
   if (rank == 0) {
     if (tid == 0) a.accepted[b] = count;
-    const bool drawn = rows > 0 && at.m > -INFINITY && !a.greedy;  // its owner writes the token
+    const bool drawn = rows > 0 && at.m > -INFINITY && !kGreedy;  // its owner writes the token
     for (int j = tid; j < a.max_rows; j += kVfThreads) {
       if (j == count && drawn) continue;
       a.tokens[(int64_t)b * a.ld_tokens + j] = j < count ? a.drafts[begin + j] : j == count ? last : -1;
@@ -316,8 +444,11 @@ cudaError_t launch_verify(const VerifyArgs& a, int n_seqs, bool bf16, cudaStream
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return bf16 ? cudaLaunchKernelEx(&cfg, verify_kernel<__nv_bfloat16>, a)
-              : cudaLaunchKernelEx(&cfg, verify_kernel<float>, a);
+  if (a.greedy)
+    return bf16 ? cudaLaunchKernelEx(&cfg, verify_kernel<__nv_bfloat16, true>, a)
+                : cudaLaunchKernelEx(&cfg, verify_kernel<float, true>, a);
+  return bf16 ? cudaLaunchKernelEx(&cfg, verify_kernel<__nv_bfloat16, false>, a)
+              : cudaLaunchKernelEx(&cfg, verify_kernel<float, false>, a);
 }
 
 int verify_launch(const draco_verify_args& v, cudaStream_t st, char* msg, size_t ml) {
