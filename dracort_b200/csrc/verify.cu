@@ -8,11 +8,11 @@
 // last row from p itself: the first index whose cumulative weight exceeds
 // u times the total.  T = 0: the first index of the largest logit.
 //
-// Bound by bytes: the logits are read once.  One cluster of 8 CTAs per
+// Bound by bytes: the logits are read once.  One cluster of 8 or 16 CTAs per
 // sequence, the vocabulary cut into one range per CTA, so that one launch does
 // everything: row maxima and sums meet in distributed shared memory, every CTA
 // walks the same accept decisions, and only the row that is drawn from is read
-// a second time (from L2).  Sums of exponentials that decide an acceptance are
+// again (from L2).  Sums of exponentials that decide an acceptance are
 // fp32 (their error of about 1e-7 moves a decision as rarely); the cumulative
 // weights of the drawn row are fp64, since an index out of 10^5 hangs on
 // differences of one in 10^5 or less.
@@ -27,9 +27,10 @@ namespace draco {
 
 namespace cg = cooperative_groups;
 
-constexpr int kVfCtas = 8;
-constexpr int kVfThreads = 512;
+constexpr int kVfCtas = 16;  // CTAs of a cluster at most
+constexpr int kVfThreads = 384;
 constexpr int kVfWarps = kVfThreads / 32;
+constexpr int kVfBlocks = 16;
 constexpr int kVfRows = 64;  // rows whose statistics are held at a time
 
 struct VerifyArgs {
@@ -102,6 +103,21 @@ __device__ __forceinline__ double weight64(float x, double m, double t256, const
   return xd == m ? 1.0 : exp2_256((xd - m) * t256, table);
 }
 
+// pairs of fp32 values
+__device__ __forceinline__ uint64_t pair_2(float a, float b) {
+  return ((uint64_t)__float_as_uint(b) << 32) | __float_as_uint(a);
+}
+__device__ __forceinline__ uint64_t add_2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // 16 bytes of logits as fp32
 template <typename T, int V>
 __device__ __forceinline__ void unpack16(const uint4& w, float (&x)[V]) {
@@ -114,24 +130,25 @@ __device__ __forceinline__ void unpack16(const uint4& w, float (&x)[V]) {
 }
 
 template <typename T, bool kGreedy>
-__global__ void __cluster_dims__(kVfCtas, 1, 1) __launch_bounds__(kVfThreads) verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kVfThreads, 3) verify_kernel(const VerifyArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
   __shared__ RowStat wstat[kVfRows][kVfWarps];     // this CTA's range, by warp
   __shared__ RowStat stat[kVfRows][kVfCtas];       // every CTA's range (each writes its column everywhere)
   __shared__ RowStat full[kVfRows];                // the whole row
   __shared__ double zsum[kVfCtas][kVfWarps];       // weights of p, by CTA and warp
   __shared__ double rsum[kVfCtas][kVfWarps];       // what is drawn from
+  __shared__ double bsum[kVfWarps][kVfBlocks];     // of the warp's blocks of 256 values, the last told sums
   __shared__ double table[kGreedy ? 1 : kTable];   // 2^(j / 256)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (!kGreedy && tid < kTable) table[tid] = exp2((double)tid / kTable);
   grid_dependency_wait();
   grid_launch_dependents();
-  const int rank = (int)cluster.block_rank(), b = blockIdx.x / kVfCtas;
+  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks(), b = blockIdx.x / ctas;
   const T* logits = static_cast<const T*>(a.logits);
   const int begin = min(max(a.row_start[b], 0), a.n);
   const int rows = max(0, min(max(a.row_start[b + 1], 0), a.n) - begin);
   // the CTA's range of the vocabulary, in units of 8 values
-  const int units = (a.vocab + 7) / 8, per_cta = (units + kVfCtas - 1) / kVfCtas;
+  const int units = (a.vocab + 7) / 8, per_cta = (units + ctas - 1) / ctas;
   const int u0 = min(units, rank * per_cta), u1 = min(units, u0 + per_cta);
   const float c = a.inv_t_log2;
 
@@ -140,14 +157,14 @@ __global__ void __cluster_dims__(kVfCtas, 1, 1) __launch_bounds__(kVfThreads) ve
   RowStat at = {-INFINITY, 0.f, 0};  // statistics of the row that the next token comes from
   for (int r0 = 0; r0 < rows && !decided; r0 += kVfRows) {
     const int nr = min(kVfRows, rows - r0);
-    // Rows side by side, 16 / nr warps each (a warp takes a row's whole share
+    // Rows side by side, 12 / nr warps each (a warp takes a row's whole share
     // of the range when there are more): few long streams instead of many short
     // ones whose latencies would add up.
     const int side = min(nr, kVfWarps), wpr = kVfWarps / side, sub = warp % wpr;
     const int per_sub = (u1 - u0 + wpr - 1) / wpr;
     const int w0 = min(a.vocab, 8 * min(u1, u0 + sub * per_sub)), w1 = min(a.vocab, 8 * min(u1, u0 + (sub + 1) * per_sub));
     for (int r = warp / wpr; r < nr && warp < side * wpr; r += side) {
-      constexpr int V = 16 / (int)sizeof(T), B = 32 / V;  // values of a load, loads in flight: 32 values of a lane
+      constexpr int V = 16 / (int)sizeof(T), B = 16 / V;  // values of a load, loads in flight: 16 values of a lane
       const T* row = logits + (int64_t)(begin + r0 + r) * a.ld_logits + w0;
       const int len = w1 - w0;
       // values before the first 16-byte boundary
@@ -171,16 +188,23 @@ __global__ void __cluster_dims__(kVfCtas, 1, 1) __launch_bounds__(kVfThreads) ve
 #pragma unroll
         for (int e = 0; e < B; ++e) {
           unpack16<T, V>(buf[e], x[e]);
-          const bool on = v0 + 32 * e + lane < vecs;
 #pragma unroll
-          for (int k = 0; k < V; ++k) x[e][k] = on ? x[e][k] : -INFINITY;
+          for (int k = 0; k < V; ++k) x[e][k] = fmaxf(x[e][k], -INFINITY);  // a NaN logit is never drawn
+        }
+        if (v0 + 32 * B > vecs) {
+#pragma unroll
+          for (int e = 0; e < B; ++e)
+            if (v0 + 32 * e + lane >= vecs) {
+#pragma unroll
+              for (int k = 0; k < V; ++k) x[e][k] = -INFINITY;
+            }
         }
         if (v0 + 32 * B < vecs) fetch(v0 + 32 * B);
         float mx = -INFINITY;
 #pragma unroll
         for (int e = 0; e < B; ++e)
 #pragma unroll
-          for (int k = 0; k < V; ++k) mx = fmaxf(mx, x[e][k]);  // (passes over a NaN)
+          for (int k = 0; k < V; ++k) mx = fmaxf(mx, x[e][k]);
         if constexpr (kGreedy) {
           if (mx >= st.m && mx > -INFINITY) {
             int first = 0x7FFFFFFF;
@@ -198,13 +222,15 @@ __global__ void __cluster_dims__(kVfCtas, 1, 1) __launch_bounds__(kVfThreads) ve
             st.m = mx;
           }
           if (st.m < INFINITY) {
+            // (x - m) c in pairs: the difference first, which is exact where it counts
+            const float nm = -st.m;
             float s0 = 0.f, s1 = 0.f;
 #pragma unroll
             for (int e = 0; e < B; ++e)
 #pragma unroll
               for (int k = 0; k < V; k += 2) {
-                const float u = fast_exp2f((x[e][k] - st.m) * c), v = fast_exp2f((x[e][k + 1] - st.m) * c);
-                s0 += u == u ? u : 0.f, s1 += v == v ? v : 0.f;
+                const uint64_t y = mul_2(add_2(pair_2(x[e][k], x[e][k + 1]), pair_2(nm, nm)), pair_2(c, c));
+                s0 += fast_exp2f(__uint_as_float((uint32_t)y)), s1 += fast_exp2f(__uint_as_float((uint32_t)(y >> 32)));
               }
             st.s += s0 + s1;
           } else {  // an infinite logit has all the weight
@@ -231,16 +257,24 @@ __global__ void __cluster_dims__(kVfCtas, 1, 1) __launch_bounds__(kVfThreads) ve
     __syncthreads();
     if (r0 > 0) cluster.sync();  // everybody has read the last rows' statistics
     for (int idx = tid; idx < nr * kVfCtas; idx += kVfThreads) {  // a thread per (row, CTA to tell)
+      if (idx % kVfCtas >= ctas) continue;
       RowStat st = wstat[idx / kVfCtas][0];
       for (int w = 1; w < wpr; ++w) st = join(st, wstat[idx / kVfCtas][w], c);
       *cluster.map_shared_rank(&stat[idx / kVfCtas][rank], idx % kVfCtas) = st;
     }
     cluster.sync();
-    if (tid < nr) {
-      RowStat st = stat[tid][0];
+    for (int r = warp; r < nr; r += kVfWarps) {  // a warp per row joins the CTAs' parts
+      RowStat st = {-INFINITY, 0.f, 0x7FFFFFFF};
+      if (lane < ctas) st = stat[r][lane];
 #pragma unroll
-      for (int k = 1; k < kVfCtas; ++k) st = join(st, stat[tid][k], c);
-      full[tid] = st;
+      for (int o = kVfCtas / 2; o > 0; o >>= 1) {
+        RowStat x;
+        x.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+        x.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+        x.i = __shfl_xor_sync(0xffffffffu, st.i, o);
+        st = join(st, x, c);
+      }
+      if (lane == 0) full[r] = st;
     }
     __syncthreads();
     // the accept decisions, a row to a lane
@@ -284,14 +318,14 @@ __global__ void __cluster_dims__(kVfCtas, 1, 1) __launch_bounds__(kVfThreads) ve
       const int x = rejected && a.probs == nullptr ? a.drafts[rr] : -1;  // a point mass is taken out
       const float* q = rejected && a.probs != nullptr ? a.probs + (int64_t)rr * a.ld_probs : nullptr;
       const double m64 = (double)at.m, t256 = a.inv_t * kTangScale;
-      // The warp's range in vocabulary order, in blocks of 32 values a lane: value
-      // k of lane L is base + 32 k + L.  Up to 2^17 entries a warp has one block,
-      // whose weights stay in registers from the first sum to the draw.
-      constexpr int K = 32;
+      // The warp's range in vocabulary order, in blocks of K values a lane: value
+      // k of lane L is base + 32 k + L.
+      constexpr int K = 8;
       const int per_warp = (per_cta + kVfWarps - 1) / kVfWarps;
       const int w0 = min(a.vocab, 8 * min(u1, u0 + warp * per_warp));
       const int w1 = min(a.vocab, 8 * min(u1, u0 + (warp + 1) * per_warp));
-      const int blocks = max(1, (w1 - w0 + 32 * K - 1) / (32 * K));
+      if (q != nullptr)  // on its way while the weights of p are summed
+        for (int i = w0 + 32 * lane; i < w1; i += 1024) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));
       double w[K];
       auto warp_sum = [](double v) {
 #pragma unroll
@@ -304,70 +338,76 @@ __global__ void __cluster_dims__(kVfCtas, 1, 1) __launch_bounds__(kVfThreads) ve
         for (int k = 0; k < K; k += 2) s0 += w[k], s1 += w[k + 1];
         return s0 + s1;
       };
-      auto weights = [&](int blk) {  // of p
-        const int i0 = w0 + blk * 32 * K + lane;
-        float v[K];
+      double inv_z = 1.0;
+      auto weights = [&](int i0, bool of_p) {  // of p, or of what may still be drawn
+        float v[K], u[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) v[k] = i0 + 32 * k < w1 ? logit(row + i0 + 32 * k) : -INFINITY;
+        if (!of_p && q != nullptr) {
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-          w[k] = i0 + 32 * (k & ~7) - lane >= w1 ? 0.0 : i0 + 32 * k < w1 ? weight64(v[k], m64, t256, table) : 0.0;
-      };
-      double inv_z = 1.0;
-      auto left = [&](int blk) {  // what may still be drawn, from the weights of p
-        const int i0 = w0 + blk * 32 * K + lane;
-        if (q == nullptr) {
+          for (int k = 0; k < K; ++k) u[k] = i0 + 32 * k < w1 ? __ldg(q + i0 + 32 * k) : 0.f;
+        }
 #pragma unroll
-          for (int k = 0; k < K; ++k)
-            if (i0 + 32 * k == x) w[k] = 0.0;
-        } else {
-#pragma unroll
-          for (int k = 0; k < K; ++k) {
-            const double d = i0 + 32 * k < w1 ? w[k] * inv_z - (double)__ldg(q + i0 + 32 * k) : 0.0;
-            w[k] = d > 0.0 ? d : 0.0;
+        for (int k = 0; k < K; ++k) {
+          w[k] = weight64(v[k], m64, t256, table);
+          if (!of_p) {
+            if (q != nullptr) {
+              const double d = w[k] * inv_z - (double)u[k];
+              w[k] = d > 0.0 ? d : 0.0;
+            } else if (i0 + 32 * k == x) {
+              w[k] = 0.0;
+            }
           }
         }
       };
-      auto tell = [&](double (*sums)[kVfWarps], double v) {  // this warp's sum to every CTA
-        v = warp_sum(v);
-        if (lane < kVfCtas) *cluster.map_shared_rank(&sums[rank][warp], lane) = v;
+      // sums of the warp's range, to every CTA, and block by block for the warp itself
+      auto tell = [&](double (*sums)[kVfWarps], bool of_p) {
+        double all = 0.0;
+        for (int i = w0, j = 0; i < w1; i += 32 * K, ++j) {
+          weights(i + lane, of_p);
+          const double v = warp_sum(lane_sum());
+          if (j < kVfBlocks && lane == 0) bsum[warp][j] = v;
+          all += v;
+        }
+        if (lane < ctas) *cluster.map_shared_rank(&sums[rank][warp], lane) = all;
       };
-      auto total = [&](double (*sums)[kVfWarps]) {  // in one order, so that all warps have the same
+      constexpr int P = kVfCtas * kVfWarps / 32;  // ranges of a lane, in order
+      auto total = [&](const double (*sums)[kVfWarps], double (&mine)[P]) {
         double v = 0.0;
 #pragma unroll
-        for (int k = 0; k < kVfCtas * kVfWarps / 32; ++k) v += (&sums[0][0])[32 * k + lane];
-        return warp_sum(v);
+        for (int k = 0; k < P; ++k) {
+          mine[k] = (P * lane + k) / kVfWarps < ctas ? (&sums[0][0])[P * lane + k] : 0.0;
+          v += mine[k];
+        }
+        return warp_sum(v);  // (the same in every warp: one order)
       };
-      double sp = 0.0, sd = 0.0;
-      for (int blk = 0; blk < blocks; ++blk) {
-        weights(blk);
-        sp += lane_sum();
-        if (q == nullptr) {
-          left(blk);
-          sd += lane_sum();
+      double mine[P];
+      tell(zsum, true);
+      const double(*drawn_from)[kVfWarps] = zsum;
+      if (rejected) {
+        if (q != nullptr) {
+          cluster.sync();
+          inv_z = 1.0 / total(zsum, mine);
         }
-      }
-      tell(zsum, sp);
-      if (q != nullptr) {
-        cluster.sync();
-        inv_z = 1.0 / total(zsum);
-        for (int blk = 0; blk < blocks; ++blk) {
-          if (blocks > 1) weights(blk);
-          left(blk);
-          sd += lane_sum();
+        if (q != nullptr || (x >= w0 && x < w1)) {
+          tell(rsum, false);
+        } else {  // a range that the point mass does not touch
+          __syncwarp();
+          if (lane < ctas) *cluster.map_shared_rank(&rsum[rank][warp], lane) = zsum[rank][warp];
         }
+        drawn_from = rsum;
       }
-      tell(rsum, sd);
       cluster.sync();
-      const bool any = total(rsum) > 0.0;  // not so: p <= q everywhere, p itself is drawn from
-      const double(*sums)[kVfWarps] = any ? rsum : zsum;
-      const double goal = (double)a.sample_u[b] * total(const_cast<double(*)[kVfWarps]>(sums));
+      double all = total(drawn_from, mine);
+      bool of_p = !rejected;
+      const bool fallback_p = rejected && !(all > 0.0);  // p <= q everywhere: p itself is drawn from
+      if (fallback_p) all = total(zsum, mine), of_p = true;
+      const double goal = (double)a.sample_u[b] * all;
       // every warp finds the range that passes the goal: the first in order;
       // rounding may leave the goal beyond all of them: the last with weight then
-      constexpr int P = kVfCtas * kVfWarps / 32;  // ranges of a lane
-      double mine[P], before = 0.0;
+      double before = 0.0;
 #pragma unroll
-      for (int k = 0; k < P; ++k) mine[k] = (&sums[0][0])[P * lane + k], before += mine[k];
+      for (int k = 0; k < P; ++k) before += mine[k];
       {
         const double own = before;
 #pragma unroll
@@ -392,20 +432,26 @@ __global__ void __cluster_dims__(kVfCtas, 1, 1) __launch_bounds__(kVfThreads) ve
       base = __shfl_sync(0xffffffffu, first == 0x7FFFFFFF ? base_last : base, max(chosen, 0) / P);
       if (chosen == rank * kVfWarps + warp) {
         int token = -1, token_last = w0;
-        for (int blk = 0; blk < blocks && token < 0; ++blk) {
-          if (blocks > 1 || !any) {
-            weights(blk);
-            if (any) left(blk);
+        for (int i = w0, j = 0; i < w1 && token < 0; i += 32 * K, ++j) {
+          if (j < kVfBlocks && !fallback_p && i + 32 * K < w1) {  // a block that stays below the goal
+            const double v = bsum[warp][j];
+            if (v > 0.0 && base + v <= goal) {
+              token_last = -2 - i;  // (its last value with weight is looked for only if nothing follows)
+              base += v;
+              continue;
+            }
+            if (!(v > 0.0)) continue;
           }
+          weights(i + lane, of_p);
           // sums of 32 consecutive values; the group and the value that pass the goal
+          double s[K];
+#pragma unroll
+          for (int k = 0; k < K; ++k) s[k] = warp_sum(w[k]);
 #pragma unroll
           for (int k = 0; k < K; ++k) {
-            const double s = warp_sum(w[k]);
-            if (token < 0 && s > 0.0) {
-              const int i = w0 + blk * 32 * K + 32 * k;
-              const unsigned some = __ballot_sync(0xffffffffu, w[k] > 0.0);
-              token_last = i + 31 - __clz(some);
-              if (base + s > goal) {
+            if (token < 0 && s[k] > 0.0) {
+              token_last = i + 32 * k + 31 - __clz(__ballot_sync(0xffffffffu, w[k] > 0.0));
+              if (base + s[k] > goal) {
                 double v = w[k];
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -413,10 +459,19 @@ __global__ void __cluster_dims__(kVfCtas, 1, 1) __launch_bounds__(kVfThreads) ve
                   if (lane >= o) v += u;
                 }
                 const unsigned over = __ballot_sync(0xffffffffu, w[k] > 0.0 && base + v > goal);
-                token = over ? i + __ffs(over) - 1 : token_last;
+                token = over ? i + 32 * k + __ffs(over) - 1 : token_last;
               }
-              base += s;
+              base += s[k];
             }
+          }
+        }
+        if (token < 0 && token_last < 0) {  // rounding: the last value with weight of the block noted
+          const int i = -2 - token_last;
+          weights(i + lane, of_p);
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            const unsigned some = __ballot_sync(0xffffffffu, w[k] > 0.0);
+            if (some) token_last = i + 32 * k + 31 - __clz(some);
           }
         }
         if (token < 0) token = token_last;
@@ -434,21 +489,38 @@ __global__ void __cluster_dims__(kVfCtas, 1, 1) __launch_bounds__(kVfThreads) ve
   }
 }
 
-cudaError_t launch_verify(const VerifyArgs& a, int n_seqs, bool bf16, cudaStream_t st) {
-  cudaLaunchAttribute attr[1];
+// 16 CTAs a sequence while all sequences' CTAs fit the GPU at four an SM, else 8
+// (a portable cluster; with 16 only a whole GPC's SMs can host one).
+template <typename T, bool kGreedy>
+static cudaError_t launch_t(const VerifyArgs& a, int n_seqs, cudaStream_t st) {
+  static int attr_set[64] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !attr_set[dev]) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(verify_kernel<T, kGreedy>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) attr_set[dev] = 1;
+  }
+  const int ctas = (int64_t)n_seqs * kVfCtas <= 4 * device_sm_count() ? kVfCtas : kVfCtas / 2;
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)n_seqs * kVfCtas);
+  cfg.gridDim = dim3((unsigned)n_seqs * ctas);
   cfg.blockDim = dim3(kVfThreads);
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (a.greedy)
-    return bf16 ? cudaLaunchKernelEx(&cfg, verify_kernel<__nv_bfloat16, true>, a)
-                : cudaLaunchKernelEx(&cfg, verify_kernel<float, true>, a);
-  return bf16 ? cudaLaunchKernelEx(&cfg, verify_kernel<__nv_bfloat16, false>, a)
-              : cudaLaunchKernelEx(&cfg, verify_kernel<float, false>, a);
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, verify_kernel<T, kGreedy>, a);
+}
+static cudaError_t launch_verify(const VerifyArgs& a, int n_seqs, bool bf16, cudaStream_t st) {
+  if (a.greedy) return bf16 ? launch_t<__nv_bfloat16, true>(a, n_seqs, st) : launch_t<float, true>(a, n_seqs, st);
+  return bf16 ? launch_t<__nv_bfloat16, false>(a, n_seqs, st) : launch_t<float, false>(a, n_seqs, st);
 }
 
 int verify_launch(const draco_verify_args& v, cudaStream_t st, char* msg, size_t ml) {
