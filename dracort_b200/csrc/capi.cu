@@ -524,7 +524,8 @@ int draco_kv_append(const draco_kv_cache* cache, const draco_kv_append_args* arg
   if (a.n == 0) return ok();
   if (!a.k || !a.v || !a.seq || !a.pos) return fail(DRACO_ERR_ARG, "%s: null pointer", fn);
   if (a.q == nullptr) a.heads = 0;
-  if (a.heads > 65536) return fail(DRACO_ERR_SHAPE, "%s: %d heads", fn, a.heads);
+  if ((int64_t)a.n * (a.heads + 2 * c.kv_heads) > 0x7FFFFFFF)
+    return fail(DRACO_ERR_SHAPE, "%s: %d tokens of %d heads in one call", fn, a.n, a.heads + 2 * c.kv_heads);
   const int64_t hd = cache->head_dim, kw = (int64_t)c.kv_heads * hd, qw = (int64_t)a.heads * hd;
   if (a.heads > 0 && ((rc = check_rows(a.q, a.ldq, qw, dtype, fn, "q")) ||
                       (rc = check_rows(a.q_out, a.ldqo, qw, dtype, fn, "q_out"))))
@@ -550,6 +551,7 @@ int draco_kv_read(const draco_kv_cache* cache, const int* seq, const int* pos, i
   if (n < 0) return fail(DRACO_ERR_SHAPE, "%s: %d rows", fn, n);
   if (n == 0) return ok();
   if (!seq || !pos || !k_out || !v_out) return fail(DRACO_ERR_ARG, "%s: null pointer", fn);
+  if ((int64_t)n * 2 * c.kv_heads > 0x7FFFFFFF) return fail(DRACO_ERR_SHAPE, "%s: %d rows in one call", fn, n);
   const int64_t kw = (int64_t)c.kv_heads * cache->head_dim;
   if ((rc = check_rows(k_out, ldk, kw, dtype, fn, "k_out")) || (rc = check_rows(v_out, ldv, kw, dtype, fn, "v_out")))
     return rc;

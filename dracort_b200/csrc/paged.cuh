@@ -54,10 +54,10 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
   if constexpr (sizeof(T) == 4) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
     x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
   } else {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
     x[0] = bf16lo(a.x), x[1] = bf16hi(a.x), x[2] = bf16lo(a.y), x[3] = bf16hi(a.y);
     x[4] = bf16lo(a.z), x[5] = bf16hi(a.z), x[6] = bf16lo(a.w), x[7] = bf16hi(a.w);
   }

@@ -9,10 +9,14 @@
 // rule of format/quantize.py).  Read: value = d * q, exact in fp32, rounded
 // once when the output is bf16.
 //
-// Both are bound by bytes.  A thread takes 8 values of a row's lower half and
-// the 8 that rotate with them, i.e. two 16-byte accesses per operand, and
-// keeps the cos / sin values of its 8 angles in registers over `rows` rows of
-// the token (they are read from the L2 otherwise as often as the data).
+// Both are bound by bytes, and short of that by latency: position -> block table
+// -> row is a chain of loads.  A block walks a run of tokens: it looks all their
+// pages up first, then its groups (the threads of a row, in one warp) take U
+// rows of a token at a time with the next rows' loads already in flight.  A
+// thread takes 8 values of a row's lower half and the 8 that rotate with them
+// (append), or 16 in a row (read): 16-byte accesses.  A Q8_0 block's maximum
+// goes through shuffles.
+#include <algorithm>
 #include <cstdio>
 
 #include "internal.h"
@@ -21,212 +25,368 @@
 namespace draco {
 
 constexpr int kKvThreads = 256;
+constexpr int kKvTokens = 512;  // tokens whose pages a block looks up at most
 
 template <int HD>
 struct KvShape {
   static constexpr int kLanes = HD / 16;              // threads of one row
-  static constexpr int kRows = kKvThreads / kLanes;   // rows of a block at a time
-  static constexpr int kChunks = HD / 8;
+  static constexpr int kPerWarp = 32 / kLanes;        // rows of a warp (HD 96: five, two lanes idle)
+  static constexpr int kRows = kKvThreads / 32 * kPerWarp;
 };
 
-template <typename T, int HD, bool Q8>
-__global__ void __launch_bounds__(kKvThreads) kv_append_kernel(
-    PagedView c, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* q_out, int64_t ldq,
-    int64_t ldk, int64_t ldv, int64_t ldqo, const float* __restrict__ cos_t, const float* __restrict__ sin_t,
-    int64_t max_positions, const int* __restrict__ seq, const int* __restrict__ pos, int heads, int reps) {
+// The groups of a call in one sequence: token by token, group g of a token's
+// `step` takes its rows g, g + step, g + 2 step, ... (U of them).  A block takes
+// the `span` groups from blockIdx.x * span on, kRows at a time.
+struct KvWalk {
+  int n, rows, step, span;
+  unsigned total;
+};
+struct KvItem {
+  int token, row;
+  bool on;
+};
+template <int HD>
+__device__ __forceinline__ KvItem kv_item(const KvWalk& w, int k) {  // step k of the block
   using S = KvShape<HD>;
-  // largest magnitude of every 8 values of the rows in flight (a Q8_0 block is four of them)
-  __shared__ __align__(16) float amax[Q8 ? S::kRows : 1][S::kChunks];
+  const int lane = threadIdx.x & 31, at = k * S::kRows + (threadIdx.x >> 5) * S::kPerWarp + lane / S::kLanes;
+  const unsigned idx = blockIdx.x * (unsigned)w.span + at;
+  KvItem it;
+  it.on = lane / S::kLanes < S::kPerWarp && at < w.span && idx < w.total;
+  it.token = it.on ? (int)(idx / (unsigned)w.step) : (int)(blockIdx.x * (unsigned)w.span / (unsigned)w.step);
+  it.row = (int)(idx % (unsigned)w.step);
+  return it;
+}
+// pages and positions of the block's tokens (page -1: outside); returns the first token
+__device__ __forceinline__ int kv_lookup(const PagedView& c, const KvWalk& w, const int* seq, const int* pos,
+                                         int64_t max_positions, int* s_page, int* s_pos) {
+  const unsigned g0 = blockIdx.x * (unsigned)w.span, g1 = min(g0 + (unsigned)w.span, w.total);
+  const int t0 = (int)(g0 / (unsigned)w.step), t1 = (int)((g1 - 1) / (unsigned)w.step);
+  for (int t = t0 + threadIdx.x; t <= t1; t += kKvThreads) {
+    const int p = pos[t], s = seq[t];
+    s_pos[t - t0] = p;
+    s_page[t - t0] = s >= 0 && s < c.n_seqs && p >= 0 && p < max_positions ? page_of(c, s, p) : -1;
+  }
+  __syncthreads();
+  return t0;
+}
+
+__device__ __forceinline__ float max_nan2(float a, float b) {  // keeps a NaN
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// largest of the values m[2] (lower chunk, upper chunk) over the four chunks of
+// each chunk's Q8_0 block; a row's lanes are l0 .. l0 + kLanes - 1
+template <int HD>
+__device__ __forceinline__ void block_max(float (&m)[2], int lane, int l0) {
+  constexpr int L = HD / 16;
+  if constexpr (L % 4 == 0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      m[h] = max_nan2(m[h], __shfl_xor_sync(0xffffffffu, m[h], 1));
+      m[h] = max_nan2(m[h], __shfl_xor_sync(0xffffffffu, m[h], 2));
+    }
+  } else {
+    float r[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int blk = (lane - l0 + h * L) / 4;
+      r[h] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int chunk = 4 * blk + e;
+        const float a = __shfl_sync(0xffffffffu, m[0], (l0 + chunk % L) & 31);
+        const float b = __shfl_sync(0xffffffffu, m[1], (l0 + chunk % L) & 31);
+        r[h] = max_nan2(r[h], chunk < L ? a : b);
+      }
+    }
+    m[0] = r[0], m[1] = r[1];
+  }
+}
+
+// a thread's 16 values of a row as loaded: 8 of each half
+template <typename T>
+struct KvRaw {
+  uint4 w[sizeof(T) == 4 ? 4 : 2];
+};
+template <typename T>
+__device__ __forceinline__ void unpack_half(const KvRaw<T>& r, int h, float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const uint4 a = r.w[2 * h], b = r.w[2 * h + 1];
+    x[0] = __uint_as_float(a.x), x[1] = __uint_as_float(a.y), x[2] = __uint_as_float(a.z), x[3] = __uint_as_float(a.w);
+    x[4] = __uint_as_float(b.x), x[5] = __uint_as_float(b.y), x[6] = __uint_as_float(b.z), x[7] = __uint_as_float(b.w);
+  } else {
+    const uint4 a = r.w[h];
+    x[0] = bf16lo(a.x), x[1] = bf16hi(a.x), x[2] = bf16lo(a.y), x[3] = bf16hi(a.y);
+    x[4] = bf16lo(a.z), x[5] = bf16hi(a.z), x[6] = bf16lo(a.w), x[7] = bf16hi(a.w);
+  }
+}
+
+struct KvAppend {
+  const void *q, *k, *v;
+  void* q_out;
+  int64_t ldq, ldk, ldv, ldqo;
+  const float *cos_t, *sin_t;
+  int64_t max_positions;
+  const int *seq, *pos;
+  int heads;
+};
+
+template <typename T, int HD, bool Q8, int U>
+__global__ void __launch_bounds__(kKvThreads) kv_append_kernel(const PagedView c, const KvAppend a, const KvWalk wk) {
+  using S = KvShape<HD>;
+  __shared__ int s_page[kKvTokens], s_pos[kKvTokens];
   grid_dependency_wait();
   grid_launch_dependents();
-  const int i = blockIdx.x;
-  const int slot = threadIdx.x / S::kLanes, lane = threadIdx.x % S::kLanes;
-  const int total = heads + 2 * c.kv_heads;
-  const bool active = slot < S::kRows;
-  const int p = pos[i], s = seq[i];
-  const bool turn = cos_t != nullptr && p >= 0 && p < max_positions;
-  int page = -1;
-  if (s >= 0 && s < c.n_seqs && p >= 0 && (turn || cos_t == nullptr)) page = page_of(c, s, p);
-  const int off = p & ((1 << c.page_shift) - 1);
-  float cs[8], sn[8];
-  if (turn && active) {
-    load8(cos_t + (int64_t)p * (HD / 2) + 8 * lane, cs);
-    load8(sin_t + (int64_t)p * (HD / 2) + 8 * lane, sn);
-  }
-  for (int u = 0; u < reps; ++u) {
-    const int r = (blockIdx.y * reps + u) * S::kRows + slot;  // q heads, then k heads, then v heads
-    const bool row = active && r < total;
-    float x[2][8];
-    if (row) {
-      const T* src;
-      if (r < heads)
-        src = q == nullptr ? nullptr : q + (int64_t)i * ldq + (int64_t)r * HD;
-      else if (r < heads + c.kv_heads)
-        src = k + (int64_t)i * ldk + (int64_t)(r - heads) * HD;
-      else
-        src = v + (int64_t)i * ldv + (int64_t)(r - heads - c.kv_heads) * HD;
-      if (src != nullptr) {
-        load8(src + 8 * lane, x[0]);
-        load8(src + HD / 2 + 8 * lane, x[1]);
-      }
-      if (turn && r < heads + c.kv_heads) {
+  const int lane32 = threadIdx.x & 31, lane = lane32 % S::kLanes;
+  const int heads = a.heads, kend = heads + c.kv_heads;
+  const int t0 = kv_lookup(c, wk, a.seq, a.pos, a.cos_t ? a.max_positions : 0x7FFFFFFFFFFFFFFFll, s_page, s_pos);
+  KvRaw<T> raw[U];
+  auto fetch = [&](const KvItem& it) {
+    const int64_t i = it.token;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = it.row + u * wk.step;
+      if (!it.on || r >= wk.rows) continue;
+      const T* src = r < heads  ? static_cast<const T*>(a.q) + i * a.ldq + (int64_t)r * HD
+                     : r < kend ? static_cast<const T*>(a.k) + i * a.ldk + (int64_t)(r - heads) * HD
+                                : static_cast<const T*>(a.v) + i * a.ldv + (int64_t)(r - kend) * HD;
+      constexpr int N = sizeof(T) == 4 ? 2 : 1;  // 16-byte words of 8 values
+      const uint4* lo = reinterpret_cast<const uint4*>(src + 8 * lane);
+      const uint4* hi = reinterpret_cast<const uint4*>(src + HD / 2 + 8 * lane);
+#pragma unroll
+      for (int e = 0; e < N; ++e) raw[u].w[e] = lo[e], raw[u].w[N + e] = hi[e];
+    }
+  };
+  const int steps = (wk.span + S::kRows - 1) / S::kRows;
+  KvItem it = kv_item<HD>(wk, 0);
+  fetch(it);
+#pragma unroll 1
+  for (int st = 0; st < steps; ++st) {
+    const int64_t i = it.token;
+    const int p = s_pos[it.token - t0], page = it.on ? s_page[it.token - t0] : -1;
+    const int off = p & ((1 << c.page_shift) - 1);
+    const bool turn = a.cos_t != nullptr && p >= 0 && p < a.max_positions;
+    float cs[8], sn[8];
+    if (turn) {
+      load8(a.cos_t + (int64_t)p * (HD / 2) + 8 * lane, cs);
+      load8(a.sin_t + (int64_t)p * (HD / 2) + 8 * lane, sn);
+    }
+    KvRaw<T> now[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) now[u] = raw[u];
+    const KvItem next = kv_item<HD>(wk, st + 1);
+    if (st + 1 < steps) fetch(next);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = it.row + u * wk.step;
+      const bool row = it.on && r < wk.rows;
+      float x[2][8];
+      unpack_half<T>(now[u], 0, x[0]);
+      unpack_half<T>(now[u], 1, x[1]);
+      if (turn && r < kend) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float a = x[0][j], b = x[1][j];
-          x[0][j] = __fsub_rn(__fmul_rn(a, cs[j]), __fmul_rn(b, sn[j]));
-          x[1][j] = __fadd_rn(__fmul_rn(b, cs[j]), __fmul_rn(a, sn[j]));
+          const float y = x[0][j], z = x[1][j];
+          x[0][j] = __fsub_rn(__fmul_rn(y, cs[j]), __fmul_rn(z, sn[j]));
+          x[1][j] = __fadd_rn(__fmul_rn(z, cs[j]), __fmul_rn(y, sn[j]));
         }
       }
-      if (r < heads && q_out != nullptr) {
-        T* dst = q_out + (int64_t)i * ldqo + (int64_t)r * HD;
+      if (row && r < heads) {
+        T* dst = static_cast<T*>(a.q_out) + i * a.ldqo + (int64_t)r * HD;
         store8(dst + 8 * lane, x[0]);
         store8(dst + HD / 2 + 8 * lane, x[1]);
       }
-    }
-    const bool keep = row && r >= heads && page >= 0;
-    const int kvr = r - heads;
-    uint8_t* blk = nullptr;
-    if (keep)
-      blk = (kvr < c.kv_heads ? c.k : c.v) + ((int64_t)page * c.kv_heads + kvr % c.kv_heads) * c.block_bytes;
-    if constexpr (!Q8) {
-      if (keep) {
-        __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(blk) + (int64_t)off * HD;
-        store8(dst + 8 * lane, x[0]);
-        store8(dst + HD / 2 + 8 * lane, x[1]);
-      }
-    } else {
-      if (keep) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float m = 0.f;
-          bool bad = false;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            bad |= x[h][j] != x[h][j];
-            x[h][j] = fminf(fmaxf(x[h][j], -kKvLimit), kKvLimit);
-            m = fmaxf(m, fabsf(x[h][j]));
-          }
-          // a NaN makes its whole block NaN (scale NaN, quants 0)
-          amax[slot][lane + h * S::kLanes] = bad ? __int_as_float(0x7FC00000) : m;
+      const bool keep = row && r >= heads && page >= 0;
+      uint8_t* blk = nullptr;
+      if (keep)
+        blk = (r < kend ? c.k : c.v) + ((int64_t)page * c.kv_heads + (r < kend ? r - heads : r - kend)) * c.block_bytes;
+      if constexpr (!Q8) {
+        if (keep) {
+          __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(blk) + (int64_t)off * HD;
+          store8(dst + 8 * lane, x[0]);
+          store8(dst + HD / 2 + 8 * lane, x[1]);
         }
-      }
-      __syncthreads();
-      if (keep) {
+      } else if (__any_sync(0xffffffffu, keep)) {
+        float m[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int chunk = lane + h * S::kLanes;
-          const float4 a = *reinterpret_cast<const float4*>(&amax[slot][chunk & ~3]);
-          const float m = fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w));
-          const bool bad = a.x != a.x || a.y != a.y || a.z != a.z || a.w != a.w;
-          const float d = bad ? __int_as_float(0x7FC00000) : __fdiv_rn(fmaxf(m, 1e-12f), 127.f);
-          uint32_t w[2] = {0u, 0u};
-          if (!bad) {
+          m[h] = fabsf(x[h][0]);
+#pragma unroll
+          for (int j = 1; j < 8; ++j) m[h] = max_nan2(m[h], fabsf(x[h][j]));
+        }
+        block_max<HD>(m, lane32, lane32 - lane);
+        if (keep) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int chunk = lane + h * S::kLanes;
+            const bool bad = m[h] != m[h];  // a NaN makes its whole block NaN (scale NaN, quants 0)
+            if (m[h] > kKvLimit) {
+              m[h] = kKvLimit;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) x[h][j] = fminf(fmaxf(x[h][j], -kKvLimit), kKvLimit);
+            }
+            const float d = bad ? m[h] : __fdiv_rn(fmaxf(m[h], 1e-12f), 127.f);
+            // rint(x / d) with the quotient rounded to fp32: by Markstein's theorem
+            // q + (x - q d) y is the rounded quotient when y is the rounded 1 / d and
+            // q = x y (values from the block's largest down to 0: nothing underflows
+            // that matters); then 1.5 * 2^23 leaves the nearest integer in the low bits
+            const float y = 1.f / d;
+            uint32_t b[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const int n = max(-127, min(127, __float2int_rn(__fdiv_rn(x[h][j], d))));
-              w[j >> 2] |= (uint32_t)(n & 0xFF) << (8 * (j & 3));
+              const float z = x[h][j] * y;
+              b[j] = __float_as_uint(fmaf(fmaf(-z, d, x[h][j]), y, z) + 12582912.f);
             }
+            uint32_t w0 = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+            uint32_t w1 = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
+            if (bad) w0 = w1 = 0u;
+            *reinterpret_cast<uint2*>(blk + (int64_t)off * HD + 8 * chunk) = make_uint2(w0, w1);
+            if ((chunk & 3) == 0)
+              reinterpret_cast<__half*>(blk + ((int64_t)HD << c.page_shift))[off * (HD / 32) + chunk / 4] =
+                  __float2half_rn(d);
           }
-          *reinterpret_cast<uint2*>(blk + (int64_t)off * HD + 8 * chunk) = make_uint2(w[0], w[1]);
-          if ((chunk & 3) == 0)
-            reinterpret_cast<__half*>(blk + ((int64_t)HD << c.page_shift))[off * (HD / 32) + chunk / 4] =
-                __float2half_rn(d);
         }
       }
-      __syncthreads();  // amax is written again for the next rows
     }
+    it = next;
   }
 }
 
 // rows of the given positions, keys to k_out and values to v_out
-// [n, kv_heads, head_dim]; a thread takes 16 values
-template <typename T, int HD, bool Q8>
-__global__ void __launch_bounds__(kKvThreads) kv_read_kernel(PagedView c, const int* __restrict__ seq,
+// [n, kv_heads, head_dim]; a thread takes 16 values of each of its rows
+template <typename T, int HD, bool Q8, int U>
+__global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const PagedView c, const int* __restrict__ seq,
                                                              const int* __restrict__ pos, T* k_out, T* v_out,
-                                                             int64_t ldk, int64_t ldv, int reps) {
+                                                             int64_t ldk, int64_t ldv, const KvWalk wk) {
   using S = KvShape<HD>;
+  __shared__ int s_page[kKvTokens], s_pos[kKvTokens];
   grid_dependency_wait();
   grid_launch_dependents();
-  const int i = blockIdx.x;
-  const int slot = threadIdx.x / S::kLanes, lane = threadIdx.x % S::kLanes;
-  if (slot >= S::kRows) return;
-  const int p = pos[i], s = seq[i];
-  const int page = s >= 0 && s < c.n_seqs && p >= 0 ? page_of(c, s, p) : -1;
-  const int off = p & ((1 << c.page_shift) - 1);
-  for (int u = 0; u < reps; ++u) {
-    const int r = (blockIdx.y * reps + u) * S::kRows + slot;
-    if (r >= 2 * c.kv_heads) return;
-    const bool is_k = r < c.kv_heads;
-    const int h = is_k ? r : r - c.kv_heads;
-    T* dst = (is_k ? k_out + (int64_t)i * ldk : v_out + (int64_t)i * ldv) + (int64_t)h * HD + 16 * lane;
-    float x[2][8] = {};
-    if (page >= 0) {  // a row outside the cache reads as zeros
-      const uint8_t* blk = (is_k ? c.k : c.v) + ((int64_t)page * c.kv_heads + h) * c.block_bytes;
-      if constexpr (Q8) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(blk + (int64_t)off * HD + 16 * lane));
-        const float d = __half2float(reinterpret_cast<const __half*>(
-            blk + ((int64_t)HD << c.page_shift))[off * (HD / 32) + lane / 2]);
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+  const int lane = (threadIdx.x & 31) % S::kLanes;
+  const int t0 = kv_lookup(c, wk, seq, pos, 0x7FFFFFFFFFFFFFFFll, s_page, s_pos);
+  uint4 w[U][Q8 ? 1 : 2];
+  uint32_t d[U];
+  auto fetch = [&](const KvItem& it) {
+    const int page = it.on ? s_page[it.token - t0] : -1, off = s_pos[it.token - t0] & ((1 << c.page_shift) - 1);
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          x[j >> 3][j & 7] = d * (float)(int8_t)((ws[j >> 2] >> (8 * (j & 3))) & 0xFF);
+    for (int u = 0; u < U; ++u) {
+      const int r = it.row + u * wk.step, h = r < c.kv_heads ? r : r - c.kv_heads;
+      const uint8_t* blk = (r < c.kv_heads ? c.k : c.v) + ((int64_t)max(page, 0) * c.kv_heads + h) * c.block_bytes;
+      const bool have = page >= 0 && r < wk.rows;  // a row outside the cache reads as zeros
+#pragma unroll
+      for (int e = 0; e < (Q8 ? 1 : 2); ++e) {
+        w[u][e] = make_uint4(0, 0, 0, 0);
+        if (have) w[u][e] = __ldg(reinterpret_cast<const uint4*>(blk + ((int64_t)off * HD + 16 * lane) * (Q8 ? 1 : 2)) + e);
+      }
+      d[u] = 0;
+      if (Q8 && have)
+        d[u] = __ldg(reinterpret_cast<const uint16_t*>(blk + ((int64_t)HD << c.page_shift)) + off * (HD / 32) + lane / 2);
+    }
+  };
+  const int steps = (wk.span + S::kRows - 1) / S::kRows;
+  KvItem it = kv_item<HD>(wk, 0);
+  fetch(it);
+#pragma unroll 1
+  for (int st = 0; st < steps; ++st) {
+    const int64_t i = it.token;
+    uint4 now[U][Q8 ? 1 : 2];
+    float sc[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int e = 0; e < (Q8 ? 1 : 2); ++e) now[u][e] = w[u][e];
+      sc[u] = f16_bits_to_f32(d[u]);
+    }
+    const KvItem next = kv_item<HD>(wk, st + 1);
+    if (st + 1 < steps) fetch(next);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = it.row + u * wk.step, h = r < c.kv_heads ? r : r - c.kv_heads;
+      if (!it.on || r >= wk.rows) continue;
+      T* dst = (r < c.kv_heads ? k_out + i * ldk : v_out + i * ldv) + (int64_t)h * HD + 16 * lane;
+      if constexpr (Q8) {
+        const uint32_t ws[4] = {now[u][0].x ^ 0x80808080u, now[u][0].y ^ 0x80808080u, now[u][0].z ^ 0x80808080u,
+                                now[u][0].w ^ 0x80808080u};
+        float x[2][8];
+#pragma unroll
+        for (int j = 0; j < 16; ++j)  // 2^23 + (quant + 128), exact
+          x[j >> 3][j & 7] =
+              sc[u] * (__uint_as_float(__byte_perm(ws[j >> 2], 0x4B000000u, 0x7440u | (j & 3))) - 8388736.f);
+        store8(dst, x[0]);
+        store8(dst + 8, x[1]);
+      } else if constexpr (sizeof(T) == 2) {
+        reinterpret_cast<uint4*>(dst)[0] = now[u][0];
+        reinterpret_cast<uint4*>(dst)[1] = now[u][1];
       } else {
-        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(blk) + (int64_t)off * HD + 16 * lane;
-        load8(src, x[0]);
-        load8(src + 8, x[1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint4 z = now[u][e];
+          float x[8] = {bf16lo(z.x), bf16hi(z.x), bf16lo(z.y), bf16hi(z.y),
+                        bf16lo(z.z), bf16hi(z.z), bf16lo(z.w), bf16hi(z.w)};
+          store8(dst + 8 * e, x);
+        }
       }
     }
-    store8(dst, x[0]);
-    store8(dst + 8, x[1]);
+    it = next;
   }
 }
 
-// Rows of one token per block and repetitions: enough blocks to fill the GPU
-// come first; then up to 4 rows per thread.
-static void rows_grid(int n, int rows, int per_block, int* reps, unsigned* gy) {
-  const int need = (rows + per_block - 1) / per_block;
-  const int64_t want = 16LL * device_sm_count();  // 8 blocks of 256 threads fit an SM
-  int u = 1;
-  while (u < 4 && u < need && (int64_t)n * ((need + 2 * u - 1) / (2 * u)) >= want) u *= 2;
-  *reps = u;
-  *gy = (unsigned)((need + u - 1) / u);
+// U rows of a thread at a time: one while the call does not fill the GPU
+// (latency counts), else `most`.  A block's span is then what gives four blocks
+// an SM, up to 16 steps and kKvTokens tokens.
+static KvWalk kv_walk(int n, int rows, int lanes, int per_step, int most, int* unroll) {
+  KvWalk w;
+  w.n = n;
+  w.rows = rows;
+  const int64_t room = 2048LL * device_sm_count();
+  *unroll = (int64_t)n * rows * lanes > room ? most : 1;
+  w.step = (rows + *unroll - 1) / *unroll;
+  const int64_t total = (int64_t)n * w.step;
+  w.total = (unsigned)total;
+  const int64_t blocks = 4LL * device_sm_count();
+  int64_t steps = std::max<int64_t>(1, std::min<int64_t>(16, total / (blocks * per_step)));
+  while (steps > 1 && steps * per_step / w.step + 2 > kKvTokens) steps /= 2;
+  w.span = (int)(steps * per_step);
+  return w;
 }
+static_assert(kKvThreads / 2 + 2 <= kKvTokens, "one step's tokens");
 
-template <typename T, int HD, bool Q8>
-static cudaError_t append_t(const PagedView& c, const draco_kv_append_args& a, cudaStream_t st) {
-  int reps;
-  unsigned gy;
-  rows_grid(a.n, a.heads + 2 * c.kv_heads, KvShape<HD>::kRows, &reps, &gy);
+template <typename Kernel, typename... Args>
+static cudaError_t launch_walk(Kernel kernel, const KvWalk& w, cudaStream_t st, Args... args) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.n, gy);
+  cfg.gridDim = dim3((w.total + (unsigned)w.span - 1) / (unsigned)w.span);
   cfg.blockDim = dim3(kKvThreads);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv_append_kernel<T, HD, Q8>, c, (const T*)a.q, (const T*)a.k, (const T*)a.v,
-                            (T*)a.q_out, a.ldq, a.ldk, a.ldv, a.ldqo, a.cos_table, a.sin_table, a.max_positions,
-                            a.seq, a.pos, a.heads, reps);
+  return cudaLaunchKernelEx(&cfg, kernel, args..., w);
+}
+
+template <typename T, int HD, bool Q8>
+static cudaError_t append_t(const PagedView& c, const draco_kv_append_args& a, cudaStream_t st) {
+  using S = KvShape<HD>;
+  constexpr int kMost = sizeof(T) == 4 ? 2 : 4;  // 32 registers of loads in flight
+  int u;
+  const KvWalk w = kv_walk(a.n, a.heads + 2 * c.kv_heads, S::kLanes, S::kRows, kMost, &u);
+  const KvAppend k = {a.q,   a.k,    a.v,         a.q_out,     a.ldq,           a.ldk, a.ldv,
+                      a.ldqo, a.cos_table, a.sin_table, a.max_positions, a.seq, a.pos, a.heads};
+  return launch_walk(u == 1 ? kv_append_kernel<T, HD, Q8, 1> : kv_append_kernel<T, HD, Q8, kMost>, w, st, c, k);
 }
 
 template <typename T, int HD, bool Q8>
 static cudaError_t read_t(const PagedView& c, const int* seq, const int* pos, int n, void* k_out, void* v_out,
                           int64_t ldk, int64_t ldv, cudaStream_t st) {
-  int reps;
-  unsigned gy;
-  rows_grid(n, 2 * c.kv_heads, KvShape<HD>::kRows, &reps, &gy);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(n, gy);
-  cfg.blockDim = dim3(kKvThreads);
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv_read_kernel<T, HD, Q8>, c, seq, pos, (T*)k_out, (T*)v_out, ldk, ldv, reps);
+  using S = KvShape<HD>;
+  constexpr int kMost = 4;
+  int u;
+  const KvWalk w = kv_walk(n, 2 * c.kv_heads, S::kLanes, S::kRows, kMost, &u);
+  return launch_walk(u == 1 ? kv_read_kernel<T, HD, Q8, 1> : kv_read_kernel<T, HD, Q8, kMost>, w, st, c, seq, pos,
+                     (T*)k_out, (T*)v_out, ldk, ldv);
 }
 
 #define DRACO_HD_SWITCH(hd, CALL) \
