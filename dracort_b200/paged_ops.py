@@ -27,7 +27,6 @@ draco/runtime/cpu/speculative.py.
 
 from __future__ import annotations
 
-import ctypes
 import threading
 from typing import Dict, Optional, Tuple
 
@@ -67,77 +66,94 @@ def _cache_type(name: str) -> int:
         raise ValueError(f"unknown cache type {name!r}; expected one of {sorted(CACHE_TYPES)}") from None
 
 
-def _on(t: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype) -> None:
-    if t.device != device or t.dtype != dtype:
-        raise ValueError(f"{name} must be a {dtype} tensor on {device}, not {t.dtype} on {t.device}")
+# The checks run on every call of a decode loop: the fast path touches each
+# tensor's properties once, and the messages are put together only on failure.
+_I32, _F32 = torch.int32, torch.float32
+_current_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
-def _vector(t: torch.Tensor, name: str, device: torch.device, n: int, dtype: torch.dtype = torch.int32) -> int:
-    _on(t, name, device, dtype)
-    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        raise DracoFormatError(f"{name} must be a contiguous tensor of {n} values, not {tuple(t.shape)}")
-    return t.data_ptr()
+def _vector(t: torch.Tensor, name: str, dev: int, n: int, dtype: torch.dtype = _I32) -> int:
+    if t.dtype is dtype and t.get_device() == dev and t.shape == (n,) and t.is_contiguous():
+        return t.data_ptr()
+    if t.dtype is not dtype or t.get_device() != dev:
+        raise ValueError(f"{name} must be a {dtype} tensor on cuda:{dev}, not {t.dtype} on {t.device}")
+    raise DracoFormatError(f"{name} must be a contiguous tensor of {n} values, not {tuple(t.shape)}")
 
 
-def _rows(t: torch.Tensor, name: str, device: torch.device, n: Optional[int], dtype: Optional[torch.dtype],
-          head_dim: int) -> int:
+def _rows(t: torch.Tensor, name: str, dev: int, n: int, dtype: torch.dtype, head_dim: int) -> int:
     """Token stride of [n, heads, head_dim] with contiguous heads."""
-    if t.device != device or t.dtype not in _DTYPES or (dtype is not None and t.dtype != dtype):
-        raise ValueError(f"{name} must be a float32 or bfloat16 tensor on {device} (all activations of a call one "
+    shape, stride = t.shape, t.stride()
+    if (t.dtype is dtype and t.get_device() == dev and len(shape) == 3 and shape[0] == n and shape[2] == head_dim
+            and stride[2] == 1 and (stride[1] == head_dim or shape[1] == 1)):
+        return stride[0] if n > 1 else shape[1] * head_dim
+    if t.dtype is not dtype or t.get_device() != dev:
+        raise ValueError(f"{name} must be a float32 or bfloat16 tensor on cuda:{dev} (all activations of a call one "
                          f"type), not {t.dtype} on {t.device}")
-    if t.dim() != 3 or (n is not None and t.shape[0] != n) or t.shape[2] != head_dim:
-        raise DracoFormatError(f"{name} must be [tokens, heads, {head_dim}], not {tuple(t.shape)}")
-    if t.shape[0] == 0:
-        return t.shape[1] * head_dim
-    if (t.stride(2) != 1 and head_dim > 1) or (t.shape[1] > 1 and t.stride(1) != head_dim):
-        raise ValueError(f"{name} must have contiguous heads (a token stride is free)")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * head_dim)
+    if len(shape) != 3 or shape[0] != n or shape[2] != head_dim:
+        raise DracoFormatError(f"{name} must be [{n}, heads, {head_dim}], not {tuple(shape)}")
+    if n == 0 or shape[1] == 0:
+        return shape[1] * head_dim
+    raise ValueError(f"{name} must have contiguous heads (a token stride is free)")
 
 
 def _cache_struct(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                   head_dim: int) -> N.KvCache:
-    if not k_cache.is_cuda:
+    shape, dtype, dev = k_cache.shape, k_cache.dtype, k_cache.get_device()
+    if dev < 0:
         raise ValueError("k_cache must be a CUDA tensor (this library has no CPU path)")
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
-        raise DracoFormatError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} must be alike, "
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype is not dtype:
+        raise DracoFormatError(f"k_cache {tuple(shape)} and v_cache {tuple(v_cache.shape)} must be alike, "
                                f"[pages, kv_heads, page_size, row]")
-    if v_cache.device != k_cache.device or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+    if v_cache.get_device() != dev or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("k_cache and v_cache must be contiguous tensors on one device")
-    pages, kv_heads, page, row = k_cache.shape
-    if k_cache.dtype == torch.bfloat16:
+    pages, kv_heads, page, row = shape
+    if dtype is torch.bfloat16:
         kind, want = N.KV_BF16, head_dim
-    elif k_cache.dtype == torch.uint8:
+    elif dtype is torch.uint8:
         kind, want = N.KV_Q8_0, head_dim // 32 * 34
     else:
-        raise ValueError(f"a cache is bfloat16 or uint8 (Q8_0 blocks), not {k_cache.dtype}")
+        raise ValueError(f"a cache is bfloat16 or uint8 (Q8_0 blocks), not {dtype}")
     if row != want:
         raise DracoFormatError(f"cache rows of {row} do not hold head_dim {head_dim}")
-    _on(block_table, "block_table", k_cache.device, torch.int32)
-    if block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    if block_table.dtype is not _I32 or block_table.get_device() != dev:
+        raise ValueError(f"block_table must be an int32 tensor on cuda:{dev}, not {block_table.dtype} on "
+                         f"{block_table.device}")
+    tshape = block_table.shape
+    tstride = block_table.stride()
+    if len(tshape) != 2 or (tshape[1] > 1 and tstride[1] != 1):
         raise DracoFormatError("block_table must be [sequences, pages] with contiguous rows")
-    c = N.KvCache()
-    c.type, c.kv_heads, c.head_dim, c.page_size, c.n_pages = kind, kv_heads, head_dim, page, pages
-    c.n_seqs, c.max_pages = block_table.shape
-    c.table_stride = block_table.stride(0)  # 0: all sequences share one row
-    c.k, c.v, c.block_table = k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr()
-    return c
+    # (a table stride of 0: all sequences share one row)
+    return N.KvCache(kind, kv_heads, head_dim, page, pages, tshape[0], tshape[1], tstride[0],
+                     k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr())
 
 
-class _Device:
-    """The tensors' device made current for a call (the library launches on the current one)."""
+def _dtype(t: torch.Tensor, name: str) -> int:
+    dt = _DTYPES.get(t.dtype)
+    if dt is None:
+        raise ValueError(f"{name} must be float32 or bfloat16, not {t.dtype}")
+    return dt
 
-    def __init__(self, device: torch.device) -> None:
-        self.index = device.index
-        self.back = torch.cuda.current_device()
 
-    def __enter__(self) -> int:
-        if self.back != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
+def _table(t: torch.Tensor, name: str, dev: int, positions: int, half: int) -> int:
+    if t.dtype is _F32 and t.get_device() == dev and t.shape == (positions, half) and t.is_contiguous():
+        return t.data_ptr()
+    if t.dtype is not _F32 or t.get_device() != dev:
+        raise ValueError(f"{name} must be a float32 tensor on cuda:{dev}, not {t.dtype} on {t.device}")
+    raise DracoFormatError(f"{name} must be a contiguous [positions, {half}] table, not {tuple(t.shape)}")
 
-    def __exit__(self, *exc) -> None:
-        if self.back != self.index:
-            torch.cuda.set_device(self.back)
+
+def _like(t: torch.Tensor, shape) -> torch.Tensor:
+    """A new contiguous tensor of t's type and device."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(shape)
+
+
+def _call(dev: int, fn, *args) -> int:
+    """fn(*args, stream) on device `dev` and its current stream."""
+    if _current_device() == dev:
+        return fn(*args, _current_stream(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, _current_stream(dev))
 
 
 def kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
@@ -153,37 +169,41 @@ def kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_cac
     bfloat16, any token stride that keeps rows on 16 bytes (slices of a fused
     projection); seq, pos int32 [n].  Tokens of a call go to distinct
     positions.  A token outside the block table or the tables writes nothing."""
-    if k.dim() != 3:
-        raise DracoFormatError(f"k must be [tokens, kv_heads, head_dim], not {tuple(k.shape)}")
-    n, kv_heads, hd = k.shape
+    shape = k.shape
+    if len(shape) != 3:
+        raise DracoFormatError(f"k must be [tokens, kv_heads, head_dim], not {tuple(shape)}")
+    n, kv_heads, hd = shape
     c = _cache_struct(k_cache, v_cache, block_table, hd)
-    dev = k_cache.device
-    if kv_heads != c.kv_heads or v.shape != k.shape:
+    dev, dtype, dt = k_cache.get_device(), k.dtype, _dtype(k, "k")
+    ldk, ldv = _rows(k, "k", dev, n, dtype, hd), _rows(v, "v", dev, n, dtype, hd)
+    if kv_heads != c.kv_heads or v.shape != shape:
         raise DracoFormatError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match the cache's {c.kv_heads} heads")
-    a = N.KvAppendArgs()
-    a.ldk, a.ldv = _rows(k, "k", dev, n, None, hd), _rows(v, "v", dev, n, k.dtype, hd)
-    a.k, a.v, a.n = k.data_ptr(), v.data_ptr(), n
+    ldq = ldqo = heads = 0
+    q_ptr = qo_ptr = None
     if q is not None:
-        a.ldq = _rows(q, "q", dev, n, k.dtype, hd)
+        ldq = _rows(q, "q", dev, n, dtype, hd)
+        heads = q.shape[1]
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            q_out, ldqo = _like(q, (n, heads, hd)), heads * hd
         elif q_out.shape != q.shape:
             raise DracoFormatError(f"q_out {tuple(q_out.shape)} is not shaped like q {tuple(q.shape)}")
-        a.ldqo = _rows(q_out, "q_out", dev, n, k.dtype, hd)
-        a.q, a.q_out, a.heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+        else:
+            ldqo = _rows(q_out, "q_out", dev, n, dtype, hd)
+        q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out needs q")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
+    cos_ptr = sin_ptr = None
+    positions = 0
     if cos is not None:
-        for t, name in ((cos, "cos"), (sin, "sin")):
-            _on(t, name, dev, torch.float32)
-            if t.dim() != 2 or t.shape != cos.shape or t.shape[1] != hd // 2 or not t.is_contiguous():
-                raise DracoFormatError(f"{name} must be a contiguous [positions, {hd // 2}] table")
-        a.cos_table, a.sin_table, a.max_positions = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-    a.seq, a.pos = _vector(seq, "seq", dev, n), _vector(pos, "pos", dev, n)
-    with _Device(dev) as stream:
-        N.check(N.load().draco_kv_append(ctypes.byref(c), ctypes.byref(a), _DTYPES[k.dtype], stream), "kv_append")
+        positions = cos.shape[0] if cos.dim() else 0
+        cos_ptr, sin_ptr = _table(cos, "cos", dev, positions, hd // 2), _table(sin, "sin", dev, positions, hd // 2)
+    a = N.KvAppendArgs(q_ptr, k.data_ptr(), v.data_ptr(), qo_ptr, ldq, ldk, ldv, ldqo, cos_ptr, sin_ptr, positions,
+                       _vector(seq, "seq", dev, n), _vector(pos, "pos", dev, n), n, heads)
+    rc = _call(dev, N.load().draco_kv_append, c, a, dt)
+    if rc:
+        N.check(rc, "kv_append")
     return q_out
 
 
@@ -193,38 +213,30 @@ def kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Ten
     [n, kv_heads, head_dim] float32 (exact) or bfloat16 (rounded once); rows
     outside the cache are zeros."""
     c = _cache_struct(k_cache, v_cache, block_table, head_dim)
-    dev, n = k_cache.device, seq.shape[0]
+    dev, n, kv_heads = k_cache.get_device(), seq.shape[0] if seq.dim() else 0, c.kv_heads
     if dtype not in _DTYPES:
         raise ValueError(f"kv_read gives float32 or bfloat16, not {dtype}")
     s, p = _vector(seq, "seq", dev, n), _vector(pos, "pos", dev, n)
-    out = torch.empty((2, n, c.kv_heads, head_dim), dtype=dtype, device=dev)
-    ld = c.kv_heads * head_dim
-    with _Device(dev) as stream:
-        N.check(N.load().draco_kv_read(ctypes.byref(c), s, p, n, out.data_ptr(),
-                                       out.data_ptr() + n * ld * out.element_size(), ld, ld, _DTYPES[dtype], stream),
-                "kv_read")
-    return out[0], out[1]
+    k = k_cache.new_empty((n, kv_heads, head_dim), dtype=dtype)
+    v = torch.empty_like(k)
+    ld = kv_heads * head_dim
+    rc = _call(dev, N.load().draco_kv_read, c, s, p, n, k.data_ptr(), v.data_ptr(), ld, ld, _DTYPES[dtype])
+    if rc:
+        N.check(rc, "kv_read")
+    return k, v
 
 
-# Workspace of attention_paged per (device, stream), zeroed once; the kernels
-# leave its counters at zero.  A call that is being captured gets one of its
-# own, zeroed in the graph: two graphs may replay at the same time.
+# Workspace of attention_paged per (device, stream), its head zeroed once; the
+# kernels leave its counters at zero.  A call that is being captured gets one of
+# its own, zeroed in the graph: two graphs may replay at the same time.
 _ws_lock = threading.Lock()
 _workspaces: Dict[Tuple[int, int], torch.Tensor] = {}
 
 
-def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-    if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        ws[:N.PAGED_WORKSPACE_HEAD].zero_()  # counters and status; the rest is written before it is read
-        return ws
-    key = (device.index, stream)
-    with _ws_lock:
-        ws = _workspaces.get(key)
-        if ws is None or ws.numel() < nbytes:
-            ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-            _workspaces[key] = ws
-        return ws
+def _new_workspace(like: torch.Tensor, nbytes: int) -> torch.Tensor:
+    ws = like.new_empty(nbytes, dtype=torch.uint8)
+    ws[:N.PAGED_WORKSPACE_HEAD].zero_()  # counters and status; the rest is written before it is read
+    return ws
 
 
 def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -242,39 +254,56 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     max_q, max_kv are upper bounds of a sequence's tokens and positions (default:
     all tokens; the whole block table); they choose the kernels and size the
-    launch, so tight bounds are faster (tokens past max_q may be left out).  scale defaults to 1 / sqrt(head_dim).
-    workspace: a zeroed uint8 tensor of attention_paged_workspace_nbytes that
-    the caller keeps (one per call that may overlap another); by default one
+    launch, so tight bounds are faster (tokens past max_q may be left out).
+    scale defaults to 1 / sqrt(head_dim).
+    workspace: a uint8 tensor of attention_paged_workspace_nbytes, zeroed once,
+    that the caller keeps (one per call that may overlap another); by default one
     per stream is kept here, and a captured call gets its own."""
-    if q.dim() != 3:
-        raise DracoFormatError(f"q must be [tokens, heads, head_dim], not {tuple(q.shape)}")
-    n, heads, hd = q.shape
+    shape = q.shape
+    if len(shape) != 3:
+        raise DracoFormatError(f"q must be [tokens, heads, head_dim], not {tuple(shape)}")
+    n, heads, hd = shape
     c = _cache_struct(k_cache, v_cache, block_table, hd)
-    dev = k_cache.device
-    a = N.AttentionPagedArgs()
-    a.ldq = _rows(q, "q", dev, n, None, hd)
+    dev, dtype, dt = k_cache.get_device(), q.dtype, _dtype(q, "q")
+    ldq = _rows(q, "q", dev, n, dtype, hd)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape:
-        raise DracoFormatError(f"out {tuple(out.shape)} is not shaped like q {tuple(q.shape)}")
-    a.ldo = _rows(out, "out", dev, n, q.dtype, hd)
-    a.q, a.out, a.n, a.heads = q.data_ptr(), out.data_ptr(), n, heads
-    a.q_start, a.kv_len = _vector(q_start, "q_start", dev, c.n_seqs + 1), _vector(kv_len, "kv_len", dev, c.n_seqs)
-    a.max_q = n if max_q is None else int(max_q)
-    a.max_kv = c.max_pages * c.page_size if max_kv is None else int(max_kv)
+        out, ldo = _like(q, shape), heads * hd
+    elif out.shape != shape:
+        raise DracoFormatError(f"out {tuple(out.shape)} is not shaped like q {tuple(shape)}")
+    else:
+        ldo = _rows(out, "out", dev, n, dtype, hd)
     if scale is not None and not 0.0 < scale < 1e30:
         raise ValueError(f"scale {scale} must be positive")
-    a.scale = 0.0 if scale is None else float(scale)
-    dt = _DTYPES[q.dtype]
-    with _Device(dev) as stream:
-        lib = N.load()
-        if workspace is None:
-            need = lib.draco_attention_paged_workspace_bytes(ctypes.byref(c), n, heads, a.max_q, a.max_kv, dt)
-            if need:  # otherwise the call below says what is wrong
-                workspace = _workspace(dev, stream, need)
-        if workspace is not None:
-            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        N.check(lib.draco_attention_paged(ctypes.byref(c), ctypes.byref(a), dt, stream), "attention_paged")
+    max_q = n if max_q is None else int(max_q)
+    max_kv = c.max_pages * c.page_size if max_kv is None else int(max_kv)
+    a = N.AttentionPagedArgs(q.data_ptr(), out.data_ptr(), ldq, ldo, _vector(q_start, "q_start", dev, c.n_seqs + 1),
+                             _vector(kv_len, "kv_len", dev, c.n_seqs), n, heads, max_q, max_kv,
+                             0.0 if scale is None else scale, None, 0)
+    lib = N.load()
+    if workspace is not None:
+        if workspace.get_device() != dev or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous tensor on cuda:{dev}")
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        rc = _call(dev, lib.draco_attention_paged, c, a, dt)
+    elif torch.cuda.is_current_stream_capturing():
+        need = lib.draco_attention_paged_workspace_bytes(c, n, heads, max_q, max_kv, dt)
+        ws = _new_workspace(k_cache, max(need, N.PAGED_WORKSPACE_HEAD))
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        rc = _call(dev, lib.draco_attention_paged, c, a, dt)
+    else:
+        key = (dev, _current_stream(dev))
+        ws = _workspaces.get(key)
+        if ws is not None:
+            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.size(0)
+        rc = _call(dev, lib.draco_attention_paged, c, a, dt)
+        if rc == N.DRACO_ERR_WORKSPACE:  # none yet, or too small
+            need = lib.draco_attention_paged_workspace_bytes(c, n, heads, max_q, max_kv, dt)
+            with _ws_lock, torch.cuda.device(dev):
+                ws = _workspaces[key] = _new_workspace(k_cache, max(need, 1 << 20))
+            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.size(0)
+            rc = _call(dev, lib.draco_attention_paged, c, a, dt)
+    if rc:
+        N.check(rc, "attention_paged")
     return out
 
 
@@ -283,7 +312,7 @@ def attention_paged_workspace_nbytes(k_cache: torch.Tensor, v_cache: torch.Tenso
                                      dtype: torch.dtype) -> int:
     """Bytes of the workspace of an attention_paged call of n tokens."""
     c = _cache_struct(k_cache, v_cache, block_table, head_dim)
-    need = N.load().draco_attention_paged_workspace_bytes(ctypes.byref(c), n, heads, max_q, max_kv, _DTYPES[dtype])
+    need = N.load().draco_attention_paged_workspace_bytes(c, n, heads, max_q, max_kv, _DTYPES[dtype])
     if need == 0:
         raise DracoFormatError(N.last_error() or "attention_paged: unsupported arguments")
     return int(need)
@@ -308,34 +337,35 @@ def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafts: torch.T
     the drafts taken, the next token, then -1); max_rows (default n) is the
     largest number of rows of a sequence.  One row per sequence is plain
     sampling."""
-    if not logits.is_cuda:
+    dev = logits.get_device()
+    if dev < 0:
         raise ValueError("logits must be a CUDA tensor (this library has no CPU path)")
-    dev = logits.device
-    if logits.dtype not in _DTYPES:
-        raise ValueError(f"logits must be float32 or bfloat16, not {logits.dtype}")
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    dt = _dtype(logits, "logits")
+    shape, stride = logits.shape, logits.stride()
+    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
         raise DracoFormatError("logits must be [rows, vocab] with contiguous rows")
-    n, vocab = logits.shape
-    seqs = row_start.shape[0] - 1
-    if row_start.dim() != 1 or seqs < 0:
+    n, vocab = shape
+    seqs = row_start.shape[0] - 1 if row_start.dim() == 1 else -1
+    if seqs < 0:
         raise DracoFormatError("row_start must be [sequences + 1]")
-    v = N.VerifyArgs()
-    v.logits, v.ld_logits, v.dtype = logits.data_ptr(), logits.stride(0), _DTYPES[logits.dtype]
+    probs_ptr, ld_probs = None, 0
     if draft_probs is not None:
-        _on(draft_probs, "draft_probs", dev, torch.float32)
-        if draft_probs.shape != logits.shape or (vocab > 1 and draft_probs.stride(1) != 1):
+        if draft_probs.dtype is not _F32 or draft_probs.get_device() != dev:
+            raise ValueError(f"draft_probs must be a float32 tensor on cuda:{dev}, not {draft_probs.dtype} on "
+                             f"{draft_probs.device}")
+        if draft_probs.shape != shape or (vocab > 1 and draft_probs.stride(1) != 1):
             raise DracoFormatError("draft_probs must be shaped like logits with contiguous rows")
-        v.draft_probs, v.ld_probs = draft_probs.data_ptr(), draft_probs.stride(0)
-    v.row_start, v.drafts = _vector(row_start, "row_start", dev, seqs + 1), _vector(drafts, "drafts", dev, n)
-    v.accept_u = _vector(accept_u, "accept_u", dev, n, torch.float32)
-    v.sample_u = _vector(sample_u, "sample_u", dev, seqs, torch.float32)
+        probs_ptr, ld_probs = draft_probs.data_ptr(), draft_probs.stride(0)
     rows = max(n, 1) if max_rows is None else int(max_rows)
     if rows < 1:
         raise ValueError(f"max_rows {rows} must be at least 1")
-    accepted = torch.empty(seqs, dtype=torch.int32, device=dev)
-    tokens = torch.empty((seqs, rows), dtype=torch.int32, device=dev)
-    v.accepted, v.tokens, v.ld_tokens = accepted.data_ptr(), tokens.data_ptr(), rows
-    v.temperature, v.n, v.n_seqs, v.vocab, v.max_rows = float(temperature), n, seqs, vocab, rows
-    with _Device(dev) as stream:
-        N.check(N.load().draco_verify_drafts(ctypes.byref(v), stream), "verify_drafts")
+    accepted = row_start.new_empty(seqs)
+    tokens = row_start.new_empty((seqs, rows))
+    v = N.VerifyArgs(logits.data_ptr(), probs_ptr, _vector(row_start, "row_start", dev, seqs + 1),
+                     _vector(drafts, "drafts", dev, n), _vector(accept_u, "accept_u", dev, n, _F32),
+                     _vector(sample_u, "sample_u", dev, seqs, _F32), accepted.data_ptr(), tokens.data_ptr(),
+                     stride[0], ld_probs, rows, temperature, dt, n, seqs, vocab, rows)
+    rc = _call(dev, N.load().draco_verify_drafts, v)
+    if rc:
+        N.check(rc, "verify_drafts")
     return accepted, tokens
