@@ -54,7 +54,8 @@ namespace draco {
 
 constexpr int kPaThreads = 128;
 constexpr float kPaLazy = 8.f;
-constexpr int kPaMinSplit = 256;  // keys of a split at least: 4 blocks of each warp
+constexpr int kPaMinSplit = 128;  // keys of a split at least: 2 blocks of each warp
+constexpr int kPaMaxSplits = 64;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;  // 0: the 16 bytes are filled with zeros and src is not read
@@ -153,10 +154,11 @@ struct PaCfg {
   static constexpr int kInit = Q8 && !F32 ? (HD / 32) * kRows * 4 : 0;  // -128 sum(q) of every block
   static constexpr int kHead = kQBytes + kInit;
   static constexpr int kMerge = kWarps * kRows * HD * 4;    // partial O of the warps
-  // three CTAs per SM for Q8_0, whose warps compute, two for bf16, whose
+  // four CTAs per SM for Q8_0, whose warps compute, two for bf16, whose
   // stages are larger, where that leaves two stages
+  static constexpr int kCtas = Q8 ? 4 : 2;
   static constexpr int stages() {
-    int s = ((Q8 ? 74 : 110) * 1024 - kHead) / (kStage * kWarps);
+    int s = ((Q8 ? 56 : 110) * 1024 - kHead) / (kStage * kWarps);
     return s < 2 ? 2 : s > 6 ? 6 : s;
   }
   static constexpr int kStages = stages();
@@ -164,6 +166,8 @@ struct PaCfg {
   static constexpr int smem() { return kHead + (kRing > kMerge ? kRing : kMerge); }
   static_assert(kRowBytes % 16 == 0 && kStride % 16 == 0 && (16 * kScale) % 16 == 0, "16-byte copies");
   static_assert(smem() <= 220 * 1024, "shared memory");
+  static_assert(kRing + kMerge > 0 && (kRing > kMerge ? kRing : kMerge) >= (kRows * kPaMaxSplits + 8 * kPaThreads) * 4,
+                "the merge's weights and sums");
 };
 
 // the key (0..7) behind row n of an 8-key MMA half: for Q8_0 an order in which
@@ -679,25 +683,60 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
   }
   __syncthreads();
   if (!last_flag) return;
+  // Merge in split order.  A warp per row turns the splits' (m, l) into weights
+  // (lanes over splits); then the threads go over the rows' values, and, where
+  // those leave threads idle, over parts of the splits.
   const float* recs = a.recs + unit * a.n_splits * kRec;
-  for (int idx = tid; idx < rows * (HD / 8); idx += kPaThreads) {
-    const int r = idx / (HD / 8), d = 8 * (idx % (HD / 8));
-    float M = -INFINITY;
-    for (int sp = 0; sp < active; ++sp) M = fmaxf(M, __ldcg(recs + (int64_t)sp * kRec + 2 * r));
-    float L = 0.f, o[8] = {};
-#pragma unroll 4
-    for (int sp = 0; sp < active; ++sp) {
-      const float* rc = recs + (int64_t)sp * kRec;
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(rc + 2 * r));
-      const float4 p0 = __ldcg(reinterpret_cast<const float4*>(rc + 2 * C::kRows + r * HD + d));
-      const float4 p1 = __ldcg(reinterpret_cast<const float4*>(rc + 2 * C::kRows + r * HD + d + 4));
-      if (ml.x == -INFINITY && ml.y == ml.y) continue;
+  float* wts = reinterpret_cast<float*>(smem + C::kHead);  // [row][split]
+  for (int r = warp; r < rows; r += W) {
+    float M = -INFINITY, L = 0.f;
+    for (int sp = lane; sp < active; sp += 32) M = fmaxf(M, __ldcg(recs + (int64_t)sp * kRec + 2 * r));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    for (int sp = lane; sp < active; sp += 32) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(recs + (int64_t)sp * kRec + 2 * r));
+      // (m -infinity: no key seen, unless l is NaN)
       const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
-      L = fmaf(f, ml.y, L);
+      L += ml.x == -INFINITY && ml.y == ml.y ? 0.f : f * ml.y;
+      wts[r * a.n_splits + sp] = f;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if (lane == 0) gl[0][r] = L;
+  }
+  __syncthreads();
+  const int items = rows * (HD / 8), parts = max(1, min(kPaThreads / items, 8));
+  float* sums = wts + ((rows * a.n_splits + 3) & ~3);  // [part][item][8]
+  for (int idx = tid; idx < items * parts; idx += kPaThreads) {
+    const int part_i = idx / items, it = idx % items, r = it / (HD / 8), d = 8 * (it % (HD / 8));
+    float o[8] = {};
+#pragma unroll 8
+    for (int sp = part_i; sp < active; sp += parts) {
+      const float* rc = recs + (int64_t)sp * kRec + 2 * C::kRows + r * HD + d;
+      const float f = wts[r * a.n_splits + sp];
+      const float4 p0 = __ldcg(reinterpret_cast<const float4*>(rc)), p1 = __ldcg(reinterpret_cast<const float4*>(rc + 4));
       o[0] = fmaf(f, p0.x, o[0]), o[1] = fmaf(f, p0.y, o[1]), o[2] = fmaf(f, p0.z, o[2]), o[3] = fmaf(f, p0.w, o[3]);
       o[4] = fmaf(f, p1.x, o[4]), o[5] = fmaf(f, p1.y, o[5]), o[6] = fmaf(f, p1.z, o[6]), o[7] = fmaf(f, p1.w, o[7]);
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
+    if (parts == 1) {
+      const float L = gl[0][r], inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = L == 0.f ? 0.f : o[e] * inv;
+      store8(out_row(r) + d, o);
+    } else {
+      *reinterpret_cast<float4*>(sums + 8 * idx) = make_float4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<float4*>(sums + 8 * idx + 4) = make_float4(o[4], o[5], o[6], o[7]);
+    }
+  }
+  if (parts == 1) return;
+  __syncthreads();
+  for (int it = tid; it < items; it += kPaThreads) {
+    const int r = it / (HD / 8), d = 8 * (it % (HD / 8));
+    float o[8] = {};
+    for (int p = 0; p < parts; ++p)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] += sums[8 * (p * items + it) + e];
+    const float L = gl[0][r], inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = L == 0.f ? 0.f : o[e] * inv;
     store8(out_row(r) + d, o);
@@ -707,30 +746,37 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-// Column tiles of a warp (NN: 1, 2, 4 or 8): the fewest that hold the rows of
-// the longest chunk, since a sequence's keys are read and converted once per
-// row tile; as far as O's HD * NN / 4 registers go.
+// Column tiles of a warp (NN: 1, 2 or 4): the fewest that hold the rows of the
+// longest chunk, since a sequence's keys are read and converted once per row
+// tile; but O's HD * NN / 4 registers leave room for other warps (drafts over
+// Q8_0 in fp32, 16-28 rows of 128: 88 us with NN 4, 72 us with two tiles of NN 2).
 static int pick_nn(int max_q, int group, int hd) {
   const int64_t rows = (int64_t)max_q * group;
-  const int most = hd <= 64 ? 8 : hd <= 128 ? 4 : 2;
+  const int most = hd <= 64 ? 4 : hd <= 128 ? 2 : 1;
   int nn = 1;
   while (nn < most && rows > 8 * nn) nn *= 2;
   return nn;
 }
-// Splits of the keys: about three CTAs for each of the two that an SM holds, so
-// that sequences of different lengths even out, none shorter than kPaMinSplit.
-static int pick_splits(int64_t units, int max_kv) {
+// Splits of the keys, none shorter than kPaMinSplit.  A few units (one sequence)
+// are all alike: two CTAs an SM, more only add to the merge (16384 Q8_0
+// positions, 8 heads: 22.9 us with 37 splits, 25.6 with 64).  Many have
+// different lengths, which two waves of smaller pieces even out (48 sequences
+// of 900-8000 positions: 165 us with one wave, 127 with two; 32 equal ones over
+// bf16: 89 and 94).  `ctas`: CTAs an SM holds.
+static int pick_splits(int64_t units, int max_kv, int ctas) {
   if (units > kPagedCounters || units < 1) return 1;
-  const int64_t want = 6LL * device_sm_count();
-  int64_t s = std::min((want + units - 1) / units, ((int64_t)max_kv + kPaMinSplit - 1) / kPaMinSplit);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(s, 128));
+  const int64_t slots = (int64_t)ctas * device_sm_count();
+  const int64_t want = units * 8 <= slots ? 2LL * device_sm_count() : 2 * slots;
+  const int64_t s = std::min(want / units, ((int64_t)max_kv + kPaMinSplit - 1) / kPaMinSplit);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(s, kPaMaxSplits));
 }
 struct PaPlan {
   int nn, splits, per_seq;
   int64_t tiles, units;
   size_t bytes;  // of partial results
 };
-static PaPlan plan_of(int n, int n_seqs, int group, int kv_heads, int hd, int max_q, int max_kv) {
+static PaPlan plan_of(int n, int n_seqs, int group, int kv_heads, int hd, int max_q, int max_kv,
+                      bool q8) {
   PaPlan p;
   p.nn = pick_nn(max_q, group, hd);
   const int R = 8 * p.nn;
@@ -740,7 +786,7 @@ static PaPlan plan_of(int n, int n_seqs, int group, int kv_heads, int hd, int ma
   p.per_seq = per > 0 && per * n_seqs <= p.tiles ? (int)per : 0;
   if (p.per_seq) p.tiles = per * n_seqs;
   p.units = p.tiles * kv_heads;
-  p.splits = pick_splits(p.units, max_kv);
+  p.splits = pick_splits(p.units, max_kv, q8 ? 4 : 2);
   p.bytes = p.splits > 1 ? (size_t)p.units * p.splits * 8 * p.nn * (hd + 2) * sizeof(float) : 0;
   return p;
 }
@@ -756,7 +802,7 @@ static int tc_from(const PagedView& c, int hd, int dtype, int group, int max_q) 
 
 size_t paged_attn_workspace_bytes(const PagedView& c, int n, int group, int hd, int dtype, int max_q, int max_kv) {
   const int from = tc_from(c, hd, dtype, group, max_q);
-  size_t bytes = plan_of(n, c.n_seqs, group, c.kv_heads, hd, from ? from - 1 : max_q, max_kv).bytes;
+  size_t bytes = plan_of(n, c.n_seqs, group, c.kv_heads, hd, from ? from - 1 : max_q, max_kv, c.type == DRACO_KV_Q8_0).bytes;
   if (from) bytes = std::max(bytes, paged_attn_tc_plan(n, c.n_seqs, group, c.kv_heads, hd, max_kv).bytes);
   return kPagedHead + bytes;
 }
@@ -788,11 +834,10 @@ static cudaError_t launch_t(const PagedAttnArgs& a, const PaPlan& p, cudaStream_
 template <int HD, bool Q8, bool F32>
 static cudaError_t launch_nn(const PagedAttnArgs& a, const PaPlan& p, cudaStream_t st) {
   if (p.nn == 1) return launch_t<HD, Q8, F32, 1>(a, p, st);
-  if (p.nn == 2) return launch_t<HD, Q8, F32, 2>(a, p, st);
   if constexpr (HD <= 64) {
-    if (p.nn == 8) return launch_t<HD, Q8, F32, 8>(a, p, st);
+    if (p.nn == 4) return launch_t<HD, Q8, F32, 4>(a, p, st);
   }
-  if constexpr (HD <= 128) return launch_t<HD, Q8, F32, 4>(a, p, st);
+  if constexpr (HD <= 128) return launch_t<HD, Q8, F32, 2>(a, p, st);
   return cudaErrorInvalidValue;  // pick_nn gives no more
 }
 template <bool Q8, bool F32>
@@ -821,7 +866,7 @@ int paged_attn_launch(PagedAttnArgs a, int hd, int dtype, int max_q, int max_kv,
   const int from = tc_from(a.c, hd, dtype, a.group, max_q);
   a.min_new = 0;
   a.max_new = from ? from : 0x7FFFFFFF;
-  const PaPlan p = plan_of(a.n, a.n_seqs, a.group, a.c.kv_heads, hd, from ? from - 1 : max_q, max_kv);
+  const PaPlan p = plan_of(a.n, a.n_seqs, a.group, a.c.kv_heads, hd, from ? from - 1 : max_q, max_kv, q8);
   a.n_splits = p.splits;
   a.per_seq = p.per_seq;
   const cudaError_t e = q8 ? (f32 ? launch_hd<true, true>(hd, a, p, st) : launch_hd<true, false>(hd, a, p, st))
