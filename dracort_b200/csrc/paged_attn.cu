@@ -56,6 +56,8 @@ constexpr int kPaThreads = 128;
 constexpr float kPaLazy = 8.f;
 constexpr int kPaMinSplit = 128;  // keys of a split at least: 2 blocks of each warp
 constexpr int kPaMaxSplits = 64;
+constexpr int kPaLookSeqs = 256;  // sequences whose lengths every CTA looks at
+constexpr int kPaMostKeys = 0x7FFFFF00;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;  // 0: the 16 bytes are filled with zeros and src is not read
@@ -197,9 +199,16 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
   if (tile.s < 0) return;
   const int kvh = blockIdx.z;
   const int rows = min(C::kRows, tile.rows - tile.row0);
-  // keys that the tile's last row sees, and this CTA's share of them
+  // Keys that the tile's last row sees, and this CTA's share of them.  The share
+  // is as long for all sequences, a part of the longest one's keys: CTAs of one
+  // length pack better than equal numbers of CTAs of every length.
   const int kend = max(0, min(tile.kv, row_limit(a, tile, tile.row0 + rows - 1)));
-  int ck = (kend + a.n_splits - 1) / a.n_splits;
+  int longest = kend;
+  if (a.n_splits > 1 && a.n_seqs <= kPaLookSeqs) {
+    for (int i = lane; i < a.n_seqs; i += 32) longest = max(longest, min(__ldg(a.kv_len + i), (int)kPaMostKeys));
+    longest = __reduce_max_sync(0xffffffffu, longest);
+  }
+  int ck = (longest + a.n_splits - 1) / a.n_splits;
   ck = max(kPaMinSplit, (ck + 63) & ~63);
   const int active = max(1, (kend + ck - 1) / ck);
   const int split = blockIdx.y;
