@@ -57,7 +57,6 @@ constexpr float kPaLazy = 8.f;
 constexpr int kPaMinSplit = 128;  // keys of a split at least: 2 blocks of each warp
 constexpr int kPaMaxSplits = 64;
 constexpr int kPaLookSeqs = 256;  // sequences whose lengths every CTA looks at
-constexpr int kPaMostKeys = 0x7FFFFF00;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;  // 0: the 16 bytes are filled with zeros and src is not read
@@ -205,8 +204,9 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
   const int kend = max(0, min(tile.kv, row_limit(a, tile, tile.row0 + rows - 1)));
   int longest = kend;
   if (a.n_splits > 1 && a.n_seqs <= kPaLookSeqs) {
-    for (int i = lane; i < a.n_seqs; i += 32) longest = max(longest, min(__ldg(a.kv_len + i), (int)kPaMostKeys));
-    longest = __reduce_max_sync(0xffffffffu, longest);
+    for (int i = lane; i < a.n_seqs; i += 32) longest = max(longest, __ldg(a.kv_len + i));
+    const int64_t cap = (int64_t)a.c.max_pages << a.c.page_shift;
+    longest = (int)min((int64_t)__reduce_max_sync(0xffffffffu, longest), cap);
   }
   int ck = (longest + a.n_splits - 1) / a.n_splits;
   ck = max(kPaMinSplit, (ck + 63) & ~63);

@@ -72,7 +72,7 @@ struct TcCfg {
   static constexpr int kThreads = Q8 ? 640 : 384;
   static constexpr int kProducers = 8;                    // Q8_0: converting warps
   // registers of a thread: softmax warpgroups, the MMA / load warpgroup, converting warpgroups
-  static constexpr int kRegsSoftmax = Q8 ? 144 : 208, kRegsOne = Q8 ? 64 : 80, kRegsConvert = 64;
+  static constexpr int kRegsSoftmax = Q8 ? 136 : 208, kRegsOne = Q8 ? 64 : 80, kRegsConvert = 72;
   static constexpr int kRegsBlock = 256 * kRegsSoftmax + 128 * kRegsOne + (kThreads - 384) * kRegsConvert;
 };
 
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
           for (int e = 0; e < 16; ++e) {
             const uint64_t x = fma_2(pair2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), sc2, ref2);
             const float u = tca_exp2(lo_2(x));
-            const float v = decltype(poly)::value && e % kTcPoly == 1 ? exp2_poly(hi_2(x)) : tca_exp2(hi_2(x));
+            const float v = decltype(poly)::value && !Q8 && e % kTcPoly == 1 ? exp2_poly(hi_2(x)) : tca_exp2(hi_2(x));
             l0 += u, l1 += v;
             p[e] = Q8 ? pack_f16(u, v) : pack_bf16(u, v);
           }
@@ -737,25 +737,33 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
       constexpr int kPass = kTcKeys / kKeysPass;   // 4 or 2
       const int pt = tid - 384, piece = pt % kPer, d0 = 16 * piece, key_l = pt / kPer;
       const bool on_d = d0 < hd;
-      uint4 qv[kPass];
-      uint32_t sv[kPass];
-      auto fetch = [&](const uint8_t* base, int j) {
+      // keys and values in registers of their own, loaded a tile ahead, and the
+      // tile's pages before that: a tile's conversion never waits for a chain of
+      // loads
+      uint4 kq[kPass], vq[kPass];
+      uint32_t ksc[kPass], vsc[kPass];
+      int pages[kPass];
+      auto look = [&](int j) {
 #pragma unroll
         for (int i = 0; i < kPass; ++i) {
           const int key = kbeg + j * kTcKeys + i * kKeysPass + key_l;
-          int page = -1;
-          if (on_d && j < nj && key < kfin) page = page_of(a.c, tile.s, key);
+          pages[i] = on_d && j < nj && key < kfin ? page_of(a.c, tile.s, key) : -1;
+        }
+      };
+      auto fetch = [&](const uint8_t* base, int j, uint4 (&qv)[kPass], uint32_t (&sv)[kPass]) {
+#pragma unroll
+        for (int i = 0; i < kPass; ++i) {
           qv[i] = make_uint4(0, 0, 0, 0);
           sv[i] = 0;
-          if (page >= 0) {
-            const int off = key & ((1 << a.c.page_shift) - 1);
-            const uint8_t* blk = base + ((int64_t)page * a.c.kv_heads + kvh) * a.c.block_bytes;
+          if (pages[i] >= 0) {
+            const int off = (kbeg + j * kTcKeys + i * kKeysPass + key_l) & ((1 << a.c.page_shift) - 1);
+            const uint8_t* blk = base + ((int64_t)pages[i] * a.c.kv_heads + kvh) * a.c.block_bytes;
             qv[i] = __ldg(reinterpret_cast<const uint4*>(blk + off * hd + d0));
             sv[i] = __ldg(reinterpret_cast<const uint16_t*>(blk + (hd << a.c.page_shift)) + off * (hd / 32) + (d0 >> 5));
           }
         }
       };
-      auto put = [&](uint8_t* tile_s) {
+      auto put = [&](uint8_t* tile_s, const uint4 (&qv)[kPass], const uint32_t (&sv)[kPass]) {
         const int c0 = (d0 >> 3) & 7, flip = (piece ^ (piece >> 2)) & 1;
 #pragma unroll
         for (int i = 0; i < kPass; ++i) {
@@ -782,12 +790,15 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
         }
       };
       bool ok = true;
-      fetch(a.c.k, 0);
+      look(0);
+      fetch(a.c.k, 0, kq, ksc);
+      fetch(a.c.v, 0, vq, vsc);
+      look(1);
       for (int j = 0; j < nj && ok; ++j) {
         const int st = j & 1;
         if (j >= 2 && !(ok = wait_warp(&bars.k_empty[st], (j >> 1) - 1))) break;
-        put(k_s + st * C::kTile);
-        fetch(a.c.v, j);
+        put(k_s + st * C::kTile, kq, ksc);
+        fetch(a.c.k, j + 1, kq, ksc);
         tca_proxy();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.k_full[st]);
@@ -796,14 +807,15 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
 #pragma unroll
           for (int i = 0; i < kPass; ++i) {
             const int b = (j - jedge) * kTcKeys + i * kKeysPass + key_l;
-            if ((sv[i] & 0x7C00u) == 0x7C00u) {
-              sv[i] = 0;
+            if ((vsc[i] & 0x7C00u) == 0x7C00u) {
+              vsc[i] = 0;
               if (b < kTcBadWords * 32) atomicOr(&s_bad[b >> 5], 1u << (b & 31));
             }
           }
         }
-        put(v_s + st * C::kTile);
-        fetch(a.c.k, j + 1);
+        put(v_s + st * C::kTile, vq, vsc);
+        fetch(a.c.v, j + 1, vq, vsc);
+        look(j + 2);
         tca_proxy();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.v_full[st]);
