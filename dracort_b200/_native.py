@@ -86,6 +86,7 @@ DTYPE_BF16 = 1
 GEMM_MAX_PROBLEMS = 16
 KV_BF16 = 1
 KV_Q8_0 = 8
+PAGED_WORKSPACE_STATUS = 8192  # byte offset of attention_paged's status (int32)
 PAGED_WORKSPACE_HEAD = 8256  # bytes of attention_paged's workspace that must be zero before its first use
 
 

@@ -23,7 +23,13 @@ numpy.  Here the whole step runs on one GPU:
   the o_proj / down GEMVs (DRACO_GEMV_ACCUMULATE);
 * the key/value cache is a per-layer fp32 tensor [slot, kv_heads, capacity,
   head_dim]: a sequence owns one slot from ``new_sequence`` to
-  ``end_sequence``.
+  ``end_sequence``;
+* with ``kv_cache_dtype`` "bf16" or "q8_0" the cache is paged instead (a half
+  or 34/128 of the bytes): sequences take pages of positions from one pool as
+  they grow, and a pass runs ``draco_kv_append`` +
+  ``draco_attention_paged`` per layer, a prompt's chunks and decode steps alike;
+* ``generate_speculative`` drafts tokens by n-gram lookup, runs them in one
+  pass and keeps what ``draco_verify_drafts`` accepts.
 
 Rows go through the GEMV 32 at a time, so prompts are processed in chunks
 of 32 tokens (each chunk attends to everything cached before it).  Results
@@ -43,6 +49,7 @@ import torch
 
 from dracort_b200 import _native as N
 from dracort_b200 import gguf_ops as G
+from dracort_b200 import paged_ops as P
 from dracort_b200.exceptions import DracoFormatError
 from dracort_b200.format.gguf_file import GGUFFile
 from dracort_b200.format.gguf_types import BLOCK_LAYOUTS, GGML_TYPE_Q6_K, Q6K_D_LAST
@@ -181,6 +188,40 @@ def cache_capacity(cfg: LlamaConfig, max_num_seqs: int, max_seq_len: Optional[in
     return cap
 
 
+_KV_TYPES = {"f32": None, "fp32": None, "float32": None, "bf16": "bf16", "bfloat16": "bf16", "q8_0": "q8_0"}
+
+
+def page_pool(cfg: LlamaConfig, cache_type: str, max_num_seqs: int, max_seq_len: Optional[int] = None,
+              kv_budget_bytes: Optional[int] = None, page_size: int = 64) -> Tuple[int, int]:
+    """(pages of a layer, positions of a sequence at most) of a paged cache:
+    pages for max_num_seqs sequences of max_seq_len (default: the context
+    length) positions, at most as many as kv_budget_bytes holds over all
+    layers; a sequence may take all of them."""
+    cap = int(cfg.max_position_embeddings)
+    if max_seq_len is not None:
+        cap = min(int(max_seq_len), cap)
+    page_bytes = 2 * P.kv_cache_nbytes(cache_type, 1, cfg.num_key_value_heads, page_size, cfg.head_dim)
+    pages = int(max_num_seqs) * -(-cap // page_size)
+    if kv_budget_bytes is not None:
+        pages = min(pages, int(kv_budget_bytes) // (cfg.num_hidden_layers * page_bytes))
+    if cap < 1 or pages < 1:
+        raise ValueError(f"the key/value cache holds no page for {max_num_seqs} sequences "
+                         f"(max_seq_len {max_seq_len}, kv_budget_bytes {kv_budget_bytes})")
+    return pages, min(cap, pages * page_size)
+
+
+def ngram_drafts(ids: Sequence[int], count: int, ngram: int = 3) -> List[int]:
+    """Up to `count` tokens that followed the latest earlier occurrence of the
+    last `ngram` tokens of ids (then of ever fewer, down to one); none: []."""
+    ids = list(ids)
+    for m in range(min(ngram, len(ids) - 1), 0, -1):
+        tail = ids[-m:]
+        for i in range(len(ids) - m - 1, -1, -1):
+            if ids[i:i + m] == tail:
+                return ids[i + m:i + m + max(count, 0)]
+    return []
+
+
 class GPUExecutionBackend:
     """``CPUExecutionBackend`` for llama-family GGUF files, on one GPU.
 
@@ -189,8 +230,11 @@ class GPUExecutionBackend:
     source          : path of a .gguf file, an open GGUFFile, or any reader with
                       a ``path`` attribute (the reference's GGUFReader);
     max_num_seqs    : sequences that may hold a key/value cache at once;
-    kv_cache_dtype  : "f32" (the cache is fp32, as the reference's default);
-    kv_budget_bytes : sizes the cache when max_seq_len is not given;
+    kv_cache_dtype  : "f32" (the cache is fp32, as the reference's default), or a
+                      paged cache of "bf16" or "q8_0" (head_dim 32, 64, 96, 128
+                      or 256);
+    kv_budget_bytes : sizes the cache when max_seq_len is not given; a paged
+                      cache's pool is never larger than it;
     memory_utilization: accepted for the reference's signature; the cache is
                       sized by max_seq_len, kv_budget_bytes or the context.
 
@@ -198,7 +242,10 @@ class GPUExecutionBackend:
 
     device      : the CUDA device;
     max_seq_len : cache rows per sequence (default: from kv_budget_bytes, else
-                  the model's context length);
+                  the model's context length); of a paged cache, the longest
+                  sequence (default: the context length);
+    page_size   : positions of a page of a paged cache (a power of two from 16
+                  to 1024);
     q6k_order   : byte order of the file's Q6_K blocks ("d_last" for llama.cpp
                   files, "d_first" for the order the reference decodes).
     """
@@ -206,9 +253,12 @@ class GPUExecutionBackend:
     def __init__(self, source, max_num_seqs: int = 1, kv_cache_dtype: str = "f32",
                  kv_budget_bytes: Optional[int] = None, memory_utilization: Optional[float] = None, *,
                  device: Union[str, torch.device] = "cuda", max_seq_len: Optional[int] = None,
-                 q6k_order: str = Q6K_D_LAST) -> None:
-        if kv_cache_dtype not in ("f32", "fp32", "float32"):
-            raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r}: the GPU decode step keeps an fp32 cache")
+                 page_size: int = 64, q6k_order: str = Q6K_D_LAST) -> None:
+        if kv_cache_dtype not in _KV_TYPES:
+            raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r}: the GPU decode step keeps an fp32 cache (\"f32\"), "
+                             "or pages of \"bf16\" or \"q8_0\"")
+        self.kv_cache_type = _KV_TYPES[kv_cache_dtype]
+        self.page_size = int(page_size)
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise ValueError("GPUExecutionBackend runs on a CUDA device (this library has no CPU path)")
@@ -267,15 +317,27 @@ class GPUExecutionBackend:
             self.layers.append(L)
         self.final_norm = entry("output_norm.weight")
         self.lm_head = None if cfg.tie_word_embeddings else entry("output.weight")
-        cap = cache_capacity(cfg, max_num_seqs, max_seq_len, kv_budget_bytes)
+        if self.kv_cache_type is None:
+            cap = cache_capacity(cfg, max_num_seqs, max_seq_len, kv_budget_bytes)
+        else:
+            pages, cap = page_pool(cfg, self.kv_cache_type, max_num_seqs, max_seq_len, kv_budget_bytes, page_size)
         self.capacity = cap
         cos, sin = rope_tables(cfg.head_dim, cap, cfg.rope_theta)
         self.cos = torch.from_numpy(cos).to(self.device)
         self.sin = torch.from_numpy(sin).to(self.device)
         self.max_num_seqs = int(max_num_seqs)
-        shape = (self.max_num_seqs, cfg.num_key_value_heads, cap, cfg.head_dim)
-        self.k_cache = [torch.zeros(shape, dtype=torch.float32, device=self.device) for _ in self.layers]
-        self.v_cache = [torch.zeros(shape, dtype=torch.float32, device=self.device) for _ in self.layers]
+        if self.kv_cache_type is None:
+            shape = (self.max_num_seqs, cfg.num_key_value_heads, cap, cfg.head_dim)
+            self.k_cache = [torch.zeros(shape, dtype=torch.float32, device=self.device) for _ in self.layers]
+            self.v_cache = [torch.zeros(shape, dtype=torch.float32, device=self.device) for _ in self.layers]
+        else:
+            both = [P.kv_cache(self.kv_cache_type, pages, cfg.num_key_value_heads, page_size, cfg.head_dim,
+                               self.device) for _ in self.layers]
+            self.k_cache, self.v_cache = [k for k, _ in both], [v for _, v in both]
+            self.block_table = torch.full((self.max_num_seqs, -(-cap // page_size)), -1, dtype=torch.int32,
+                                          device=self.device)
+            self._free_pages = list(range(pages))
+            self._pages: Dict[int, List[int]] = {}
         self._free = list(range(self.max_num_seqs))
         self._slot: Dict[int, int] = {}
         self._len: Dict[int, int] = {}
@@ -295,6 +357,8 @@ class GPUExecutionBackend:
         self._next_seq_id += 1
         self._slot[seq_id] = self._free.pop(0)
         self._len[seq_id] = 0
+        if self.kv_cache_type is not None:
+            self._pages[seq_id] = []
         return seq_id
 
     def end_sequence(self, seq_id: int) -> None:
@@ -302,6 +366,8 @@ class GPUExecutionBackend:
         self._len.pop(seq_id, None)
         if slot is not None:
             self._free.append(slot)
+            if self.kv_cache_type is not None:
+                self._free_pages.extend(self._pages.pop(seq_id))
 
     def truncate_sequence(self, seq_id: int, new_length: int) -> None:
         """Forget cached positions from new_length on (the rows are rewritten
@@ -309,6 +375,26 @@ class GPUExecutionBackend:
         if seq_id not in self._slot or not 0 <= new_length <= self._len[seq_id]:
             raise ValueError(f"cannot truncate sequence {seq_id} to {new_length}")
         self._len[seq_id] = new_length
+        if self.kv_cache_type is not None:
+            owned, keep = self._pages[seq_id], -(-new_length // self.page_size)
+            self._free_pages.extend(owned[keep:])
+            del owned[keep:]
+
+    def _reserve(self, lengths: Dict[int, int]) -> None:
+        """Pages for the given sequences up to the given lengths (all or none)."""
+        if self.kv_cache_type is None:
+            return
+        grow = {s: -(-n // self.page_size) - len(self._pages[s]) for s, n in lengths.items()}
+        need = sum(g for g in grow.values() if g > 0)
+        if need > len(self._free_pages):
+            raise RuntimeError(f"the key/value cache has {len(self._free_pages)} free pages of {self.page_size} positions; "
+                               f"this step takes {need} (end or truncate a sequence)")
+        for s, g in grow.items():
+            if g > 0:
+                owned, new = self._pages[s], self._free_pages[:g]
+                del self._free_pages[:g]
+                self.block_table[self._slot[s], len(owned):len(owned) + g] = torch.tensor(new, dtype=torch.int32)
+                owned.extend(new)
 
     # -- compute --------------------------------------------------------------
     def _group(self, weights: Sequence[object], x: torch.Tensor, ys: Sequence[torch.Tensor],
@@ -377,7 +463,19 @@ class GPUExecutionBackend:
              "v": f32(n, kvh * hd), "attn": f32(n, heads * hd), "gate": f32(n, ffn),
              "up": f32(n, ffn), "logits": f32(n, cfg.vocab_size), "normed": f32(n, cfg.hidden_size),
              "copied": torch.cuda.Event()}
-        ws_bytes = self._lib.draco_attention_workspace_bytes(n, heads, hd, self.capacity - 1)
+        if self.kv_cache_type is None:
+            ws_bytes = self._lib.draco_attention_workspace_bytes(n, heads, hd, self.capacity - 1)
+        else:
+            # a sequence's rows in a pass: one each (decode), or all n of one sequence (a prompt's chunk)
+            width = self.block_table.shape[1]
+            b["forms"] = {
+                form: {"table": torch.zeros((seqs, width), dtype=torch.int32, device=dev),
+                       "start": torch.tensor(start, dtype=torch.int32, device=dev),
+                       "kv_len": torch.zeros(seqs, dtype=torch.int32, device=dev), "max_q": max_q}
+                for form, seqs, start, max_q in ((True, n, list(range(n + 1)), 1), (False, 1, [0, n], n))}
+            ws_bytes = max(P.attention_paged_workspace_nbytes(self.k_cache[0], self.v_cache[0], f["table"], n, heads,
+                                                              hd, f["max_q"], bound, torch.float32)
+                           for f in b["forms"].values() for bound in self._bounds())
         b["attn_ws"] = torch.zeros(int(ws_bytes), dtype=torch.uint8, device=dev)
         h = b["hidden"]
         b["layers"] = [
@@ -396,8 +494,20 @@ class GPUExecutionBackend:
     @property
     def launches_per_layer(self) -> int:
         """Library kernels one decode token (a pass of one row) starts per
-        layer: the four GEMV steps plus the attention."""
-        return sum(g.launches for g in self._buffers(1)["layers"][0]) + 1
+        layer: the four GEMV steps plus the attention (over a paged cache
+        the append and the attention)."""
+        return sum(g.launches for g in self._buffers(1)["layers"][0]) + (1 if self.kv_cache_type is None else 2)
+
+    def _bound(self, need: int) -> int:
+        """The attention bound of a pass whose largest position is need - 1."""
+        return min(self.capacity, max(64, 1 << (need - 1).bit_length()))
+
+    def _bounds(self) -> List[int]:
+        """Every value of _bound."""
+        out = [self._bound(1)]
+        while out[-1] < self.capacity:
+            out.append(self._bound(out[-1] + 1))
+        return out
 
     def _run(self, n: int, b: Dict[str, object], max_pos: int, decode: bool) -> None:
         """Enqueue one pass of the n staged rows on the current stream (decode:
@@ -412,9 +522,23 @@ class GPUExecutionBackend:
         stream = G._stream_ptr(self.device)
         q, k, v, attn, ws = b["q"], b["k"], b["v"], b["attn"], b["attn_ws"]
         seq, pos = b["seq"].data_ptr(), b["pos"].data_ptr()
+        if self.kv_cache_type is not None:
+            f = b["forms"][decode]
+            seqs = f["table"].shape[0]
+            torch.index_select(self.block_table, 0, ids[1][:seqs], out=f["table"])
+            torch.add(b["pos"][n - seqs:], 1, out=f["kv_len"])
+            q3, k3, v3, attn3 = (t.view(n, -1, hd) for t in (q, k, v, attn))
         for li, (qkv, o_proj, gate_up, down) in enumerate(b["layers"]):
             qkv()
             kc, vc = self.k_cache[li], self.v_cache[li]
+            if self.kv_cache_type is not None:
+                P.kv_append(q3, k3, v3, kc, vc, self.block_table, b["seq"], b["pos"], self.cos, self.sin, q_out=q3)
+                P.attention_paged(q3, kc, vc, f["table"], f["start"], f["kv_len"], max_q=f["max_q"],
+                                  max_kv=max_pos + 1, out=attn3, workspace=ws)
+                o_proj()
+                gate_up()
+                down()
+                continue
             if decode:
                 N.check(self._lib.draco_attention_decode(
                     q.data_ptr(), k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr(), self.cos.data_ptr(),
@@ -460,8 +584,7 @@ class GPUExecutionBackend:
         st[2, :] = torch.as_tensor(list(positions), dtype=torch.int64)
         b["ids"].copy_(st, non_blocking=True)
         b["copied"].record()
-        need = int(max(positions)) + 1
-        bound = min(self.capacity, max(64, 1 << (need - 1).bit_length()))
+        bound = self._bound(int(max(positions)) + 1)
         decode = len(set(slots)) == n
         key = (n, bound, decode)
         g = self._graphs.get(key)
@@ -500,6 +623,7 @@ class GPUExecutionBackend:
         slot = self._slot[seq_id]
         chunks = []
         with torch.cuda.device(self.device):
+            self._reserve({seq_id: start_position + len(ids)})
             for c0 in range(0, len(ids), _ROWS):
                 part = ids[c0:c0 + _ROWS]
                 pos = [start_position + c0 + j for j in range(len(part))]
@@ -528,6 +652,7 @@ class GPUExecutionBackend:
         self._check_tokens(ids)
         outs = []
         with torch.cuda.device(self.device):
+            self._reserve({s: self._len[s] + 1 for s in seq_ids})
             for c0 in range(0, n, _ROWS):
                 sl = slice(c0, c0 + _ROWS)
                 outs.append(self._forward([self._slot[s] for s in seq_ids[sl]], ids[sl],
@@ -550,3 +675,61 @@ class GPUExecutionBackend:
             return ids
         finally:
             self.end_sequence(seq_id)
+
+    def generate_speculative(self, prompt_ids: Sequence[int], max_new_tokens: int, num_drafts: int = 4,
+                             ngram: int = 3, temperature: float = 0.0, seed: Optional[int] = None) -> List[int]:
+        """Generation by drafting and verifying: `num_drafts` tokens at most are
+        looked up behind an earlier occurrence of the last `ngram` tokens, run
+        together with the newest token as one pass, and the verification keeps
+        those that sampling at `temperature` (0: greedy) would have given,
+        with the token after them.  The result is distributed as without
+        drafts; greedy, it is the tokens of the largest logits.  ``seed`` fixes
+        the draws.  (The reference drafts by n-gram lookup and verifies
+        greedily, draco/runtime/cpu/speculative.py.)"""
+        if not 0 <= num_drafts < _ROWS:
+            raise ValueError(f"num_drafts {num_drafts} must lie in 0..{_ROWS - 1}")
+        if ngram < 1:
+            raise ValueError(f"ngram {ngram} must be at least 1")
+        if not 0.0 <= temperature < 1e30:
+            raise ValueError(f"temperature {temperature} must not be negative")
+        ids = [int(t) for t in prompt_ids]
+        if not ids:
+            raise ValueError("the prompt holds no token")
+        self._check_tokens(ids)
+        end = len(ids) + max_new_tokens
+        if end - 1 > self.capacity:
+            raise ValueError(f"{len(ids)} + {max_new_tokens} tokens exceed the cache capacity of {self.capacity} "
+                             "positions")
+        rng = np.random.default_rng(seed)
+        if max_new_tokens < 1:
+            return ids
+        seq_id = self.new_sequence()
+        try:
+            if len(ids) > 1:
+                self.forward_step(seq_id, np.array(ids[:-1]), 0)
+            while len(ids) < end:
+                # the newest token is not cached yet; a pass gives one token more than it drafts
+                drafts = ngram_drafts(ids, min(num_drafts, end - len(ids) - 1), ngram)
+                taken = self._verified(seq_id, ids[-1:] + drafts, temperature, rng)
+                ids.extend(taken)
+                self.truncate_sequence(seq_id, len(ids) - 1)
+            return ids
+        finally:
+            self.end_sequence(seq_id)
+
+    def _verified(self, seq_id: int, tokens: List[int], temperature: float, rng: np.random.Generator) -> List[int]:
+        """One pass over [newest token, drafts...] of a sequence, and the tokens
+        that its verification gives (the drafts taken and one more)."""
+        n, start = len(tokens), self._len[seq_id]
+        with torch.cuda.device(self.device):
+            self._reserve({seq_id: start + n})
+            logits = self._forward([self._slot[seq_id]] * n, tokens, [start + j for j in range(n)])
+            self._len[seq_id] = start + n
+            # uniform in [0, 1) as fp32: 24 random bits
+            u = torch.from_numpy((rng.integers(0, 1 << 24, n + 1) / float(1 << 24)).astype(np.float32)).to(self.device)
+            rows = torch.tensor([0, n] + tokens[1:] + [-1], dtype=torch.int32).to(self.device)
+            _, out = P.verify_drafts(logits, rows[:2], rows[2:], u[:n], u[n:], temperature=temperature)
+            got = [t for t in out[0].tolist() if t >= 0]
+        if not got:
+            raise RuntimeError("the model's logits are not finite: no token can be drawn")
+        return got

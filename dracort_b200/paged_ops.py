@@ -307,6 +307,29 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     return out
 
 
+def attention_paged_status(workspace: Optional[torch.Tensor] = None) -> int:
+    """Device status of attention_paged: 0, or DRACO_ERR_TIMEOUT after a bounded
+    wait inside a kernel ran out (the outputs of that call are then invalid).
+    Waits for the GPU; reads the given workspace, or all that this module keeps
+    on the current device, and makes a workspace that reports an error ready for
+    use again."""
+    if workspace is None:
+        dev = _current_device()
+        with _ws_lock:
+            kept = [ws for (d, _), ws in _workspaces.items() if d == dev]
+        torch.cuda.synchronize(dev)
+    else:
+        kept = [workspace]
+        torch.cuda.synchronize(workspace.device)
+    for ws in kept:
+        rc = int(ws[N.PAGED_WORKSPACE_STATUS:N.PAGED_WORKSPACE_STATUS + 4].view(torch.int32).item())
+        if rc:
+            ws[:N.PAGED_WORKSPACE_HEAD].zero_()
+            torch.cuda.synchronize(ws.device)
+            return rc
+    return 0
+
+
 def attention_paged_workspace_nbytes(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                                      n: int, heads: int, head_dim: int, max_q: int, max_kv: int,
                                      dtype: torch.dtype) -> int:

@@ -390,6 +390,178 @@ def test_own_workspace():
         P.attention_paged(*b, max_q=1, max_kv=3001, workspace=ws[:need - 16])
 
 
+@pytest.mark.parametrize("heads,kv,hd,page", [(32, 8, 128, 64), (6, 1, 96, 16), (40, 2, 64, 32)])
+@pytest.mark.parametrize("cache", ["bf16", "q8_0"])
+def test_long_and_short_sequences_in_one_batch(heads, kv, hd, page, cache):
+    """Chunks, drafts, single tokens and sequences of none side by side: every
+    sequence is taken by one of the kernels."""
+    new = [200, 1, 0, 3, 64, 33, 17, 129, 1]
+    b = batch(new, [100, 700, 30, 0, 50, 0, 15, 1000, 0], heads, kv, hd, page, cache, BF16, seed=21)
+    out = torch.full_like(b[0], math.nan)
+    P.attention_paged(*b, max_q=200, max_kv=1129, out=out)
+    check(*b, out)
+    check(*b, P.attention_paged(*b))  # loose bounds
+
+
+@pytest.mark.parametrize("cache", ["bf16", "q8_0"])
+def test_long_chunk_of_one_head_is_split_and_merged(cache):
+    b = batch([150], [9000], 4, 1, 128, 64, cache, BF16, seed=22)
+    out = P.attention_paged(*b, max_q=150, max_kv=9150)
+    check(*b, out)
+    for _ in range(3):
+        assert torch.equal(P.attention_paged(*b, max_q=150, max_kv=9150), out)  # merged in a fixed order
+
+
+def test_one_table_row_for_all_sequences():
+    q, kc, vc, table, q_start, _ = batch([3, 3, 3], [40, 40, 40], 4, 2, 64, 16, "q8_0", F32, seed=23)
+    rows, lens = table[1:2].expand(3, -1), i32([43, 43, 43])
+    out = P.attention_paged(q, kc, vc, rows, q_start, lens, max_q=3, max_kv=43)
+    check(q, kc, vc, rows, q_start, lens, out)
+    k, v = P.kv_read(kc, vc, rows, i32([0, 1, 2]), i32([5, 5, 5]), 64)
+    assert torch.equal(k[0], k[1]) and torch.equal(k[0], k[2])
+    assert torch.equal(k[0].double(), R.values(kc)[int(table[1, 0]), :, 5])
+
+
+def test_arguments_that_are_refused():
+    q, kc, vc, table, q_start, kv_len = batch([2], [10], 4, 2, 64, 16, "bf16", F32, seed=24)
+    seq, pos = i32([0, 0]), i32([10, 11])
+    k, v = q[:, :2], q[:, 2:]
+    cos, sin = tables(64, 32)
+    ok = P.kv_append(q, k, v, kc, vc, table, seq, pos, cos, sin)
+    assert ok.shape == q.shape
+    half = torch.float16
+    from dracort_b200.exceptions import DracoFormatError
+    for err, call in [
+            (ValueError, lambda: P.kv_append(q.to(half), k.to(half), v.to(half), kc, vc, table, seq, pos)),
+            (ValueError, lambda: P.kv_append(q, k.bfloat16(), v, kc, vc, table, seq, pos)),
+            (ValueError, lambda: P.kv_append(q, k, v, kc, vc, table, seq.long(), pos)),
+            (ValueError, lambda: P.kv_append(q, k, v, kc, vc, table.long(), seq, pos)),
+            (ValueError, lambda: P.kv_append(q, k, v, kc, vc, table.cpu(), seq, pos)),
+            (ValueError, lambda: P.kv_append(q, k, v, kc, vc, table, seq, pos, cos)),
+            (ValueError, lambda: P.kv_append(None, k, v, kc, vc, table, seq, pos, q_out=q)),
+            (ValueError, lambda: P.kv_append(q.transpose(1, 2).contiguous().transpose(1, 2), k, v, kc, vc, table, seq,
+                                             pos)),
+            (DracoFormatError, lambda: P.kv_append(q, k, v[:1], kc, vc, table, seq, pos)),
+            (DracoFormatError, lambda: P.kv_append(q, k[:, :1], v[:, :1], kc, vc, table, seq, pos)),
+            (DracoFormatError, lambda: P.kv_append(q, k, v, kc, vc, table, seq[:1], pos)),
+            (DracoFormatError, lambda: P.kv_append(q, k, v, kc, vc, table, seq, pos, cos[:, :16], sin[:, :16])),
+            (DracoFormatError, lambda: P.kv_append(q, k, v, kc, vc[:-1], table, seq, pos)),
+            (DracoFormatError, lambda: P.kv_append(q, k, v, kc, vc, table[0], seq, pos)),
+            (DracoFormatError, lambda: P.kv_append(q[..., :32], k[..., :32], v[..., :32], kc, vc, table, seq, pos)),
+            (ValueError, lambda: P.kv_append(q, k, v, kc.half(), vc.half(), table, seq, pos)),
+            (ValueError, lambda: P.kv_read(kc, vc, table, seq, pos, 64, half)),
+            (DracoFormatError, lambda: P.kv_read(kc, vc, table, seq, pos[:1], 64)),
+            (DracoFormatError, lambda: P.kv_read(kc, vc, table, seq, pos, 32)),
+            (ValueError, lambda: P.attention_paged(q.to(half), kc, vc, table, q_start, kv_len)),
+            (DracoFormatError, lambda: P.attention_paged(q[:, :3], kc, vc, table, q_start, kv_len)),
+            (DracoFormatError, lambda: P.attention_paged(q, kc, vc, table, q_start[:1], kv_len)),
+            (DracoFormatError, lambda: P.attention_paged(q, kc, vc, table, q_start, i32([12, 12]))),
+            (ValueError, lambda: P.attention_paged(q, kc, vc, table, q_start, kv_len, scale=0.0)),
+            (ValueError, lambda: P.attention_paged(q, kc, vc, table, q_start, kv_len, scale=math.nan)),
+            (ValueError, lambda: P.attention_paged(q, kc, vc, table, q_start, kv_len, out=q.bfloat16())),
+            (DracoFormatError, lambda: P.attention_paged(q, kc, vc, table, q_start, kv_len, max_q=-1)),
+            (DracoFormatError, lambda: P.attention_paged(q[:1].expand(2, -1, -1), kc, vc, table, q_start, kv_len,
+                                                         out=q[:1].expand(2, -1, -1))),
+            (ValueError, lambda: P.attention_paged(q, kc, vc, table, q_start, kv_len,
+                                                   workspace=torch.zeros(64, dtype=torch.uint8)))]:
+        with pytest.raises(err):
+            call()
+    a = verify_inputs([2, 1], 50, 1)
+    for err, call in [
+            (ValueError, lambda: P.verify_drafts(a[0].to(half), *a[1:5])),
+            (ValueError, lambda: P.verify_drafts(a[0], a[1], a[2].long(), *a[3:5])),
+            (ValueError, lambda: P.verify_drafts(*a[:5], temperature=-1.0)),
+            (ValueError, lambda: P.verify_drafts(*a[:5], max_rows=0)),
+            (ValueError, lambda: P.verify_drafts(*a[:5], draft_probs=a[5].double())),
+            (DracoFormatError, lambda: P.verify_drafts(*a[:5], draft_probs=a[5][:, 1:])),
+            (DracoFormatError, lambda: P.verify_drafts(a[0].t(), *a[1:5])),
+            (DracoFormatError, lambda: P.verify_drafts(*a[:4], a[4][:1])),
+            (DracoFormatError, lambda: P.verify_drafts(a[0], a[1][0], *a[2:5]))]:
+        with pytest.raises(err):
+            call()
+
+
+def test_status_of_the_workspaces():
+    b = batch([1], [300], 8, 2, 128, 64, "bf16", F32, seed=25)
+    P.attention_paged(*b)
+    assert P.attention_paged_status() == 0
+    ws = torch.zeros(P.attention_paged_workspace_nbytes(*b[1:4], 1, 8, 128, 1, 301, F32), dtype=torch.uint8, device=DEV)
+    ws[8192] = 5  # as a kernel records it
+    assert P.attention_paged_status(ws) == 5
+    assert P.attention_paged_status(ws) == 0 and int(ws.sum()) == 0
+    check(*b, P.attention_paged(*b, max_q=1, max_kv=301, workspace=ws))
+
+
+# ---------------------------------------------------------------------------
+# a serving step: append, attend, verify
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cache", ["bf16", "q8_0"])
+def test_a_step_of_prompts_drafts_and_single_tokens(cache, dtype):
+    """The operators as a step runs them, eager and replayed from a graph whose
+    inputs change: each is compared with its statement on what it was given."""
+    heads, kv, hd, page, vocab = 8, 2, 64, 16, 500
+    new, past = [5, 1, 80, 3], [60, 33, 0, 15]
+    g = gen(31)
+    n, seqs = sum(new), len(new)
+    kc, vc = make_cache(cache, 40, kv, page, hd, g)
+    table = torch.randperm(40, generator=g, device=DEV)[:24].reshape(4, 6).to(torch.int32)
+    cos, sin = tables(hd, 128)
+    head = randn(heads * hd, vocab, g=g) * 0.2
+    starts = [0]
+    for a in new:
+        starts.append(starts[-1] + a)
+    q_start = i32(starts)
+    seq = i32([s for s in range(seqs) for _ in range(new[s])])
+    pos, kv_len = i32([0] * n), i32([0] * seqs)
+    qkv = torch.zeros(n, heads + 2 * kv, hd, dtype=dtype, device=DEV)
+    drafts, au, su = i32([0] * n), torch.zeros(n, device=DEV), torch.zeros(seqs, device=DEV)
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv], qkv[:, heads + kv:]
+
+    def step():
+        rq = P.kv_append(q, k, v, kc, vc, table, seq, pos, cos, sin)
+        o = P.attention_paged(rq, kc, vc, table, q_start, kv_len, max_q=80, max_kv=96)
+        logits = torch.matmul(o.reshape(n, -1).float(), head)
+        return rq, o, logits, P.verify_drafts(logits, q_start, drafts, au, su, temperature=0.9, max_rows=80)
+
+    def fill(seed):
+        gg = gen(seed)
+        at = [p + seed % 3 for p in past]
+        qkv.copy_(randn(n, heads + 2 * kv, hd, g=gg, dtype=dtype))
+        pos.copy_(i32([at[s] + j for s in range(seqs) for j in range(new[s])]))
+        kv_len.copy_(i32([at[s] + new[s] for s in range(seqs)]))
+        drafts.copy_(torch.randint(0, 8, (n,), generator=gg, device=DEV).to(torch.int32))
+        au.copy_(torch.rand(n, generator=gg, device=DEV) * 0.02)
+        su.copy_(torch.rand(seqs, generator=gg, device=DEV))
+
+    def verify_step(got):
+        rq, o, logits, (count, tokens) = got
+        # the largest count of accepted drafts and the tokens
+        want_c, want_t, margin = R.verify(logits.cpu(), q_start.cpu(), drafts.cpu(), au.cpu(), su.cpu(), None, 0.9, 80)
+        assert margin > 1e-6
+        assert count.tolist() == want_c and tokens.tolist() == want_t
+        check(rq, kc, vc, table, q_start, kv_len, o)
+        ck, cv = P.kv_read(kc, vc, table, seq, pos, hd)
+        at = pos.long()
+        assert torch.equal(ck.double(), R.cached_values(R.rotate(k, cos[at], sin[at]), cache))
+        assert torch.equal(cv.double(), R.cached_values(v, cache))
+        turned = R.rotate(q, cos[at], sin[at])
+        assert torch.equal(rq.double(), turned.to(dtype).double())
+
+    fill(0)
+    step()  # (the matrix product's own workspace is made outside the capture)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in range(1, 4):
+        fill(seed)
+        graph.replay()
+        verify_step(captured)
+        eager = step()
+        verify_step(eager)
+        assert torch.equal(eager[1], captured[1]) and torch.equal(eager[3][1], captured[3][1])
+
+
 # ---------------------------------------------------------------------------
 # verification of drafts
 # ---------------------------------------------------------------------------
