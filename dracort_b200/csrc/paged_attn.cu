@@ -55,7 +55,9 @@ namespace draco {
 constexpr int kPaThreads = 128;
 constexpr float kPaLazy = 8.f;
 constexpr int kPaMinSplit = 128;  // keys of a split at least: 2 blocks of each warp
-constexpr int kPaMaxSplits = 64;
+constexpr int kPaMaxSplits = 64;  // two a lane of the merging warp
+constexpr int64_t kPaFew = 2;
+constexpr float kPaFixed = 250.f;
 constexpr int kPaLookSeqs = 256;  // sequences whose lengths every CTA looks at
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
@@ -154,7 +156,7 @@ struct PaCfg {
   static constexpr int kQBytes = kTerms * (HD / 32) * NN * 512;
   static constexpr int kInit = Q8 && !F32 ? (HD / 32) * kRows * 4 : 0;  // -128 sum(q) of every block
   static constexpr int kHead = kQBytes + kInit;
-  static constexpr int kMerge = kWarps * kRows * HD * 4;    // partial O of the warps
+  static constexpr int kMerge = kWarps * kRows * (HD + 4) * 4;    // partial O of the warps
   // four CTAs per SM for Q8_0, whose warps compute, two for bf16, whose
   // stages are larger, where that leaves two stages
   static constexpr int kCtas = Q8 ? 4 : 2;
@@ -180,13 +182,54 @@ __device__ __forceinline__ int key_of(int n) {
   return (0x57463120 >> (4 * n)) & 0xF;
 }
 
+// Keys of a split: the same for all tiles of the batch, so that all CTAs but a
+// tile's last run equally long, and so many that the batch makes one or two
+// whole waves of a.want CTAs of a head: with T tiles, whose lengths end
+// anywhere in their last split, total / ck + T / 2 CTAs.  A wave takes as long
+// as a split's keys and the kPaFixed that its beginning and its merge are worth.
+// fresh0, kv0: new tokens and keys of sequence `lane`, loaded beforehand.
+template <int R>
+__device__ __forceinline__ int split_keys(const PagedAttnArgs& a, int kend, int fresh0, int kv0) {
+  int longest = kend;
+  float total = (float)kend, tiles = 1.f;
+  if (a.n_seqs <= kPaLookSeqs) {
+    const int64_t cap = (int64_t)a.c.max_pages << a.c.page_shift;
+    total = tiles = 0.f;
+    int fresh = fresh0, kv = kv0;
+    for (int i = threadIdx.x & 31;;) {
+      if (fresh > 0 && fresh >= a.min_new && fresh < a.max_new) {
+        kv = (int)min((int64_t)max(kv, 0), cap);
+        const float t = (float)((fresh * a.group + R - 1) / R);
+        longest = max(longest, kv);
+        total += t * (float)kv, tiles += t;
+      }
+      i += 32;
+      if (i >= a.n_seqs) break;
+      fresh = seq_begin(a, i + 1) - seq_begin(a, i), kv = __ldg(a.kv_len + i);
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {  // the same sums in every lane of every CTA
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+      tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    }
+  }
+  float aim = fminf(total / fmaxf(a.want - 0.5f * tiles, 0.25f * a.want), (float)longest);
+  if (a.waves > 1) {
+    const float two = total / fmaxf(2.f * a.want - 0.5f * tiles, 0.5f * a.want);
+    if (2.f * (two + kPaFixed) < aim + kPaFixed) aim = two;
+  }
+  const int ck = max((int)aim, (longest + a.n_splits - 1) / a.n_splits);
+  return max(kPaMinSplit, (ck + 63) & ~63);
+}
+
 template <int HD, bool Q8, bool F32, int NN>
 __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
   using C = PaCfg<HD, Q8, F32, NN>;
   using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
   constexpr int NT = C::kTerms, KS = C::kStride, NB = HD / 32, W = C::kWarps;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float row_scale[C::kRows];
+  __shared__ float row_scale[C::kRows], row_max[NB][C::kRows];
   __shared__ float gm[W][C::kRows], gl[W][C::kRows];
   __shared__ int last_flag;
   grid_dependency_wait();
@@ -194,24 +237,20 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   // the last tiles of a prompt see the most keys: they start first
   const int tile_id = gridDim.x - 1 - blockIdx.x;
+  int fresh0 = 0, kv0 = 0;
+  if (lane < a.n_seqs && a.n_splits > 1) {
+    fresh0 = seq_begin(a, lane + 1) - seq_begin(a, lane);
+    kv0 = __ldg(a.kv_len + lane);
+  }
   const RowTile tile = find_tile(a, tile_id, C::kRows);
   if (tile.s < 0) return;
-  const int kvh = blockIdx.z;
+  const int kvh = blockIdx.y;
   const int rows = min(C::kRows, tile.rows - tile.row0);
-  // Keys that the tile's last row sees, and this CTA's share of them.  The share
-  // is as long for all sequences, a part of the longest one's keys: CTAs of one
-  // length pack better than equal numbers of CTAs of every length.
+  // Keys that the tile's last row sees, and this CTA's share of them.
   const int kend = max(0, min(tile.kv, row_limit(a, tile, tile.row0 + rows - 1)));
-  int longest = kend;
-  if (a.n_splits > 1 && a.n_seqs <= kPaLookSeqs) {
-    for (int i = lane; i < a.n_seqs; i += 32) longest = max(longest, __ldg(a.kv_len + i));
-    const int64_t cap = (int64_t)a.c.max_pages << a.c.page_shift;
-    longest = (int)min((int64_t)__reduce_max_sync(0xffffffffu, longest), cap);
-  }
-  int ck = (longest + a.n_splits - 1) / a.n_splits;
-  ck = max(kPaMinSplit, (ck + 63) & ~63);
+  const int ck = a.n_splits > 1 ? split_keys<C::kRows>(a, kend, fresh0, kv0) : max(kend, 1);
   const int active = max(1, (kend + ck - 1) / ck);
-  const int split = blockIdx.y;
+  const int split = blockIdx.z;  // slowest: CTAs without keys start last
   if (split >= active) return;
   const int kbeg = split * ck, kfin = min(kend, kbeg + ck);
 
@@ -249,6 +288,42 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
       }
     }
   };
+  // --- q: read ahead of the keys; a thread holds 8 dims of a row and 32-dim block, kQItems times
+  constexpr int kQItems = (NB * NN * 32 + kPaThreads - 1) / kPaThreads;
+  const T* qbase = static_cast<const T*>(a.q);
+  constexpr int QW = F32 ? 8 : 4;  // words of 8 dims
+  uint32_t raw[kQItems][QW];
+#pragma unroll
+  for (int i = 0; i < kQItems; ++i) {
+    const int idx = tid + i * kPaThreads, lg = (idx & 31) >> 2, lt = idx & 3;
+    const int nt = (idx >> 5) % NN, blk = (idx >> 5) / NN, r = 8 * nt + lg;
+#pragma unroll
+    for (int e = 0; e < QW; ++e) raw[i][e] = 0u;
+    if (blk < NB && r < rows) {
+      const int rr = tile.row0 + r;
+      const T* p = qbase + (int64_t)(tile.start + rr / a.group) * a.ldq +
+                   (int64_t)(kvh * a.group + rr % a.group) * HD + 32 * blk;
+      if constexpr (Q8) {
+#pragma unroll
+        for (int e = 0; e < QW; e += 4) {
+          const uint4 u = *reinterpret_cast<const uint4*>(p + 8 * lt + e);
+          raw[i][e] = u.x, raw[i][e + 1] = u.y, raw[i][e + 2] = u.z, raw[i][e + 3] = u.w;
+        }
+      } else {
+        // the dims behind (2t, 2t+1) and (2t+8, 2t+9) of the block's two steps
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const T* u = p + 16 * (e >> 1) + 8 * (e & 1) + 2 * lt;
+          if constexpr (F32) {
+            const uint2 w = *reinterpret_cast<const uint2*>(u);
+            raw[i][2 * e] = w.x, raw[i][2 * e + 1] = w.y;
+          } else {
+            raw[i][e] = *reinterpret_cast<const uint32_t*>(u);
+          }
+        }
+      }
+    }
+  }
   int page_next = block_page(0);
 #pragma unroll
   for (int b = 0; b < C::kStages - 1; ++b) {
@@ -259,65 +334,52 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
   }
 
   // --- q as B fragments in shared memory: [term][32 dims][column tile][lane] of two MMA steps
-  const T* qbase = static_cast<const T*>(a.q);
-  auto q_row = [&](int r) -> const T* {  // row r of the tile
-    const int rr = tile.row0 + r;
-    return qbase + (int64_t)(tile.start + rr / a.group) * a.ldq + (int64_t)(kvh * a.group + rr % a.group) * HD;
-  };
-  if constexpr (Q8) {  // the row's power-of-two scale
-    constexpr int TPR = kPaThreads / C::kRows < 16 ? kPaThreads / C::kRows : 16;  // threads of a row
-    float m = 0.f;
-    const int r = tid / TPR;
-    if (r < rows) {
-      const T* p = q_row(r);
-      for (int j = tid % TPR; j < HD / 8; j += TPR) {
-        float x[8];
-        load8(p + 8 * j, x);
+  float* init = reinterpret_cast<float*>(smem + C::kQBytes);  // [32 dims][row]
+  float x[kQItems][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
-      }
+  for (int i = 0; i < kQItems; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (F32)
+        x[i][2 * e] = __uint_as_float(raw[i][2 * e]), x[i][2 * e + 1] = __uint_as_float(raw[i][2 * e + 1]);
+      else
+        x[i][2 * e] = bf16lo(raw[i][e]), x[i][2 * e + 1] = bf16hi(raw[i][e]);
     }
+  if constexpr (Q8) {  // the rows' largest values
 #pragma unroll
-    for (int o = TPR / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    // 2^(exponent + 1) > m; rows of zeros, infinities and NaN keep scale 1
-    float s = 1.f;
-    if (m > 1e-30f && m < 1e38f) s = __int_as_float((__float_as_int(m) & 0x7F800000) + 0x00800000);
-    if (tid % TPR == 0 && r < C::kRows) row_scale[r] = s;
+    for (int i = 0; i < kQItems; ++i) {
+      const int idx = tid + i * kPaThreads, nt = (idx >> 5) % NN, blk = (idx >> 5) / NN;
+      float big = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[i][e]));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      if (t == 0 && blk < NB) row_max[blk][8 * nt + g] = big;
+    }
     __syncthreads();
   }
-  float* init = reinterpret_cast<float*>(smem + C::kQBytes);  // [32 dims][row]
-  for (int idx = tid; idx < NB * NN * 32; idx += kPaThreads) {
-    const int ln = idx & 31, nt = (idx >> 5) % NN, blk = (idx >> 5) / NN;
-    const int lg = ln >> 2, lt = ln & 3, r = 8 * nt + lg;
-    // the dims behind (2t, 2t+1) and (2t+8, 2t+9) of the block's two steps
-    float x[8] = {};
-    if (r < rows) {
-      const T* p = q_row(r) + 32 * blk;
-      if constexpr (Q8) {
-        load8(p + 8 * lt, x);
-        const float inv = 1.f / row_scale[r];  // a power of two: exact
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= inv;
-      } else {
+  for (int i = 0; i < kQItems; ++i) {
+    const int idx = tid + i * kPaThreads, nt = (idx >> 5) % NN, blk = (idx >> 5) / NN, r = 8 * nt + g;
+    if (blk >= NB) break;
+    if constexpr (Q8) {  // the row's power-of-two scale
+      float big = row_max[0][r];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int d = 16 * (e >> 1) + 8 * (e & 1) + 2 * lt;
-          if constexpr (F32) {
-            const float2 u = *reinterpret_cast<const float2*>(p + d);
-            x[2 * e] = u.x, x[2 * e + 1] = u.y;
-          } else {
-            const uint32_t u = *reinterpret_cast<const uint32_t*>(p + d);
-            x[2 * e] = bf16lo(u), x[2 * e + 1] = bf16hi(u);
-          }
-        }
-      }
+      for (int e = 1; e < NB; ++e) big = fmaxf(big, row_max[e][r]);
+      // 2^(exponent + 1) > big; rows of zeros, infinities and NaN keep scale 1
+      float s = 1.f;
+      if (big > 1e-30f && big < 1e38f) s = __int_as_float((__float_as_int(big) & 0x7F800000) + 0x00800000);
+      if (t == 0 && blk == 0) row_scale[r] = s;
+      const float inv = 1.f / s;  // exact
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[i][e] *= inv;
     }
     uint32_t f[4][NT];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) split2<Q8, NT>(x[2 * e], x[2 * e + 1], f[e]);
+    for (int e = 0; e < 4; ++e) split2<Q8, NT>(x[i][2 * e], x[i][2 * e + 1], f[e]);
 #pragma unroll
     for (int e = 0; e < NT; ++e)
-      *reinterpret_cast<uint4*>(smem + (((e * NB + blk) * NN + nt) * 32 + ln) * 16) =
+      *reinterpret_cast<uint4*>(smem + (((e * NB + blk) * NN + nt) * 32 + lane) * 16) =
           make_uint4(f[0][e], f[1][e], f[2][e], f[3][e]);
     if constexpr (C::kInit > 0) {
       float q = 0.f;  // of the fp16 values
@@ -328,7 +390,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
       }
       q += __shfl_xor_sync(0xffffffffu, q, 1);
       q += __shfl_xor_sync(0xffffffffu, q, 2);
-      if (lt == 0) init[blk * C::kRows + r] = q * (-128.f / 16777216.f);
+      if (t == 0) init[blk * C::kRows + r] = q * (-128.f / 16777216.f);
     }
   }
   __syncthreads();
@@ -622,7 +684,8 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
   __syncthreads();  // the rings are free: partial O of the warps go over them
-  float* part = reinterpret_cast<float*>(smem + C::kHead);  // [warp][row][HD]
+  constexpr int PS = HD + 4;  // a row's stride: the stores below touch every bank once
+  float* part = reinterpret_cast<float*>(smem + C::kHead);  // [warp][row][PS]
 #pragma unroll
   for (int n = 0; n < NN; ++n) {
     if (g == 0) {
@@ -631,7 +694,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float* p = part + (warp * C::kRows + 8 * n + 2 * t + e) * HD;
+      float* p = part + (warp * C::kRows + 8 * n + 2 * t + e) * PS;
       if constexpr (Q8) {
 #pragma unroll
         for (int i = 0; i < HD / 16; i += 2)
@@ -663,8 +726,8 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
       if (gm[w][r] == -INFINITY && gl[w][r] == gl[w][r]) continue;  // no key seen by this warp
       const float f = gm[w][r] == -INFINITY ? 0.f : fast_exp2(gm[w][r] - M);
       L = fmaf(f, gl[w][r], L);
-      const float4 p0 = *reinterpret_cast<const float4*>(part + (w * C::kRows + r) * HD + d);
-      const float4 p1 = *reinterpret_cast<const float4*>(part + (w * C::kRows + r) * HD + d + 4);
+      const float4 p0 = *reinterpret_cast<const float4*>(part + (w * C::kRows + r) * PS + d);
+      const float4 p1 = *reinterpret_cast<const float4*>(part + (w * C::kRows + r) * PS + d + 4);
       o[0] = fmaf(f, p0.x, o[0]), o[1] = fmaf(f, p0.y, o[1]), o[2] = fmaf(f, p0.z, o[2]), o[3] = fmaf(f, p0.w, o[3]);
       o[4] = fmaf(f, p1.x, o[4]), o[5] = fmaf(f, p1.y, o[5]), o[6] = fmaf(f, p1.z, o[6]), o[7] = fmaf(f, p1.w, o[7]);
     }
@@ -697,17 +760,28 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
   // those leave threads idle, over parts of the splits.
   const float* recs = a.recs + unit * a.n_splits * kRec;
   float* wts = reinterpret_cast<float*>(smem + C::kHead);  // [row][split]
-  for (int r = warp; r < rows; r += W) {
-    float M = -INFINITY, L = 0.f;
-    for (int sp = lane; sp < active; sp += 32) M = fmaxf(M, __ldcg(recs + (int64_t)sp * kRec + 2 * r));
+  constexpr int RW = C::kRows / W;
+  float2 ml[RW][2];  // of two splits a lane (kPaMaxSplits): all rows' loads together
+#pragma unroll
+  for (int i = 0; i < RW; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = warp + i * W, sp = lane + 32 * h;
+      ml[i][h] = make_float2(-INFINITY, 0.f);
+      if (r < rows && sp < active) ml[i][h] = __ldcg(reinterpret_cast<const float2*>(recs + (int64_t)sp * kRec + 2 * r));
+    }
+#pragma unroll
+  for (int i = 0; i < RW; ++i) {
+    const int r = warp + i * W;
+    float M = fmaxf(ml[i][0].x, ml[i][1].x), L = 0.f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    for (int sp = lane; sp < active; sp += 32) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(recs + (int64_t)sp * kRec + 2 * r));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
       // (m -infinity: no key seen, unless l is NaN)
-      const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
-      L += ml.x == -INFINITY && ml.y == ml.y ? 0.f : f * ml.y;
-      wts[r * a.n_splits + sp] = f;
+      const float f = ml[i][h].x == -INFINITY ? 0.f : fast_exp2(ml[i][h].x - M);
+      L += ml[i][h].x == -INFINITY && ml[i][h].y == ml[i][h].y ? 0.f : f * ml[i][h].y;
+      if (r < rows && lane + 32 * h < active) wts[r * a.n_splits + lane + 32 * h] = f;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
@@ -775,8 +849,7 @@ static int pick_nn(int max_q, int group, int hd) {
 static int pick_splits(int64_t units, int max_kv, int ctas) {
   if (units > kPagedCounters || units < 1) return 1;
   const int64_t slots = (int64_t)ctas * device_sm_count();
-  const int64_t want = units * 8 <= slots ? 2LL * device_sm_count() : 2 * slots;
-  const int64_t s = std::min(want / units, ((int64_t)max_kv + kPaMinSplit - 1) / kPaMinSplit);
+  const int64_t s = std::min(4 * slots / units, ((int64_t)max_kv + kPaMinSplit - 1) / kPaMinSplit);
   return (int)std::max<int64_t>(1, std::min<int64_t>(s, kPaMaxSplits));
 }
 struct PaPlan {
@@ -817,22 +890,31 @@ size_t paged_attn_workspace_bytes(const PagedView& c, int n, int group, int hd, 
 }
 
 template <int HD, bool Q8, bool F32, int NN>
-static cudaError_t launch_t(const PagedAttnArgs& a, const PaPlan& p, cudaStream_t st) {
+static cudaError_t launch_t(PagedAttnArgs a, const PaPlan& p, cudaStream_t st) {
   using C = PaCfg<HD, Q8, F32, NN>;
-  static int attr_set[64] = {0};
-  int dev = 0;
+  static int ctas_of[64] = {0};  // CTAs an SM holds
+  int dev = 0, ctas = 0;
   cudaGetDevice(&dev);
-  if (dev >= 64 || !attr_set[dev]) {
+  if (dev < 64) ctas = ctas_of[dev];
+  if (ctas == 0) {
     cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<HD, Q8, F32, NN>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem());
+    if (e == cudaSuccess)
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, paged_attn_kernel<HD, Q8, F32, NN>, kPaThreads,
+                                                        C::smem());
     if (e != cudaSuccess) return e;
-    if (dev < 64) attr_set[dev] = 1;
+    ctas = std::max(ctas, 1);
+    if (dev < 64) ctas_of[dev] = ctas;
   }
+  const int64_t slots = (int64_t)ctas * device_sm_count();
+  const bool few = p.units * 8 <= slots;
+  a.want = (float)(few ? kPaFew * device_sm_count() : slots) / (float)a.c.kv_heads;
+  a.waves = few ? 1 : 2;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.tiles, (unsigned)p.splits, (unsigned)a.c.kv_heads);
+  cfg.gridDim = dim3((unsigned)p.tiles, (unsigned)a.c.kv_heads, (unsigned)p.splits);
   cfg.blockDim = dim3(kPaThreads);
   cfg.dynamicSmemBytes = C::smem();
   cfg.stream = st;

@@ -27,6 +27,8 @@ struct PagedAttnArgs {
   int n, n_seqs, heads, group, n_splits;
   int min_new, max_new;  // this kernel takes the sequences with min_new <= new tokens < max_new
   int per_seq;           // row tiles of every sequence, or 0: tiles by the tokens' places
+  float want;            // warp MMA: CTAs of a key/value head that run at a time
+  int waves;             // ... and how often over at most
 };
 
 struct RowTile {
