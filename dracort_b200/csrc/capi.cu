@@ -622,7 +622,7 @@ int draco_verify_drafts(const draco_verify_args* args, void* stream) {
   if (a.n < 0 || a.n_seqs < 0 || a.vocab < 1 || a.max_rows < 1 || a.n_seqs > (1 << 24) || a.vocab > (1 << 30))
     return fail(DRACO_ERR_SHAPE, "%s: %d rows of %d, %d sequences of at most %d rows", fn, a.n, a.vocab, a.n_seqs,
                 a.max_rows);
-  if (!(a.temperature >= 0.f) || a.temperature > 1e30f)
+  if (!(a.temperature >= 0.f) || a.temperature > 1e30f || (a.temperature > 0.f && a.temperature < 1e-30f))
     return fail(DRACO_ERR_ARG, "%s: temperature %g", fn, (double)a.temperature);
   if (a.n_seqs == 0) return ok();
   if (!a.row_start || !a.accepted || !a.tokens || (a.n > 0 && (!a.logits || !a.drafts)) ||

@@ -18,7 +18,7 @@
 // fragment through two 8x8 transposes (movmatrix).
 // A warp takes the 16-key blocks of the CTA's key range in turn with the three
 // others, fills its own ring with cp.async and waits for nobody; the warps
-// merge in shared memory.  Long ranges are split over CTAs (blockIdx.y) and
+// merge in shared memory.  Long ranges are split over CTAs (blockIdx.z) and
 // merged, in split order, by the last CTA to arrive.
 //
 // Precision.  fp32 activations keep 22-24 bits: operands go into the MMAs as
@@ -157,11 +157,11 @@ struct PaCfg {
   static constexpr int kInit = Q8 && !F32 ? (HD / 32) * kRows * 4 : 0;  // -128 sum(q) of every block
   static constexpr int kHead = kQBytes + kInit;
   static constexpr int kMerge = kWarps * kRows * (HD + 4) * 4;    // partial O of the warps
-  // four CTAs per SM for Q8_0, whose warps compute, two for bf16, whose
-  // stages are larger, where that leaves two stages
-  static constexpr int kCtas = Q8 ? 4 : 2;
+  // shared memory for four CTAs per SM over Q8_0, whose warps compute, three
+  // over bf16 (32 sequences of 4000: 94 us with two, 90 with three), where that
+  // leaves two stages
   static constexpr int stages() {
-    int s = ((Q8 ? 56 : 110) * 1024 - kHead) / (kStage * kWarps);
+    int s = ((Q8 ? 56 : 74) * 1024 - kHead) / (kStage * kWarps);
     return s < 2 ? 2 : s > 6 ? 6 : s;
   }
   static constexpr int kStages = stages();
@@ -868,7 +868,7 @@ static PaPlan plan_of(int n, int n_seqs, int group, int kv_heads, int hd, int ma
   p.per_seq = per > 0 && per * n_seqs <= p.tiles ? (int)per : 0;
   if (p.per_seq) p.tiles = per * n_seqs;
   p.units = p.tiles * kv_heads;
-  p.splits = pick_splits(p.units, max_kv, q8 ? 4 : 2);
+  p.splits = pick_splits(p.units, max_kv, q8 ? 4 : 3);
   p.bytes = p.splits > 1 ? (size_t)p.units * p.splits * 8 * p.nn * (hd + 2) * sizeof(float) : 0;
   return p;
 }

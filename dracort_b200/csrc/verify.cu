@@ -79,29 +79,41 @@ __device__ __forceinline__ float logit(const T* p) {
   return x == x ? x : -INFINITY;  // a NaN logit is never drawn
 }
 
-// 2^(t / 256) for t <= 0 in fp64 (a few units in the last place), by P. T. P.
-// Tang's table-driven method: t = 256 k + j + f with |f| <= 1/2, the value is
-// 2^k 2^(j/256) e^r, r = f ln2 / 256, e^r by its Taylor series to r^4 (r^5 / 120 <
-// 4e-17).  Half the fp64 instructions of exp(), which bound the drawing.
-constexpr double kTangScale = 369.3299304675746;  // 256 / ln2
+// An fp32 value as fp64 by its bits (the conversion instruction runs at a
+// quarter of the fp64 rate): exact, but that zero, subnormal values and
+// infinities come out as numbers of 2^-127 .. 2^-126 and 2^128.
+__device__ __forceinline__ double wide(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return __hiloint2double((int)((u & 0x80000000u) | (((u & 0x7FFFFFFFu) >> 3) + 0x38000000u)), (int)(u << 29));
+}
+
+// exp((x - m) / T) in fp64 by P. T. P. Tang's table-driven method: with k the
+// integer next to (x - m) 256 / (T ln2), found in fp32, r = (x - m) / T - k ln2 /
+// 256 (|r| < 0.0014), the value is 2^(k / 256) e^r, the first factor from a table
+// and the exponent, e^r by its Taylor series to r^3: 2e-13 of the value.  Half
+// the fp64 instructions of exp(), which bound the drawing.
+constexpr float kTangScale = 369.32993f;  // 256 / ln2
 constexpr int kTable = 256;
-__device__ __forceinline__ double exp2_256(double t, const double* table) {
-  const double kd = t + 6755399441055744.0;  // 1.5 * 2^52: the nearest integer in the low bits
-  const int n = __double2loint(kd);
-  const double r = (t - (kd - 6755399441055744.0)) * 0.0027076061740622863;  // ln2 / 256
-  double p = fma(r, 1.0 / 24.0, 1.0 / 6.0);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  p *= table[n & (kTable - 1)];
-  const double v = __hiloint2double(__double2hiint(p) + ((n >> 8) << 20), __double2loint(p));
-  return t > -256000.0 ? v : 0.0;  // below 2^-1000 (and for -infinity): nothing
-}
-// exp((x - m) / T); t256 = 256 / (T ln2)
-__device__ __forceinline__ double weight64(float x, double m, double t256, const double* table) {
-  const double xd = (double)x;
-  return xd == m ? 1.0 : exp2_256((xd - m) * t256, table);
-}
+struct Weight64 {
+  float m, scale;   // the row's maximum, 256 / (T ln2)
+  double inv_t, m_t;  // 1 / T, m / T
+  const double* table;  // 2^(j / 256)
+  __device__ __forceinline__ double operator()(float x) const {
+    const float t = (x - m) * scale;
+    const float kf = t + 12582912.f;  // 1.5 * 2^23: the nearest integer in the low bits
+    const int k = __float_as_int(kf) - 0x4B400000;
+    // 1.5 * 2^52 + 2^31 + k, for k of either sign in the low word, less its offset
+    const double kd = __hiloint2double(0x43380000, (int)((uint32_t)k + 0x80000000u)) - 6755401588539392.0;
+    const double r = fma(kd, -0.0027076061740622863, fma(wide(x), inv_t, -m_t));
+    double p = fma(r, 1.0 / 6.0, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    p *= table[k & (kTable - 1)];
+    const double v = __hiloint2double(__double2hiint(p) + ((k >> 8) << 20), __double2loint(p));
+    // below 2^-1000 (and for -infinity) nothing; the maximum itself may be infinite
+    return x == m ? 1.0 : t > -256000.f ? v : 0.0;
+  }
+};
 
 // pairs of fp32 values
 __device__ __forceinline__ uint64_t pair_2(float a, float b) {
@@ -317,7 +329,7 @@ __global__ void __launch_bounds__(kVfThreads, 3) verify_kernel(const VerifyArgs 
       const T* row = logits + (int64_t)rr * a.ld_logits;
       const int x = rejected && a.probs == nullptr ? a.drafts[rr] : -1;  // a point mass is taken out
       const float* q = rejected && a.probs != nullptr ? a.probs + (int64_t)rr * a.ld_probs : nullptr;
-      const double m64 = (double)at.m, t256 = a.inv_t * kTangScale;
+      const Weight64 weight{at.m, (float)a.inv_t * kTangScale, a.inv_t, (double)at.m * a.inv_t, table};
       // The warp's range in vocabulary order, in blocks of K values a lane: value
       // k of lane L is base + 32 k + L.
       constexpr int K = 8;
@@ -349,11 +361,11 @@ __global__ void __launch_bounds__(kVfThreads, 3) verify_kernel(const VerifyArgs 
         }
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-          w[k] = weight64(v[k], m64, t256, table);
+          w[k] = weight(v[k]);
           if (!of_p) {
             if (q != nullptr) {
-              const double d = w[k] * inv_z - (double)u[k];
-              w[k] = d > 0.0 ? d : 0.0;
+              const double d = fma(w[k], inv_z, -wide(u[k]));
+              w[k] = __double2hiint(d) > 0 ? d : 0.0;
             } else if (i0 + 32 * k == x) {
               w[k] = 0.0;
             }

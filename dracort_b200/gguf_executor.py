@@ -690,8 +690,8 @@ class GPUExecutionBackend:
             raise ValueError(f"num_drafts {num_drafts} must lie in 0..{_ROWS - 1}")
         if ngram < 1:
             raise ValueError(f"ngram {ngram} must be at least 1")
-        if not 0.0 <= temperature < 1e30:
-            raise ValueError(f"temperature {temperature} must not be negative")
+        if not (temperature == 0.0 or 1e-30 < temperature < 1e30):
+            raise ValueError(f"temperature {temperature} must be 0 (greedy) or positive")
         ids = [int(t) for t in prompt_ids]
         if not ids:
             raise ValueError("the prompt holds no token")

@@ -572,7 +572,7 @@ size_t draco_attention_paged_workspace_bytes(const draco_kv_cache* cache, int n,
  *   draft_probs : fp32 [n, vocab], row stride ld_probs: the drafter's
  *                 probabilities, or NULL: each draft was certain
  *   accept_u    : fp32 [n], sample_u fp32 [n_seqs]: uniform numbers in [0, 1)
- *   temperature : p = softmax(logits / temperature); 0: greedy
+ *   temperature : p = softmax(logits / temperature), 1e-30 .. 1e30; 0: greedy
  * Draft x of row r is taken while accept_u[r] * q(x) < p(x) (greedy: x is the
  * first index of the largest logit); at the first that is not, the next token
  * is drawn from max(p - q, 0) (from p where that is zero everywhere), after the

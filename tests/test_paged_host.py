@@ -101,7 +101,7 @@ def test_attention_calls_that_are_refused(status, kw):
 
 @pytest.mark.parametrize("status,kw", [
     (TYPE, dict(dtype=9)), (SHAPE, dict(n=-1)), (SHAPE, dict(n_seqs=-1)), (SHAPE, dict(vocab=0)),
-    (SHAPE, dict(max_rows=0)), (SHAPE, dict(vocab=(1 << 30) + 1)), (ARG, dict(temperature=-0.5)),
+    (SHAPE, dict(max_rows=0)), (SHAPE, dict(vocab=(1 << 30) + 1)), (ARG, dict(temperature=-0.5)), (ARG, dict(temperature=1e-38)),
     (ARG, dict(temperature=float("nan"))), (ARG, dict(row_start=None)), (ARG, dict(accepted=None)),
     (ARG, dict(tokens=None)), (ARG, dict(logits=None)), (ARG, dict(drafts=None)), (ARG, dict(accept_u=None)),
     (ARG, dict(sample_u=None)), (SHAPE, dict(ld_logits=-1)), (SHAPE, dict(ld_tokens=3)),
