@@ -255,7 +255,8 @@ __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(const PagedView c
 }
 
 // rows of the given positions, keys to k_out and values to v_out
-// [n, kv_heads, head_dim]; a thread takes 16 values of each of its rows
+// [n, kv_heads, head_dim]; a thread takes 16 values of each of its rows, in groups
+// whose 16-byte stores touch those of the next lane
 template <typename T, int HD, bool Q8, int U>
 __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const PagedView c, const int* __restrict__ seq,
                                                              const int* __restrict__ pos, T* k_out, T* v_out,
@@ -266,8 +267,8 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const PagedView c, 
   grid_launch_dependents();
   const int lane = (threadIdx.x & 31) % S::kLanes;
   const int t0 = kv_lookup(c, wk, seq, pos, 0x7FFFFFFFFFFFFFFFll, s_page, s_pos);
-  uint4 w[U][Q8 ? 1 : 2];
-  uint32_t d[U];
+  constexpr int V = 16 / (int)sizeof(T), G = 16 / V, W = Q8 ? V / 4 : V / 2;  // values and words of a group, groups
+  uint32_t w[U][G][W], d[U][G];
   auto fetch = [&](const KvItem& it) {
     const int page = it.on ? s_page[it.token - t0] : -1, off = s_pos[it.token - t0] & ((1 << c.page_shift) - 1);
 #pragma unroll
@@ -276,13 +277,26 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const PagedView c, 
       const uint8_t* blk = (r < c.kv_heads ? c.k : c.v) + ((int64_t)max(page, 0) * c.kv_heads + h) * c.block_bytes;
       const bool have = page >= 0 && r < wk.rows;  // a row outside the cache reads as zeros
 #pragma unroll
-      for (int e = 0; e < (Q8 ? 1 : 2); ++e) {
-        w[u][e] = make_uint4(0, 0, 0, 0);
-        if (have) w[u][e] = __ldg(reinterpret_cast<const uint4*>(blk + ((int64_t)off * HD + 16 * lane) * (Q8 ? 1 : 2)) + e);
+      for (int e = 0; e < G; ++e) {
+        const int at = V * (lane + e * S::kLanes);
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(blk + ((int64_t)off * HD + at) * (Q8 ? 1 : 2));
+#pragma unroll
+        for (int j = 0; j < W; ++j) w[u][e][j] = 0u;
+        d[u][e] = 0u;
+        if (have) {
+          if constexpr (W == 4) {
+            const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+            w[u][e][0] = x.x, w[u][e][1] = x.y, w[u][e][2] = x.z, w[u][e][3] = x.w;
+          } else if constexpr (W == 2) {
+            const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+            w[u][e][0] = x.x, w[u][e][1] = x.y;
+          } else {
+            w[u][e][0] = __ldg(p);
+          }
+          if constexpr (Q8)
+            d[u][e] = __ldg(reinterpret_cast<const uint16_t*>(blk + ((int64_t)HD << c.page_shift)) + off * (HD / 32) + at / 32);
+        }
       }
-      d[u] = 0;
-      if (Q8 && have)
-        d[u] = __ldg(reinterpret_cast<const uint16_t*>(blk + ((int64_t)HD << c.page_shift)) + off * (HD / 32) + lane / 2);
     }
   };
   const int steps = (wk.span + S::kRows - 1) / S::kRows;
@@ -291,64 +305,84 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const PagedView c, 
 #pragma unroll 1
   for (int st = 0; st < steps; ++st) {
     const int64_t i = it.token;
-    uint4 now[U][Q8 ? 1 : 2];
-    float sc[U];
+    uint32_t now[U][G][W];
+    float sc[U][G];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < (Q8 ? 1 : 2); ++e) now[u][e] = w[u][e];
-      sc[u] = f16_bits_to_f32(d[u]);
-    }
+      for (int e = 0; e < G; ++e) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) now[u][e][j] = w[u][e][j];
+        sc[u][e] = f16_bits_to_f32(d[u][e]);
+      }
     const KvItem next = kv_item<HD>(wk, st + 1);
     if (st + 1 < steps) fetch(next);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int r = it.row + u * wk.step, h = r < c.kv_heads ? r : r - c.kv_heads;
       if (!it.on || r >= wk.rows) continue;
-      T* dst = (r < c.kv_heads ? k_out + i * ldk : v_out + i * ldv) + (int64_t)h * HD + 16 * lane;
-      if constexpr (Q8) {
-        const uint32_t ws[4] = {now[u][0].x ^ 0x80808080u, now[u][0].y ^ 0x80808080u, now[u][0].z ^ 0x80808080u,
-                                now[u][0].w ^ 0x80808080u};
-        float x[2][8];
+      T* dst = (r < c.kv_heads ? k_out + i * ldk : v_out + i * ldv) + (int64_t)h * HD + V * lane;
 #pragma unroll
-        for (int j = 0; j < 16; ++j)  // 2^23 + (quant + 128), exact
-          x[j >> 3][j & 7] =
-              sc[u] * (__uint_as_float(__byte_perm(ws[j >> 2], 0x4B000000u, 0x7440u | (j & 3))) - 8388736.f);
-        store8(dst, x[0]);
-        store8(dst + 8, x[1]);
-      } else if constexpr (sizeof(T) == 2) {
-        reinterpret_cast<uint4*>(dst)[0] = now[u][0];
-        reinterpret_cast<uint4*>(dst)[1] = now[u][1];
-      } else {
+      for (int e = 0; e < G; ++e) {
+        float x[V];
+        if constexpr (Q8) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint4 z = now[u][e];
-          float x[8] = {bf16lo(z.x), bf16hi(z.x), bf16lo(z.y), bf16hi(z.y),
-                        bf16lo(z.z), bf16hi(z.z), bf16lo(z.w), bf16hi(z.w)};
-          store8(dst + 8 * e, x);
+          for (int j = 0; j < V; ++j)  // 2^23 + (quant + 128), exact
+            x[j] = sc[u][e] * (__uint_as_float(__byte_perm(now[u][e][j >> 2] ^ 0x80808080u, 0x4B000000u,
+                                                           0x7440u | (j & 3))) - 8388736.f);
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; j += 2) x[j] = bf16lo(now[u][e][j / 2]), x[j + 1] = bf16hi(now[u][e][j / 2]);
         }
+        uint4 o;
+        if constexpr (sizeof(T) == 4)
+          o = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+        else if constexpr (!Q8)
+          o = make_uint4(now[u][e][0], now[u][e][1], now[u][e][2], now[u][e][3]);
+        else
+          o = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+        *reinterpret_cast<uint4*>(dst + V * e * S::kLanes) = o;
       }
     }
     it = next;
   }
 }
 
+// CTAs of a kernel that an SM holds
+template <auto Kernel>
+static int kv_ctas() {
+  static int ctas_of[64] = {0};
+  int dev = 0, ctas = 0;
+  cudaGetDevice(&dev);
+  if (dev < 64) ctas = ctas_of[dev];
+  if (ctas == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, Kernel, kKvThreads, 0) != cudaSuccess) ctas = 1;
+    ctas = std::max(ctas, 1);
+    if (dev < 64) ctas_of[dev] = ctas;
+  }
+  return ctas;
+}
+
 // U rows of a thread at a time: one while the call does not fill the GPU
-// (latency counts), else `most`.  A block's span is then what gives four blocks
-// an SM, up to 16 steps and kKvTokens tokens.
-static KvWalk kv_walk(int n, int rows, int lanes, int per_step, int most, int* unroll) {
+// (latency counts), else `most`.
+static int kv_unroll(int n, int rows, int lanes, int most) {
+  return (int64_t)n * rows * lanes > 2048LL * device_sm_count() ? most : 1;
+}
+// A block's span: up to 16 steps and kKvTokens tokens, as many as make whole
+// waves of blocks (8.4k prompt tokens to Q8_0 with 16 steps, 2.2 waves: 46 us;
+// three waves of 12: see the kernel).
+static KvWalk kv_walk(int n, int rows, int per_step, int unroll, int ctas) {
   KvWalk w;
   w.n = n;
   w.rows = rows;
-  const int64_t room = 2048LL * device_sm_count();
-  *unroll = (int64_t)n * rows * lanes > room ? most : 1;
-  w.step = (rows + *unroll - 1) / *unroll;
+  w.step = (rows + unroll - 1) / unroll;
   const int64_t total = (int64_t)n * w.step;
   w.total = (unsigned)total;
-  const int64_t blocks = 4LL * device_sm_count();
-  int64_t steps = std::max<int64_t>(1, std::min<int64_t>(16, total / (blocks * per_step)));
-  while (steps > 1 && steps * per_step / w.step + 2 > kKvTokens) steps /= 2;
-  w.span = (int)(steps * per_step);
+  const int64_t all = (total + per_step - 1) / per_step, slots = (int64_t)ctas * device_sm_count();
+  int64_t most = 16;
+  while (most > 1 && most * per_step / w.step + 2 > kKvTokens) most /= 2;
+  const int64_t waves = std::max<int64_t>(1, (all + most * slots - 1) / (most * slots));
+  w.span = (int)(std::max<int64_t>(1, (all + waves * slots - 1) / (waves * slots)) * per_step);
   return w;
 }
 static_assert(kKvThreads / 2 + 2 <= kKvTokens, "one step's tokens");
@@ -371,8 +405,9 @@ template <typename T, int HD, bool Q8>
 static cudaError_t append_t(const PagedView& c, const draco_kv_append_args& a, cudaStream_t st) {
   using S = KvShape<HD>;
   constexpr int kMost = sizeof(T) == 4 ? 2 : 4;  // 32 registers of loads in flight
-  int u;
-  const KvWalk w = kv_walk(a.n, a.heads + 2 * c.kv_heads, S::kLanes, S::kRows, kMost, &u);
+  const int rows = a.heads + 2 * c.kv_heads, u = kv_unroll(a.n, rows, S::kLanes, kMost);
+  const KvWalk w = kv_walk(a.n, rows, S::kRows, u,
+                           u == 1 ? kv_ctas<kv_append_kernel<T, HD, Q8, 1>>() : kv_ctas<kv_append_kernel<T, HD, Q8, kMost>>());
   const KvAppend k = {a.q,   a.k,    a.v,         a.q_out,     a.ldq,           a.ldk, a.ldv,
                       a.ldqo, a.cos_table, a.sin_table, a.max_positions, a.seq, a.pos, a.heads};
   return launch_walk(u == 1 ? kv_append_kernel<T, HD, Q8, 1> : kv_append_kernel<T, HD, Q8, kMost>, w, st, c, k);
@@ -382,9 +417,10 @@ template <typename T, int HD, bool Q8>
 static cudaError_t read_t(const PagedView& c, const int* seq, const int* pos, int n, void* k_out, void* v_out,
                           int64_t ldk, int64_t ldv, cudaStream_t st) {
   using S = KvShape<HD>;
-  constexpr int kMost = 4;
-  int u;
-  const KvWalk w = kv_walk(n, 2 * c.kv_heads, S::kLanes, S::kRows, kMost, &u);
+  constexpr int kMost = 2;
+  const int rows = 2 * c.kv_heads, u = kv_unroll(n, rows, S::kLanes, kMost);
+  const KvWalk w = kv_walk(n, rows, S::kRows, u,
+                           u == 1 ? kv_ctas<kv_read_kernel<T, HD, Q8, 1>>() : kv_ctas<kv_read_kernel<T, HD, Q8, kMost>>());
   return launch_walk(u == 1 ? kv_read_kernel<T, HD, Q8, 1> : kv_read_kernel<T, HD, Q8, kMost>, w, st, c, seq, pos,
                      (T*)k_out, (T*)v_out, ldk, ldv);
 }
