@@ -466,7 +466,7 @@ static int check_kv_cache(const draco_kv_cache* c, const char* fn, PagedView* vi
                 "head_dim 32, 64, 96, 128 or 256; at most 1024 heads)",
                 fn, c->n_pages, c->page_size, c->kv_heads, c->head_dim);
   if (c->n_seqs < 0 || c->max_pages < 1 || c->table_stride < 0 ||
-      (int64_t)c->max_pages * c->page_size > 0x7FFFFFFF)
+      (int64_t)c->max_pages * c->page_size > 0x7FFF0000)  // positions, with room to round up, are 32-bit
     return fail(DRACO_ERR_SHAPE, "%s: block table of %d sequences, %d pages each, stride %lld", fn, c->n_seqs,
                 c->max_pages, (long long)c->table_stride);
   if (!c->k || !c->v || (c->n_seqs > 0 && !c->block_table)) return fail(DRACO_ERR_ARG, "%s: null cache pointer", fn);
@@ -573,7 +573,7 @@ int draco_attention_paged(const draco_kv_cache* cache, const draco_attention_pag
   if (a.n < 0 || a.heads < 1 || a.heads > 65536 || a.heads % c.kv_heads)
     return fail(DRACO_ERR_SHAPE, "%s: %d tokens, %d heads over %d key/value heads", fn, a.n, a.heads, c.kv_heads);
   if (a.max_q < 0 || a.max_kv < 0) return fail(DRACO_ERR_SHAPE, "%s: max_q %d, max_kv %d", fn, a.max_q, a.max_kv);
-  if (!(a.scale >= 0.f) || a.scale > 1e30f) return fail(DRACO_ERR_ARG, "%s: scale %g", fn, (double)a.scale);
+  if (!(a.scale >= 0.f) || a.scale > 65536.f) return fail(DRACO_ERR_ARG, "%s: scale %g", fn, (double)a.scale);
   if (a.n == 0 || c.n_seqs == 0) return ok();
   if ((int64_t)a.n * (a.heads / c.kv_heads) > 0x7FFF0000) return fail(DRACO_ERR_SHAPE, "%s: %d tokens", fn, a.n);
   if (!a.q || !a.out || !a.q_start || !a.kv_len) return fail(DRACO_ERR_ARG, "%s: null pointer", fn);
@@ -626,7 +626,7 @@ int draco_verify_drafts(const draco_verify_args* args, void* stream) {
     return fail(DRACO_ERR_ARG, "%s: temperature %g", fn, (double)a.temperature);
   if (a.n_seqs == 0) return ok();
   if (!a.row_start || !a.accepted || !a.tokens || (a.n > 0 && (!a.logits || !a.drafts)) ||
-      (a.temperature > 0.f && (!a.accept_u || !a.sample_u)))
+      (a.temperature > 0.f && ((a.n > 0 && !a.accept_u) || !a.sample_u)))
     return fail(DRACO_ERR_ARG, "%s: null pointer", fn);
   if (a.ld_logits < 0 || a.ld_tokens < a.max_rows || (a.draft_probs && a.ld_probs < 0))
     return fail(DRACO_ERR_SHAPE, "%s: a negative row stride, or rows of tokens that overlap", fn);

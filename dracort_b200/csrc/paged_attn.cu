@@ -56,8 +56,7 @@ constexpr int kPaThreads = 128;
 constexpr float kPaLazy = 8.f;
 constexpr int kPaMinSplit = 128;  // keys of a split at least: 2 blocks of each warp
 constexpr int kPaMaxSplits = 64;  // two a lane of the merging warp
-constexpr int64_t kPaFew = 2;
-constexpr float kPaFixed = 250.f;
+constexpr float kPaFixed = 250.f;  // keys' worth of time that a CTA's beginning and merge take (12k clocks at 45-60 a key)
 constexpr int kPaLookSeqs = 256;  // sequences whose lengths every CTA looks at
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
@@ -191,7 +190,7 @@ __device__ __forceinline__ int key_of(int n) {
 template <int R>
 __device__ __forceinline__ int split_keys(const PagedAttnArgs& a, int kend, int fresh0, int kv0) {
   int longest = kend;
-  float total = (float)kend, tiles = 1.f;
+  float tiles = (float)gridDim.x, total = tiles * (float)kend;  // many sequences: as if all were alike
   if (a.n_seqs <= kPaLookSeqs) {
     const int64_t cap = (int64_t)a.c.max_pages << a.c.page_shift;
     total = tiles = 0.f;
@@ -219,6 +218,7 @@ __device__ __forceinline__ int split_keys(const PagedAttnArgs& a, int kend, int 
     const float two = total / fmaxf(2.f * a.want - 0.5f * tiles, 0.5f * a.want);
     if (2.f * (two + kPaFixed) < aim + kPaFixed) aim = two;
   }
+  aim = fminf(aim, 1073741824.f);  // (rounded up below; two splits hold any sequence)
   const int ck = max((int)aim, (longest + a.n_splits - 1) / a.n_splits);
   return max(kPaMinSplit, (ck + 63) & ~63);
 }
@@ -840,12 +840,9 @@ static int pick_nn(int max_q, int group, int hd) {
   while (nn < most && rows > 8 * nn) nn *= 2;
   return nn;
 }
-// Splits of the keys, none shorter than kPaMinSplit.  A few units (one sequence)
-// are all alike: two CTAs an SM, more only add to the merge (16384 Q8_0
-// positions, 8 heads: 22.9 us with 37 splits, 25.6 with 64).  Many have
-// different lengths, which two waves of smaller pieces even out (48 sequences
-// of 900-8000 positions: 165 us with one wave, 127 with two; 32 equal ones over
-// bf16: 89 and 94).  `ctas`: CTAs an SM holds.
+// Splits of the keys at most, none shorter than kPaMinSplit: the grid's; the
+// kernel, which sees the lengths, uses those that it needs (split_keys).  Twice
+// what two waves take of sequences that are alike.  `ctas`: CTAs an SM holds.
 static int pick_splits(int64_t units, int max_kv, int ctas) {
   if (units > kPagedCounters || units < 1) return 1;
   const int64_t slots = (int64_t)ctas * device_sm_count();
@@ -876,14 +873,16 @@ static PaPlan plan_of(int n, int n_seqs, int group, int kv_heads, int hd, int ma
 // New tokens from which a sequence goes to the tensor-memory kernel, or 0: none
 // does.  Its CTA takes 256 rows at a time however few there are.
 constexpr int kTcMinRows = 64;
-static int tc_from(const PagedView& c, int hd, int dtype, int group, int max_q) {
+static int tc_from(const PagedView& c, int n, int hd, int dtype, int group, int max_q, int max_kv) {
   if (!paged_attn_tc_takes(c, hd, dtype, group, 1 << c.page_shift)) return 0;
   const int from = kTcMinRows / group + 1;
-  return max_q >= from ? from : 0;
+  if (max_q < from) return 0;
+  // (its tiles are the grid's y)
+  return paged_attn_tc_plan(n, c.n_seqs, group, c.kv_heads, hd, max_kv).tiles <= 65535 ? from : 0;
 }
 
 size_t paged_attn_workspace_bytes(const PagedView& c, int n, int group, int hd, int dtype, int max_q, int max_kv) {
-  const int from = tc_from(c, hd, dtype, group, max_q);
+  const int from = tc_from(c, n, hd, dtype, group, max_q, max_kv);
   size_t bytes = plan_of(n, c.n_seqs, group, c.kv_heads, hd, from ? from - 1 : max_q, max_kv, c.type == DRACO_KV_Q8_0).bytes;
   if (from) bytes = std::max(bytes, paged_attn_tc_plan(n, c.n_seqs, group, c.kv_heads, hd, max_kv).bytes);
   return kPagedHead + bytes;
@@ -907,8 +906,13 @@ static cudaError_t launch_t(PagedAttnArgs a, const PaPlan& p, cudaStream_t st) {
     if (dev < 64) ctas_of[dev] = ctas;
   }
   const int64_t slots = (int64_t)ctas * device_sm_count();
+  // A few units (one sequence) are all alike: two CTAs an SM, more only add to
+  // the merge (16384 Q8_0 positions, 8 heads: 26.1 us with one, 21.1 with two,
+  // 22.3 with three).  Others have different lengths, which two waves of smaller
+  // pieces may even out (48 sequences of 900-8000 positions: 132 us with one
+  // wave, 115 with two; drafts of nine: 59 and 66): the kernel chooses.
   const bool few = p.units * 8 <= slots;
-  a.want = (float)(few ? kPaFew * device_sm_count() : slots) / (float)a.c.kv_heads;
+  a.want = (float)(few ? 2LL * device_sm_count() : slots) / (float)a.c.kv_heads;
   a.waves = few ? 1 : 2;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -954,7 +958,7 @@ int paged_attn_launch(PagedAttnArgs a, int hd, int dtype, int max_q, int max_kv,
   a.recs = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kPagedHead);
   // long sequences to the tensor-memory kernel, the others (any that a batch
   // holds beside them: the lengths are on the device) to the warp MMA
-  const int from = tc_from(a.c, hd, dtype, a.group, max_q);
+  const int from = tc_from(a.c, a.n, hd, dtype, a.group, max_q, max_kv);
   a.min_new = 0;
   a.max_new = from ? from : 0x7FFFFFFF;
   const PaPlan p = plan_of(a.n, a.n_seqs, a.group, a.c.kv_heads, hd, from ? from - 1 : max_q, max_kv, q8);

@@ -153,6 +153,7 @@ __global__ void __launch_bounds__(kVfThreads, 3) verify_kernel(const VerifyArgs 
   __shared__ double table[kGreedy ? 1 : kTable];   // 2^(j / 256)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (!kGreedy && tid < kTable) table[tid] = exp2((double)tid / kTable);
+  cluster.barrier_arrive();  // waited for before the first store to another CTA: it has started then
   grid_dependency_wait();
   grid_launch_dependents();
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks(), b = blockIdx.x / ctas;
@@ -267,7 +268,10 @@ __global__ void __launch_bounds__(kVfThreads, 3) verify_kernel(const VerifyArgs 
       if (lane == 0) wstat[r][sub] = wst;
     }
     __syncthreads();
-    if (r0 > 0) cluster.sync();  // everybody has read the last rows' statistics
+    if (r0 > 0)
+      cluster.sync();  // everybody has read the last rows' statistics
+    else
+      cluster.barrier_wait();
     for (int idx = tid; idx < nr * kVfCtas; idx += kVfThreads) {  // a thread per (row, CTA to tell)
       if (idx % kVfCtas >= ctas) continue;
       RowStat st = wstat[idx / kVfCtas][0];
@@ -319,6 +323,7 @@ __global__ void __launch_bounds__(kVfThreads, 3) verify_kernel(const VerifyArgs 
     __syncthreads();  // full is written again for the next rows
   }
 
+  if (rows == 0) cluster.barrier_wait();
   int last = -1;
   if (rows > 0 && at.m > -INFINITY) {
     if constexpr (kGreedy) {

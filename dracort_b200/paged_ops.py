@@ -272,10 +272,11 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise DracoFormatError(f"out {tuple(out.shape)} is not shaped like q {tuple(shape)}")
     else:
         ldo = _rows(out, "out", dev, n, dtype, hd)
-    if scale is not None and not 0.0 < scale < 1e30:
-        raise ValueError(f"scale {scale} must be positive")
-    max_q = n if max_q is None else int(max_q)
-    max_kv = c.max_pages * c.page_size if max_kv is None else int(max_kv)
+    if scale is not None and not 1e-30 < scale <= 65536.0:
+        raise ValueError(f"scale {scale} must be positive and at most 65536")
+    held = c.max_pages * c.page_size
+    max_q = n if max_q is None or max_q > n else int(max_q)
+    max_kv = held if max_kv is None or max_kv > held else int(max_kv)
     a = N.AttentionPagedArgs(q.data_ptr(), out.data_ptr(), ldq, ldo, _vector(q_start, "q_start", dev, c.n_seqs + 1),
                              _vector(kv_len, "kv_len", dev, c.n_seqs), n, heads, max_q, max_kv,
                              0.0 if scale is None else scale, None, 0)
@@ -365,7 +366,7 @@ def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafts: torch.T
         raise ValueError("logits must be a CUDA tensor (this library has no CPU path)")
     dt = _dtype(logits, "logits")
     shape, stride = logits.shape, logits.stride()
-    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
+    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1) or shape[0] > 0x7FFFFFFF:
         raise DracoFormatError("logits must be [rows, vocab] with contiguous rows")
     n, vocab = shape
     seqs = row_start.shape[0] - 1 if row_start.dim() == 1 else -1

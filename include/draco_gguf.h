@@ -455,7 +455,8 @@ size_t draco_attention_workspace_bytes(int n, int heads, int head_dim, int max_p
  * for all), row p % page_size.  Sequences may share pages (a common prefix).  A position beyond
  * the table, or whose entry is outside 0..n_pages - 1, is never accessed: it
  * is not written, and reads as zeros.
- * head_dim 32, 64, 96, 128 or 256; page_size a power of two from 16 to 1024;
+ * head_dim 32, 64, 96, 128 or 256; page_size a power of two from 16 to 1024; at
+ * most 0x7FFF0000 positions per sequence;
  * k and v 16-byte aligned.  The reference's paged attention and block manager
  * (draco/attention/paged.py:26-269, draco/kv_cache/block.py:119-441) keep
  * pages of 16- or 32-bit values in torch. */
@@ -532,7 +533,7 @@ int draco_kv_read(const draco_kv_cache* cache, const int* seq, const int* pos, i
  * max_kv are upper bounds of the sequences' new tokens and cached positions.
  * They choose the kernels and size the launch and the workspace: tight ones
  * are faster; tokens of a sequence past max_q may be left out.
- * scale 0 means 1 / sqrt(head_dim).  m, l and the output are accumulated in
+ * scale is at most 65536; 0 means 1 / sqrt(head_dim).  m, l and the output are accumulated in
  * fp32; fp32 activations keep fp32 accuracy, bf16 ones round the
  * probabilities to 16 bits.
  * Workspace: at least draco_attention_paged_workspace_bytes() bytes, 16-byte

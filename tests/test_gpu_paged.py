@@ -332,6 +332,32 @@ def test_many_sequences():
     check(*b, P.attention_paged(*b, max_q=3, max_kv=93))
 
 
+def test_more_sequences_than_a_grid_s_second_dimension():
+    """70000 sequences of a token or two over one shared table row, with the default bounds."""
+    g = gen(33)
+    kc, vc = make_cache("bf16", 4, 1, 16, 32, g)
+    table = i32([[2, 0, 3]]).expand(70000, -1)
+    n = 70000 + 65
+    starts = torch.arange(70001, dtype=torch.int32, device=DEV)
+    starts[40000:] += 65  # one of them has 66
+    kv_len = torch.randint(1, 49, (70000,), generator=g, device=DEV).to(torch.int32)
+    kv_len[39999] = 40
+    q = randn(n, 1, 32, g=g, dtype=BF16)
+    out = P.attention_paged(q, kc, vc, table, starts, kv_len)
+    pick = [0, 1, 39998, 39999, 40000, 65535, 65536, 69999]
+    rows = torch.cat([torch.arange(int(starts[s]), int(starts[s + 1]), device=DEV) for s in pick])
+    sub = [0]
+    for s in pick:
+        sub.append(sub[-1] + int(starts[s + 1] - starts[s]))
+    check(q[rows], kc, vc, table[:8], i32(sub), kv_len[torch.tensor(pick, device=DEV)], out[rows])
+
+
+def test_bounds_above_any_length_are_taken_as_none():
+    b = batch([2, 1], [100, 3], 4, 2, 64, 16, "bf16", F32, seed=34)
+    want = P.attention_paged(*b)
+    assert torch.equal(P.attention_paged(*b, max_q=2 ** 32, max_kv=2 ** 40), want)
+
+
 def test_offsets_past_32_bits():
     """A cache of more than 2^32 bytes: its last pages."""
     pages, kv, page, hd = 17000, 8, 128, 128
@@ -648,6 +674,17 @@ def test_verify_of_more_rows_than_are_held_at_a_time_and_strided_logits():
     assert count.tolist() == want[0] == [149] and tokens.tolist() == want[1]
     count, short = P.verify_drafts(*args, draft_probs=probs, max_rows=10)
     assert count.tolist() == [149] and short.tolist() == [want[1][0][:10]]
+
+
+def test_verify_of_no_rows_at_all():
+    for t in (0.0, 1.0):
+        count, tokens = P.verify_drafts(torch.zeros((0, 50), device=DEV), i32([0, 0, 0]), i32([]),
+                                        torch.zeros(0, device=DEV), torch.zeros(2, device=DEV), temperature=t,
+                                        max_rows=3)
+        assert count.tolist() == [0, 0] and tokens.tolist() == [[-1] * 3] * 2
+    count, tokens = P.verify_drafts(torch.zeros((0, 50), device=DEV), i32([0]), i32([]), torch.zeros(0, device=DEV),
+                                    torch.zeros(0, device=DEV))
+    assert count.shape == (0,) and tokens.shape == (0, 1)
 
 
 def test_verify_in_a_graph():

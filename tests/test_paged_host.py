@@ -62,7 +62,7 @@ TYPE, SHAPE, ALIGN, ARG = N.DRACO_ERR_TYPE, N.DRACO_ERR_SHAPE, N.DRACO_ERR_ALIGN
     (TYPE, dict(type=0)), (TYPE, dict(type=2)), (SHAPE, dict(kv_heads=0)), (SHAPE, dict(kv_heads=1025)),
     (SHAPE, dict(head_dim=48)), (SHAPE, dict(head_dim=512)), (SHAPE, dict(page_size=8)), (SHAPE, dict(page_size=48)),
     (SHAPE, dict(page_size=2048)), (SHAPE, dict(n_pages=0)), (SHAPE, dict(n_seqs=-1)), (SHAPE, dict(max_pages=0)),
-    (SHAPE, dict(max_pages=1 << 27)), (SHAPE, dict(table_stride=-1)), (ARG, dict(k=None)), (ARG, dict(v=None)),
+    (SHAPE, dict(max_pages=1 << 27)), (SHAPE, dict(max_pages=(1 << 27) - 1)), (SHAPE, dict(table_stride=-1)), (ARG, dict(k=None)), (ARG, dict(v=None)),
     (ARG, dict(block_table=None)), (ALIGN, dict(k=PTR + 8)), (ALIGN, dict(v=PTR + 2)),
     (ALIGN, dict(block_table=PTR + 2))])
 def test_caches_that_are_refused(call, status, kw):
@@ -92,7 +92,7 @@ def test_reads_that_are_refused(status, kw):
 @pytest.mark.parametrize("status,kw", [
     (TYPE, dict(dtype=7)), (SHAPE, dict(n=-1)), (SHAPE, dict(heads=0)), (SHAPE, dict(heads=5)),
     (SHAPE, dict(max_q=-1)), (SHAPE, dict(max_kv=-1)), (ARG, dict(scale=-1.0)), (ARG, dict(scale=float("nan"))),
-    (ARG, dict(scale=float("inf"))), (ARG, dict(q=None)), (ARG, dict(out=None)), (ARG, dict(q_start=None)),
+    (ARG, dict(scale=float("inf"))), (ARG, dict(scale=65537.0)), (ARG, dict(q=None)), (ARG, dict(out=None)), (ARG, dict(q_start=None)),
     (ARG, dict(kv_len=None)), (SHAPE, dict(ldq=252)), (SHAPE, dict(ldo=0)), (ALIGN, dict(q=PTR + 4)),
     (ALIGN, dict(ldo=257)), (ALIGN, dict(kv_len=PTR + 1)), (SHAPE, dict(n=0x7FFFFFF0))])
 def test_attention_calls_that_are_refused(status, kw):
