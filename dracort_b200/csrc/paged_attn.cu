@@ -153,10 +153,11 @@ struct PaCfg {
   static constexpr int kRows = 8 * NN;                    // rows of a tile
   static constexpr int kWarps = kPaThreads / 32;
   static constexpr int kRowBytes = Q8 ? HD : HD * 2;
-  // row strides in shared memory without bank conflicts: ldmatrix wants the 8
-  // rows of a matrix 16 bytes apart (mod 128), the Q8_0 loads want 4 rows 32
-  // or 96 bytes apart
-  static constexpr int kStride = Q8 ? HD + (HD % 64 == 0 ? 32 : 0) : HD * 2 + 16;
+  // rows 16 bytes apart (mod 128) in shared memory: what ldmatrix wants of the 8
+  // rows of a matrix.  The Q8_0 loads take 32 bytes of 4 rows, which 32 bytes
+  // apart would not collide in any bank, but were slower (48 steps below: 112 us,
+  // 105 so).
+  static constexpr int kStride = kRowBytes + 16;
   static constexpr int kScale = Q8 ? HD / 16 : 0;           // scale bytes of a row
   static constexpr int kTile = 16 * (kStride + kScale);     // 16 keys, or values
   static constexpr int kStage = 2 * kTile;
@@ -174,20 +175,12 @@ struct PaCfg {
   static constexpr int kStages = stages();
   static constexpr int kRing = kStages * kStage * kWarps;
   static constexpr int smem() { return kHead + (kRing > kMerge ? kRing : kMerge); }
+  static constexpr int kMinCtas = NN == 1 && HD <= 128 ? 4 : 3;  // bounds the registers
   static_assert(kRowBytes % 16 == 0 && kStride % 16 == 0 && (16 * kScale) % 16 == 0, "16-byte copies");
   static_assert(smem() <= 220 * 1024, "shared memory");
   static_assert(kRing + kMerge > 0 && (kRing > kMerge ? kRing : kMerge) >= (kRows * kPaMaxSplits + 8 * kPaThreads) * 4,
                 "the merge's weights and sums");
 };
-
-// the key (0..7) behind row n of an 8-key MMA half: for Q8_0 an order in which
-// both the key loads (rows 0..3 and 4..7 together) and the value loads (n even,
-// n odd) touch rows that differ mod 4
-template <bool Q8>
-__device__ __forceinline__ int key_of(int n) {
-  if constexpr (!Q8) return n;
-  return (0x57463120 >> (4 * n)) & 0xF;
-}
 
 // Keys of a split: the same for all tiles of the batch, so that all CTAs but a
 // tile's last run equally long, and so many that the batch makes one or two
@@ -232,7 +225,7 @@ __device__ __forceinline__ int split_keys(const PagedAttnArgs& a, int kend, int 
 }
 
 template <int HD, bool Q8, bool F32, int NN>
-__global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(kPaThreads, (PaCfg<HD, Q8, F32, NN>::kMinCtas)) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
   using C = PaCfg<HD, Q8, F32, NN>;
   using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
   constexpr int NT = C::kTerms, KS = C::kStride, NB = HD / 32, W = C::kWarps;
@@ -403,7 +396,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
   }
   __syncthreads();
 
-  // --- this thread's columns: rows 8 nt + 2t, + 1; its keys: key_of(g), 8 + key_of(g) of a block
+  // --- this thread's columns: rows 8 nt + 2t, + 1; its keys: g, g + 8 of a block
   int lim[NN][2];
   float sc[NN][2];
   const int first = min(tile.kv, row_limit(a, tile, tile.row0));  // the first row sees the fewest keys
@@ -417,7 +410,6 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
       sc[n][e] = a.scale_log2;
       if constexpr (Q8) sc[n][e] *= row_scale[r] * (F32 ? 1.f : 16777216.f);
     }
-  const int kg = key_of<Q8>(g), kc0 = key_of<Q8>(2 * t), kc1 = key_of<Q8>(2 * t + 1);
   constexpr float kShift = Q8 ? 6.f : 0.f;  // fp16 P: 2^6 at the reference, at most 2^14
   float acc[HD / 16][NN][4];
 #pragma unroll
@@ -464,7 +456,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     if constexpr (Q8) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint8_t* p = ks_s + (kg + 8 * h) * C::kScale;
+        const uint8_t* p = ks_s + (g + 8 * h) * C::kScale;
         if constexpr (NB == 1)
           dk[h][0] = *reinterpret_cast<const uint16_t*>(p);
         else if constexpr (NB == 3)
@@ -485,7 +477,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
       } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint2 w = *reinterpret_cast<const uint2*>(k_s + (kg + 8 * h) * KS + 32 * blk + 8 * t);
+          const uint2 w = *reinterpret_cast<const uint2*>(k_s + (g + 8 * h) * KS + 32 * blk + 8 * t);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const uint32_t x = (e ? w.y : w.x) ^ 0x80808080u;  // quant + 128
@@ -537,7 +529,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
 #pragma unroll
     for (int n = 0; n < NN; ++n) {
       if (edge) {
-        const int ka = k16 + kg, kb = ka + 8;
+        const int ka = k16 + g, kb = ka + 8;
         if (ka >= lim[n][0]) s[n][0] = -INFINITY;
         if (ka >= lim[n][1]) s[n][1] = -INFINITY;
         if (kb >= lim[n][0]) s[n][2] = -INFINITY;
@@ -586,10 +578,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
       if (__any_sync(0xffffffffu, bad)) {
 #pragma unroll 1
         for (int j = 0; j < 16; ++j) {
-          int src = 0;  // the quad that holds P of key j
-          for (int n = 0; n < 8; ++n)
-            if (key_of<Q8>(n) == (j & 7)) src = n;
-          src = 4 * src + t;
+          const int src = 4 * (j & 7) + t;  // holds P of key j
 #pragma unroll
           for (int n = 0; n < NN; ++n) {
             const float p0 = __shfl_sync(0xffffffffu, j < 8 ? s[n][0] : s[n][2], src);
@@ -649,7 +638,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
         uint32_t hi[2][4], lo[2][4];  // [keys 2t.. / 2t + 8..][dim 4g + j of the block]
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int ka = 8 * h + kc0, kb = 8 * h + kc1;
+          const int ka = 8 * h + 2 * t, kb = ka + 1;
           const uint32_t wa = *reinterpret_cast<const uint32_t*>(v_s + ka * KS + 32 * blk + 4 * g) ^ 0x80808080u;
           const uint32_t wb = *reinterpret_cast<const uint32_t*>(v_s + kb * KS + 32 * blk + 4 * g) ^ 0x80808080u;
           const uint32_t da = *reinterpret_cast<const uint16_t*>(vs_s + ka * C::kScale + 2 * blk);
