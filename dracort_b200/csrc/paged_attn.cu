@@ -633,6 +633,25 @@ __global__ void __launch_bounds__(kPaThreads, (PaCfg<HD, Q8, F32, NN>::kMinCtas)
         }
       }
     } else {
+      // scales of keys 2t, 2t + 1 and those + 8: neighbours, NB words
+      uint32_t dv[2][NB];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* p = vs_s + (8 * h + 2 * t) * C::kScale;
+        if constexpr (NB % 4 == 0) {
+#pragma unroll
+          for (int e = 0; e < NB; e += 4) {
+            const uint4 w = *reinterpret_cast<const uint4*>(p + 4 * e);
+            dv[h][e] = w.x, dv[h][e + 1] = w.y, dv[h][e + 2] = w.z, dv[h][e + 3] = w.w;
+          }
+        } else if constexpr (NB == 2) {
+          const uint2 w = *reinterpret_cast<const uint2*>(p);
+          dv[h][0] = w.x, dv[h][1] = w.y;
+        } else {
+#pragma unroll
+          for (int e = 0; e < NB; ++e) dv[h][e] = *reinterpret_cast<const uint32_t*>(p + 4 * e);
+        }
+      }
 #pragma unroll
       for (int blk = 0; blk < NB; ++blk) {
         uint32_t hi[2][4], lo[2][4];  // [keys 2t.. / 2t + 8..][dim 4g + j of the block]
@@ -641,9 +660,9 @@ __global__ void __launch_bounds__(kPaThreads, (PaCfg<HD, Q8, F32, NN>::kMinCtas)
           const int ka = 8 * h + 2 * t, kb = ka + 1;
           const uint32_t wa = *reinterpret_cast<const uint32_t*>(v_s + ka * KS + 32 * blk + 4 * g) ^ 0x80808080u;
           const uint32_t wb = *reinterpret_cast<const uint32_t*>(v_s + kb * KS + 32 * blk + 4 * g) ^ 0x80808080u;
-          const uint32_t da = *reinterpret_cast<const uint16_t*>(vs_s + ka * C::kScale + 2 * blk);
-          const uint32_t db = *reinterpret_cast<const uint16_t*>(vs_s + kb * C::kScale + 2 * blk);
-          const uint32_t dd = da | (db << 16);
+          // (key 2t's is half blk of the words, key 2t + 1's half NB + blk)
+          const uint32_t dd = __byte_perm(dv[h][blk / 2], dv[h][(NB + blk) / 2],
+                                          (blk & 1 ? 0x32 : 0x10) | ((NB + blk) & 1 ? 0x7600 : 0x5400));
           const uint32_t ab[2] = {__byte_perm(wa, wb, 0x5140), __byte_perm(wa, wb, 0x7362)};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
