@@ -27,6 +27,8 @@ draco/runtime/cpu/speculative.py.
 
 from __future__ import annotations
 
+import ctypes
+import struct
 import threading
 from typing import Dict, Optional, Tuple
 
@@ -67,7 +69,45 @@ def _cache_type(name: str) -> int:
 
 
 # The checks run on every call of a decode loop: the fast path touches each
-# tensor's properties once, and the messages are put together only on failure.
+# tensor's properties once, the messages are put together only on failure, and
+# the argument structures are packed as bytes (the mirrors of _native take three
+# times as long to fill).
+_KV_CACHE = struct.Struct("@7iq3P")           # draco_kv_cache
+_KV_APPEND = struct.Struct("@4P4q2Pq2P2i")    # draco_kv_append_args
+_ATTENTION = struct.Struct("@2P2q2P4if2P")    # draco_attention_paged_args
+_VERIFY = struct.Struct("@8P3qf5i")           # draco_verify_args
+
+
+class _Functions:
+    """The library's functions, with structures taken as packed bytes."""
+
+    def __init__(self) -> None:
+        lib, vp, ci = N.load(), ctypes.c_void_p, ctypes.c_int
+
+        def fn(name, *args, restype=ci):
+            f = lib[name]  # (an object of its own: _native's prototypes stay)
+            f.argtypes, f.restype = list(args), restype
+            return f
+
+        i64 = ctypes.c_int64
+        self.kv_append = fn("draco_kv_append", vp, vp, ci, vp)
+        self.kv_read = fn("draco_kv_read", vp, vp, vp, ci, vp, vp, i64, i64, ci, vp)
+        self.attention_paged = fn("draco_attention_paged", vp, vp, ci, vp)
+        self.workspace_bytes = fn("draco_attention_paged_workspace_bytes", vp, ci, ci, ci, ci, ci,
+                                  restype=ctypes.c_size_t)
+        self.verify_drafts = fn("draco_verify_drafts", vp, vp)
+
+
+_functions: Optional[_Functions] = None
+
+
+def _lib() -> _Functions:
+    global _functions
+    if _functions is None:
+        _functions = _Functions()
+    return _functions
+
+
 _I32, _F32 = torch.int32, torch.float32
 _current_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
@@ -98,7 +138,8 @@ def _rows(t: torch.Tensor, name: str, dev: int, n: int, dtype: torch.dtype, head
 
 
 def _cache_struct(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
-                  head_dim: int) -> N.KvCache:
+                  head_dim: int) -> Tuple[bytes, int, int, int]:
+    """(packed draco_kv_cache, kv_heads, sequences, positions of a sequence at most)"""
     shape, dtype, dev = k_cache.shape, k_cache.dtype, k_cache.get_device()
     if dev < 0:
         raise ValueError("k_cache must be a CUDA tensor (this library has no CPU path)")
@@ -124,8 +165,9 @@ def _cache_struct(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: tor
     if len(tshape) != 2 or (tshape[1] > 1 and tstride[1] != 1):
         raise DracoFormatError("block_table must be [sequences, pages] with contiguous rows")
     # (a table stride of 0: all sequences share one row)
-    return N.KvCache(kind, kv_heads, head_dim, page, pages, tshape[0], tshape[1], tstride[0],
-                     k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr())
+    seqs, width = tshape
+    return _KV_CACHE.pack(kind, kv_heads, head_dim, page, pages, seqs, width, tstride[0], k_cache.data_ptr(),
+                          v_cache.data_ptr(), block_table.data_ptr()), kv_heads, seqs, width * page
 
 
 def _dtype(t: torch.Tensor, name: str) -> int:
@@ -173,13 +215,13 @@ def kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_cac
     if len(shape) != 3:
         raise DracoFormatError(f"k must be [tokens, kv_heads, head_dim], not {tuple(shape)}")
     n, kv_heads, hd = shape
-    c = _cache_struct(k_cache, v_cache, block_table, hd)
+    c, cache_heads, _, _ = _cache_struct(k_cache, v_cache, block_table, hd)
     dev, dtype, dt = k_cache.get_device(), k.dtype, _dtype(k, "k")
     ldk, ldv = _rows(k, "k", dev, n, dtype, hd), _rows(v, "v", dev, n, dtype, hd)
-    if kv_heads != c.kv_heads or v.shape != shape:
-        raise DracoFormatError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match the cache's {c.kv_heads} heads")
+    if kv_heads != cache_heads or v.shape != shape:
+        raise DracoFormatError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match the cache's {cache_heads} heads")
     ldq = ldqo = heads = 0
-    q_ptr = qo_ptr = None
+    q_ptr = qo_ptr = 0
     if q is not None:
         ldq = _rows(q, "q", dev, n, dtype, hd)
         heads = q.shape[1]
@@ -194,14 +236,14 @@ def kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_cac
         raise ValueError("q_out needs q")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
-    cos_ptr = sin_ptr = None
+    cos_ptr = sin_ptr = 0
     positions = 0
     if cos is not None:
         positions = cos.shape[0] if cos.dim() else 0
         cos_ptr, sin_ptr = _table(cos, "cos", dev, positions, hd // 2), _table(sin, "sin", dev, positions, hd // 2)
-    a = N.KvAppendArgs(q_ptr, k.data_ptr(), v.data_ptr(), qo_ptr, ldq, ldk, ldv, ldqo, cos_ptr, sin_ptr, positions,
-                       _vector(seq, "seq", dev, n), _vector(pos, "pos", dev, n), n, heads)
-    rc = _call(dev, N.load().draco_kv_append, c, a, dt)
+    a = _KV_APPEND.pack(q_ptr, k.data_ptr(), v.data_ptr(), qo_ptr, ldq, ldk, ldv, ldqo, cos_ptr, sin_ptr, positions,
+                        _vector(seq, "seq", dev, n), _vector(pos, "pos", dev, n), n, heads)
+    rc = _call(dev, _lib().kv_append, c, a, dt)
     if rc:
         N.check(rc, "kv_append")
     return q_out
@@ -212,15 +254,15 @@ def kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Ten
     """The keys and values at position pos[i] of sequence seq[i] (int32 [n]), as
     [n, kv_heads, head_dim] float32 (exact) or bfloat16 (rounded once); rows
     outside the cache are zeros."""
-    c = _cache_struct(k_cache, v_cache, block_table, head_dim)
-    dev, n, kv_heads = k_cache.get_device(), seq.shape[0] if seq.dim() else 0, c.kv_heads
+    c, kv_heads, _, _ = _cache_struct(k_cache, v_cache, block_table, head_dim)
+    dev, n = k_cache.get_device(), seq.shape[0] if seq.dim() else 0
     if dtype not in _DTYPES:
         raise ValueError(f"kv_read gives float32 or bfloat16, not {dtype}")
     s, p = _vector(seq, "seq", dev, n), _vector(pos, "pos", dev, n)
     k = k_cache.new_empty((n, kv_heads, head_dim), dtype=dtype)
     v = torch.empty_like(k)
     ld = kv_heads * head_dim
-    rc = _call(dev, N.load().draco_kv_read, c, s, p, n, k.data_ptr(), v.data_ptr(), ld, ld, _DTYPES[dtype])
+    rc = _call(dev, _lib().kv_read, c, s, p, n, k.data_ptr(), v.data_ptr(), ld, ld, _DTYPES[dtype])
     if rc:
         N.check(rc, "kv_read")
     return k, v
@@ -263,7 +305,7 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if len(shape) != 3:
         raise DracoFormatError(f"q must be [tokens, heads, head_dim], not {tuple(shape)}")
     n, heads, hd = shape
-    c = _cache_struct(k_cache, v_cache, block_table, hd)
+    c, _, seqs, held = _cache_struct(k_cache, v_cache, block_table, hd)
     dev, dtype, dt = k_cache.get_device(), q.dtype, _dtype(q, "q")
     ldq = _rows(q, "q", dev, n, dtype, hd)
     if out is None:
@@ -274,35 +316,32 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         ldo = _rows(out, "out", dev, n, dtype, hd)
     if scale is not None and not 1e-30 < scale <= 65536.0:
         raise ValueError(f"scale {scale} must be positive and at most 65536")
-    held = c.max_pages * c.page_size
-    max_q = n if max_q is None or max_q > n else int(max_q)
-    max_kv = held if max_kv is None or max_kv > held else int(max_kv)
-    a = N.AttentionPagedArgs(q.data_ptr(), out.data_ptr(), ldq, ldo, _vector(q_start, "q_start", dev, c.n_seqs + 1),
-                             _vector(kv_len, "kv_len", dev, c.n_seqs), n, heads, max_q, max_kv,
-                             0.0 if scale is None else scale, None, 0)
-    lib = N.load()
+    max_q = n if max_q is None or max_q > n else max(int(max_q), -1)
+    max_kv = held if max_kv is None or max_kv > held else max(int(max_kv), -1)
+    lib = _lib()
+    start_ptr, len_ptr = _vector(q_start, "q_start", dev, seqs + 1), _vector(kv_len, "kv_len", dev, seqs)
+
+    def run(ws: Optional[torch.Tensor]) -> int:
+        ptr, nbytes = (0, 0) if ws is None else (ws.data_ptr(), ws.numel() * ws.element_size())
+        a = _ATTENTION.pack(q.data_ptr(), out.data_ptr(), ldq, ldo, start_ptr, len_ptr, n, heads, max_q, max_kv,
+                            0.0 if scale is None else scale, ptr, nbytes)
+        return _call(dev, lib.attention_paged, c, a, dt)
+
     if workspace is not None:
         if workspace.get_device() != dev or not workspace.is_contiguous():
             raise ValueError(f"workspace must be a contiguous tensor on cuda:{dev}")
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        rc = _call(dev, lib.draco_attention_paged, c, a, dt)
+        rc = run(workspace)
     elif torch.cuda.is_current_stream_capturing():
-        need = lib.draco_attention_paged_workspace_bytes(c, n, heads, max_q, max_kv, dt)
-        ws = _new_workspace(k_cache, max(need, N.PAGED_WORKSPACE_HEAD))
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        rc = _call(dev, lib.draco_attention_paged, c, a, dt)
+        need = lib.workspace_bytes(c, n, heads, max_q, max_kv, dt)
+        rc = run(_new_workspace(k_cache, max(need, N.PAGED_WORKSPACE_HEAD)))
     else:
         key = (dev, _current_stream(dev))
-        ws = _workspaces.get(key)
-        if ws is not None:
-            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.size(0)
-        rc = _call(dev, lib.draco_attention_paged, c, a, dt)
+        rc = run(_workspaces.get(key))
         if rc == N.DRACO_ERR_WORKSPACE:  # none yet, or too small
-            need = lib.draco_attention_paged_workspace_bytes(c, n, heads, max_q, max_kv, dt)
+            need = lib.workspace_bytes(c, n, heads, max_q, max_kv, dt)
             with _ws_lock, torch.cuda.device(dev):
                 ws = _workspaces[key] = _new_workspace(k_cache, max(need, 1 << 20))
-            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.size(0)
-            rc = _call(dev, lib.draco_attention_paged, c, a, dt)
+            rc = run(ws)
     if rc:
         N.check(rc, "attention_paged")
     return out
@@ -335,8 +374,8 @@ def attention_paged_workspace_nbytes(k_cache: torch.Tensor, v_cache: torch.Tenso
                                      n: int, heads: int, head_dim: int, max_q: int, max_kv: int,
                                      dtype: torch.dtype) -> int:
     """Bytes of the workspace of an attention_paged call of n tokens."""
-    c = _cache_struct(k_cache, v_cache, block_table, head_dim)
-    need = N.load().draco_attention_paged_workspace_bytes(c, n, heads, max_q, max_kv, _DTYPES[dtype])
+    c, _, _, held = _cache_struct(k_cache, v_cache, block_table, head_dim)
+    need = _lib().workspace_bytes(c, n, heads, max(min(max_q, n), -1), max(min(max_kv, held), -1), _DTYPES[dtype])
     if need == 0:
         raise DracoFormatError(N.last_error() or "attention_paged: unsupported arguments")
     return int(need)
@@ -372,7 +411,7 @@ def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafts: torch.T
     seqs = row_start.shape[0] - 1 if row_start.dim() == 1 else -1
     if seqs < 0:
         raise DracoFormatError("row_start must be [sequences + 1]")
-    probs_ptr, ld_probs = None, 0
+    probs_ptr, ld_probs = 0, 0
     if draft_probs is not None:
         if draft_probs.dtype is not _F32 or draft_probs.get_device() != dev:
             raise ValueError(f"draft_probs must be a float32 tensor on cuda:{dev}, not {draft_probs.dtype} on "
@@ -383,13 +422,15 @@ def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafts: torch.T
     rows = max(n, 1) if max_rows is None else int(max_rows)
     if rows < 1:
         raise ValueError(f"max_rows {rows} must be at least 1")
+    if not 0.0 <= temperature <= 1e30:
+        raise ValueError(f"temperature {temperature} must lie in 0 .. 1e30")
     accepted = row_start.new_empty(seqs)
     tokens = row_start.new_empty((seqs, rows))
-    v = N.VerifyArgs(logits.data_ptr(), probs_ptr, _vector(row_start, "row_start", dev, seqs + 1),
+    v = _VERIFY.pack(logits.data_ptr(), probs_ptr, _vector(row_start, "row_start", dev, seqs + 1),
                      _vector(drafts, "drafts", dev, n), _vector(accept_u, "accept_u", dev, n, _F32),
                      _vector(sample_u, "sample_u", dev, seqs, _F32), accepted.data_ptr(), tokens.data_ptr(),
                      stride[0], ld_probs, rows, temperature, dt, n, seqs, vocab, rows)
-    rc = _call(dev, N.load().draco_verify_drafts, v)
+    rc = _call(dev, _lib().verify_drafts, v)
     if rc:
         N.check(rc, "verify_drafts")
     return accepted, tokens

@@ -4,6 +4,7 @@ sizes of caches, and the host logic of GPUExecutionBackend's paged cache and of
 its n-gram drafts."""
 
 import ctypes
+import re
 from pathlib import Path
 
 import pytest
@@ -118,6 +119,20 @@ def test_calls_of_nothing_succeed():
     assert verify(n_seqs=0) == N.DRACO_OK
     assert lib.draco_kv_append(None, N.KvAppendArgs(), 0, None) == ARG
     assert lib.draco_verify_drafts(None, None) == ARG
+
+
+def test_packed_structures_are_laid_out_as_the_c_ones():
+    def ctype(code):
+        return {"i": ctypes.c_int, "q": ctypes.c_int64, "P": ctypes.c_void_p, "f": ctypes.c_float}[code]
+
+    for packed, mirror in ((P._KV_CACHE, N.KvCache), (P._KV_APPEND, N.KvAppendArgs), (P._ATTENTION, N.AttentionPagedArgs),
+                           (P._VERIFY, N.VerifyArgs)):
+        codes = re.sub(r"(\d+)(\w)", lambda m: m[2] * int(m[1]), packed.format.lstrip("@"))
+        types = [t for _, t in mirror._fields_]
+        assert [ctype(c) if t is not ctypes.c_size_t else t for c, t in zip(codes, types, strict=True)] == types
+        assert packed.size == ctypes.sizeof(mirror)  # (with the same order and sizes: the same native alignment)
+        values = [0.5 if t is ctypes.c_float else 16 * i + 16 for i, t in enumerate(types)]
+        assert packed.pack(*values) == bytes(mirror(*values))
 
 
 def test_cache_sizes():
