@@ -47,11 +47,11 @@
 //
 // Measured, 32 query heads over 8 of 128 unless said otherwise: 40 decode steps
 // over 500-8000 bf16 positions 136 us (6.0 TB/s); 48 over 900-8000 Q8_0
-// positions 115 us (4.2 TB/s: about 380 instructions for a block of 16 keys, and
-// two stages of loads for a warp); nine sequences of 4-7 drafts, fp32 over up to
-// 6000 Q8_0 positions 59 us (840 instructions a block: two terms of everything);
-// one fp32 step of 32 heads over 1024 bf16 positions 11.6 us, most of it the
-// chain lengths -> page -> keys and the splits' merge.
+// positions 104 us (4.6 TB/s: about 380 instructions for a block of 16 keys, issued
+// at 59 % of the rate by four CTAs an SM); nine sequences of 4-7 drafts, fp32 over
+// up to 6000 Q8_0 positions 56 us (840 instructions a block: two terms of
+// everything); one fp32 step of 32 heads over 1024 bf16 positions 11.0 us, most of
+// it the chain lengths -> page -> keys and the splits' merge.
 #include <algorithm>
 #include <cstdio>
 
