@@ -18,11 +18,11 @@
 // differences of one in 10^5 or less.
 //
 // Measured: 48 sequences of 2-8 rows of 128000 fp32 logits with the drafter's
-// probabilities 79 us (1.9 TB/s); for a sequence of five rows 15 us of it read
-// the logits, 22 are the two passes of fp64 weights over the row drawn from (the
+// probabilities 73 us (2.1 TB/s); for a sequence of five rows 15 us of it read
+// the logits, 17 are the two passes of fp64 weights over the row drawn from (the
 // sum of p, then of max(p - q, 0)), 5 find the token, 13 go to barriers and
 // decisions; longer sequences take the rest.  One sequence of five rows of 32000
-// 12.4 us.
+// 11.6 us.
 #include <cooperative_groups.h>
 
 #include <cstdio>
@@ -77,12 +77,15 @@ __device__ __forceinline__ RowStat join(RowStat a, RowStat b, float c) {
   return r;
 }
 template <typename T>
-__device__ __forceinline__ float logit(const T* p) {
-  float x;
+__device__ __forceinline__ float value(const T* p) {
   if constexpr (sizeof(T) == 4)
-    x = *p;
+    return *p;
   else
-    x = __bfloat162float(*p);
+    return __bfloat162float(*p);
+}
+template <typename T>
+__device__ __forceinline__ float logit(const T* p) {
+  const float x = value(p);
   return x == x ? x : -INFINITY;  // a NaN logit is never drawn
 }
 
@@ -101,6 +104,7 @@ __device__ __forceinline__ double wide(float x) {
 // the fp64 instructions of exp(), which bound the drawing.
 constexpr float kTangScale = 369.32993f;  // 256 / ln2
 constexpr int kTable = 256;
+// The rounding of m / T is a factor of all weights, and goes with their sum.
 struct Weight64 {
   float m, scale;   // the row's maximum, 256 / (T ln2)
   double inv_t, m_t;  // 1 / T, m / T
@@ -117,8 +121,7 @@ struct Weight64 {
     p = fma(p, r, 1.0);
     p *= table[k & (kTable - 1)];
     const double v = __hiloint2double(__double2hiint(p) + ((k >> 8) << 20), __double2loint(p));
-    // below 2^-1000 (and for -infinity) nothing; the maximum itself may be infinite
-    return x == m ? 1.0 : t > -256000.f ? v : 0.0;
+    return t > -256000.f ? v : 0.0;  // below 2^-1000, for -infinity and for NaN nothing
   }
 };
 
@@ -365,15 +368,32 @@ __global__ void __launch_bounds__(kVfThreads, 3) verify_kernel(const VerifyArgs 
       double inv_z = 1.0;
       auto weights = [&](int i0, bool of_p) {  // of p, or of what may still be drawn
         float v[K], u[K];
+        const bool whole = i0 - lane + 32 * K <= w1;
+        if (whole) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) v[k] = i0 + 32 * k < w1 ? logit(row + i0 + 32 * k) : -INFINITY;
+          for (int k = 0; k < K; ++k) v[k] = value(row + i0 + 32 * k);
+        } else {
+#pragma unroll
+          for (int k = 0; k < K; ++k) v[k] = i0 + 32 * k < w1 ? value(row + i0 + 32 * k) : -INFINITY;
+        }
         if (!of_p && q != nullptr) {
+          if (whole) {
 #pragma unroll
-          for (int k = 0; k < K; ++k) u[k] = i0 + 32 * k < w1 ? __ldg(q + i0 + 32 * k) : 0.f;
+            for (int k = 0; k < K; ++k) u[k] = __ldg(q + i0 + 32 * k);
+          } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k) u[k] = i0 + 32 * k < w1 ? __ldg(q + i0 + 32 * k) : 0.f;
+          }
+        }
+        if (fabs(weight.m_t) < 1e9) {
+#pragma unroll
+          for (int k = 0; k < K; ++k) w[k] = weight(v[k]);
+        } else {  // the rounding of m / T is no small one: the maximum's weight is one (infinite logits share it)
+#pragma unroll
+          for (int k = 0; k < K; ++k) w[k] = v[k] == at.m ? 1.0 : weight(v[k]);
         }
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-          w[k] = weight(v[k]);
           if (!of_p) {
             if (q != nullptr) {
               const double d = fma(w[k], inv_z, -wide(u[k]));

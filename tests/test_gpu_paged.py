@@ -676,6 +676,25 @@ def test_verify_of_more_rows_than_are_held_at_a_time_and_strided_logits():
     assert count.tolist() == [149] and short.tolist() == [want[1][0][:10]]
 
 
+@pytest.mark.parametrize("temperature", [1e-29, 1e-18, 1e-9, 1e-3, 1e29])
+@pytest.mark.parametrize("offset", [0.0, 37.0, -3e4, 1e30])
+def test_verify_at_extreme_temperatures_and_logits(temperature, offset):
+    """Nearly greedy and nearly uniform, with logits far from zero: the two
+    largest are equal, and share the weight when the others have none."""
+    n, vocab = 64, 1000
+    g = gen(35)
+    logits = randn(n, vocab, g=g) + offset
+    top = logits.amax(-1, keepdim=True) + 1.0
+    logits.scatter_(1, torch.tensor([[300, 700]], device=DEV).expand(n, 2), top.expand(n, 2))
+    u = (torch.arange(n, device=DEV) + 0.5) / n
+    starts = torch.arange(n + 1, dtype=torch.int32, device=DEV)
+    _, t = P.verify_drafts(logits, starts, i32([0] * n), torch.zeros(n, device=DEV), u, temperature=temperature,
+                           max_rows=1)
+    _, want, margin = R.verify(logits.cpu(), starts.cpu(), torch.zeros(n, dtype=torch.int32), torch.zeros(n), u.cpu(),
+                               None, float(torch.tensor(temperature, dtype=torch.float32)), 1)
+    assert margin > 1e-9 and t.tolist() == want
+
+
 def test_verify_of_no_rows_at_all():
     for t in (0.0, 1.0):
         count, tokens = P.verify_drafts(torch.zeros((0, 50), device=DEV), i32([0, 0, 0]), i32([]),
