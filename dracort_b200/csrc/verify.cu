@@ -18,7 +18,7 @@
 // differences of one in 10^5 or less.
 //
 // Measured: 48 sequences of 2-8 rows of 128000 fp32 logits with the drafter's
-// probabilities 73 us (2.1 TB/s); for a sequence of five rows 15 us of it read
+// probabilities 72 us (2.1 TB/s); for a sequence of five rows 15 us of it read
 // the logits, 17 are the two passes of fp64 weights over the row drawn from (the
 // sum of p, then of max(p - q, 0)), 5 find the token, 13 go to barriers and
 // decisions; longer sequences take the rest.  One sequence of five rows of 32000
