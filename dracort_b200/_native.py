@@ -79,6 +79,7 @@ EXPORTED_SYMBOLS = (
     "draco_attention_paged",
     "draco_attention_paged_workspace_bytes",
     "draco_verify_drafts",
+    "draco_verify_drafts_at",
 )
 
 DTYPE_F32 = 0
@@ -341,6 +342,8 @@ def load() -> ctypes.CDLL:
         lib.draco_attention_paged_workspace_bytes.argtypes = [ctypes.POINTER(KvCache)] + [c_int] * 5
         lib.draco_verify_drafts.restype = c_int
         lib.draco_verify_drafts.argtypes = [ctypes.POINTER(VerifyArgs), vp]
+        lib.draco_verify_drafts_at.restype = c_int
+        lib.draco_verify_drafts_at.argtypes = [ctypes.POINTER(VerifyArgs), ctypes.c_double, vp]
         lib.draco_gguf_gemv.restype = c_int
         lib.draco_gguf_gemv.argtypes = [c_int, vp, vp, vp, vp, c_int, i64, i64, vp, ctypes.c_size_t, vp]
         _lib = lib

@@ -614,6 +614,11 @@ size_t draco_attention_paged_workspace_bytes(const draco_kv_cache* cache, int n,
 }
 
 int draco_verify_drafts(const draco_verify_args* args, void* stream) {
+  if (!args) return fail(DRACO_ERR_ARG, "verify_drafts: null arguments");
+  return draco_verify_drafts_at(args, (double)args->temperature, stream);
+}
+
+int draco_verify_drafts_at(const draco_verify_args* args, double temperature, void* stream) {
   const char* fn = "verify_drafts";
   if (!args) return fail(DRACO_ERR_ARG, "%s: null arguments", fn);
   const draco_verify_args& a = *args;
@@ -622,11 +627,11 @@ int draco_verify_drafts(const draco_verify_args* args, void* stream) {
   if (a.n < 0 || a.n_seqs < 0 || a.vocab < 1 || a.max_rows < 1 || a.n_seqs > (1 << 24) || a.vocab > (1 << 30))
     return fail(DRACO_ERR_SHAPE, "%s: %d rows of %d, %d sequences of at most %d rows", fn, a.n, a.vocab, a.n_seqs,
                 a.max_rows);
-  if (!(a.temperature >= 0.f) || a.temperature > 1e30f || (a.temperature > 0.f && a.temperature < 1e-30f))
-    return fail(DRACO_ERR_ARG, "%s: temperature %g", fn, (double)a.temperature);
+  if (!(temperature >= 0.0) || temperature > (double)1e30f || (temperature > 0.0 && temperature < 1e-30))
+    return fail(DRACO_ERR_ARG, "%s: temperature %g", fn, temperature);
   if (a.n_seqs == 0) return ok();
   if (!a.row_start || !a.accepted || !a.tokens || (a.n > 0 && (!a.logits || !a.drafts)) ||
-      (a.temperature > 0.f && ((a.n > 0 && !a.accept_u) || !a.sample_u)))
+      (temperature > 0.0 && ((a.n > 0 && !a.accept_u) || !a.sample_u)))
     return fail(DRACO_ERR_ARG, "%s: null pointer", fn);
   if (a.ld_logits < 0 || a.ld_tokens < a.max_rows || (a.draft_probs && a.ld_probs < 0))
     return fail(DRACO_ERR_SHAPE, "%s: a negative row stride, or rows of tokens that overlap", fn);
@@ -638,6 +643,6 @@ int draco_verify_drafts(const draco_verify_args* args, void* stream) {
         reinterpret_cast<uintptr_t>(a.tokens)) & 3))
     return fail(DRACO_ERR_ALIGN, "%s: pointers must be aligned to their elements", fn);
   char msg[200] = {0};
-  rc = verify_launch(a, (cudaStream_t)stream, msg, sizeof(msg));
+  rc = verify_launch(a, temperature, (cudaStream_t)stream, msg, sizeof(msg));
   return rc ? fail(rc, "%s", msg) : ok();
 }

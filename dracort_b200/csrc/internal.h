@@ -73,7 +73,7 @@ cudaError_t launch_kv_read(const PagedView& c, int hd, int dtype, const int* seq
 int paged_attn_launch(PagedAttnArgs a, int hd, int dtype, int max_q, int max_kv, void* ws, size_t ws_bytes,
                       cudaStream_t st, char* msg, size_t ml);
 size_t paged_attn_workspace_bytes(const PagedView& c, int n, int group, int hd, int dtype, int max_q, int max_kv);
-int verify_launch(const draco_verify_args& v, cudaStream_t st, char* msg, size_t ml);
+int verify_launch(const draco_verify_args& v, double temperature, cudaStream_t st, char* msg, size_t ml);
 
 // Number of SMs of the current device (cached per device).
 int device_sm_count();

@@ -567,7 +567,7 @@ static cudaError_t launch_verify(const VerifyArgs& a, int n_seqs, bool bf16, cud
   return bf16 ? launch_t<__nv_bfloat16, false>(a, n_seqs, st) : launch_t<float, false>(a, n_seqs, st);
 }
 
-int verify_launch(const draco_verify_args& v, cudaStream_t st, char* msg, size_t ml) {
+int verify_launch(const draco_verify_args& v, double temperature, cudaStream_t st, char* msg, size_t ml) {
   VerifyArgs a;
   a.logits = v.logits;
   a.probs = v.draft_probs;
@@ -580,8 +580,8 @@ int verify_launch(const draco_verify_args& v, cudaStream_t st, char* msg, size_t
   a.ld_logits = v.ld_logits;
   a.ld_probs = v.ld_probs;
   a.ld_tokens = v.ld_tokens;
-  a.greedy = v.temperature == 0.f;
-  a.inv_t = a.greedy ? 1.0 : 1.0 / (double)v.temperature;
+  a.greedy = temperature == 0.0;
+  a.inv_t = a.greedy ? 1.0 : 1.0 / temperature;
   a.inv_t_log2 = (float)(a.inv_t * 1.4426950408889634);
   a.n = v.n;
   a.vocab = v.vocab;

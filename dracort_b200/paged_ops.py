@@ -95,7 +95,7 @@ class _Functions:
         self.attention_paged = fn("draco_attention_paged", vp, vp, ci, vp)
         self.workspace_bytes = fn("draco_attention_paged_workspace_bytes", vp, ci, ci, ci, ci, ci,
                                   restype=ctypes.c_size_t)
-        self.verify_drafts = fn("draco_verify_drafts", vp, vp)
+        self.verify_drafts = fn("draco_verify_drafts_at", vp, ctypes.c_double, vp)
 
 
 _functions: Optional[_Functions] = None
@@ -393,7 +393,8 @@ def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafts: torch.T
     float32; none: each draft was certain), draft x of row r is taken while
     accept_u[r] * q(x) < p(x); at the first that is not, the next token is drawn
     from max(p - q, 0), after the last from p: the first index whose cumulative
-    weight exceeds sample_u[s] times the total.  temperature 0 is greedy.
+    weight exceeds sample_u[s] times the total.  temperature (1e-30 .. 1e30, taken
+    as the 64-bit number it is) 0 is greedy.
     accept_u [n] and sample_u [sequences] are float32 in [0, 1).
 
     Returns accepted (int32 [sequences]) and tokens (int32 [sequences, max_rows]:
@@ -422,15 +423,15 @@ def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafts: torch.T
     rows = max(n, 1) if max_rows is None else int(max_rows)
     if rows < 1:
         raise ValueError(f"max_rows {rows} must be at least 1")
-    if not 0.0 <= temperature <= 1e30:
-        raise ValueError(f"temperature {temperature} must lie in 0 .. 1e30")
+    if not (temperature == 0.0 or 1e-30 <= temperature <= 1e30):
+        raise ValueError(f"temperature {temperature} must be 0 (greedy) or lie in 1e-30 .. 1e30")
     accepted = row_start.new_empty(seqs)
     tokens = row_start.new_empty((seqs, rows))
     v = _VERIFY.pack(logits.data_ptr(), probs_ptr, _vector(row_start, "row_start", dev, seqs + 1),
                      _vector(drafts, "drafts", dev, n), _vector(accept_u, "accept_u", dev, n, _F32),
                      _vector(sample_u, "sample_u", dev, seqs, _F32), accepted.data_ptr(), tokens.data_ptr(),
-                     stride[0], ld_probs, rows, temperature, dt, n, seqs, vocab, rows)
-    rc = _call(dev, _lib().verify_drafts, v)
+                     stride[0], ld_probs, rows, 0.0, dt, n, seqs, vocab, rows)
+    rc = _call(dev, _lib().verify_drafts, v, temperature)
     if rc:
         N.check(rc, "verify_drafts")
     return accepted, tokens

@@ -573,7 +573,8 @@ size_t draco_attention_paged_workspace_bytes(const draco_kv_cache* cache, int n,
  *   draft_probs : fp32 [n, vocab], row stride ld_probs: the drafter's
  *                 probabilities, or NULL: each draft was certain
  *   accept_u    : fp32 [n], sample_u fp32 [n_seqs]: uniform numbers in [0, 1)
- *   temperature : p = softmax(logits / temperature), 1e-30 .. 1e30; 0: greedy
+ *   temperature : p = softmax(logits / temperature), 1e-30 .. 1e30; 0: greedy.
+ *                 fp32; draco_verify_drafts_at takes it in fp64
  * Draft x of row r is taken while accept_u[r] * q(x) < p(x) (greedy: x is the
  * first index of the largest logit); at the first that is not, the next token
  * is drawn from max(p - q, 0) (from p where that is zero everywhere), after the
@@ -604,6 +605,10 @@ typedef struct draco_verify_args {
   int max_rows;
 } draco_verify_args;
 int draco_verify_drafts(const draco_verify_args* args, void* stream);
+/* The same at a temperature of 64 bits; args->temperature is not read.  (Most
+ * decimal temperatures are not fp32 numbers: rounded, they move the cumulative
+ * weights by about 1e-8, and draw another of 10^5 tokens now and then.) */
+int draco_verify_drafts_at(const draco_verify_args* args, double temperature, void* stream);
 
 /* Single-weight convenience form of draco_gguf_gemv_grouped. */
 int draco_gguf_gemv(int qtype, const void* w_tiled, const float* x, float* y, const float* bias,
