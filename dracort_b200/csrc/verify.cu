@@ -12,10 +12,10 @@
 // sequence, the vocabulary cut into one range per CTA, so that one launch does
 // everything: row maxima and sums meet in distributed shared memory, every CTA
 // walks the same accept decisions, and only the row that is drawn from is read
-// again (from L2).  Sums of exponentials that decide an acceptance are
-// fp32 (their error of about 1e-7 moves a decision as rarely); the cumulative
-// weights of the drawn row are fp64, since an index out of 10^5 hangs on
-// differences of one in 10^5 or less.
+// again (from L2).  Sums of exponentials that decide an acceptance are fp32; a
+// decision whose sides lie within their errors (some 1e-5 of each other) is made
+// from fp64 sums of its row.  The cumulative weights of the drawn row are fp64,
+// since an index out of 10^5 hangs on differences of one in 10^5 or less.
 //
 // Measured: 48 sequences of 2-8 rows of 128000 fp32 logits with the drafter's
 // probabilities 72 us (2.1 TB/s); for a sequence of five rows 15 us of it read
@@ -123,7 +123,32 @@ struct Weight64 {
     const double v = __hiloint2double(__double2hiint(p) + ((k >> 8) << 20), __double2loint(p));
     return t > -256000.f ? v : 0.0;  // below 2^-1000, for -infinity and for NaN nothing
   }
+  // with m / T so large that its rounding is no small one, the maximum's weight is
+  // one (infinite logits share it)
+  __device__ __forceinline__ double any(float x) const {
+    return x == m && !(fabs(m_t) < 1e9) ? 1.0 : (*this)(x);
+  }
 };
+
+// The sum of a row's weights in fp64, by the CTA and the same in each of its
+// threads, and in every CTA: one order.  Out of line: few calls get here, and the
+// kernel's registers are bounded.
+template <typename T>
+__device__ __noinline__ double row_weight(const T* row, int vocab, Weight64 weight, double* scratch) {
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < vocab; i += kVfThreads) {
+    const float x = value(row + i);
+    sum += weight.any(x);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  sum = 0.0;
+  for (int w = 0; w < kVfWarps; ++w) sum += scratch[w];
+  __syncthreads();
+  return sum;
+}
 
 // pairs of fp32 values
 __device__ __forceinline__ uint64_t pair_2(float a, float b) {
@@ -303,10 +328,16 @@ __global__ void __launch_bounds__(kVfThreads, 3) verify_kernel(const VerifyArgs 
       if (lane == 0) full[r] = st;
     }
     __syncthreads();
-    // the accept decisions, a row to a lane
+    // The accept decisions, a row to a lane.  The two sides are compared in fp32's
+    // accuracy first; where they lie closer than its errors, in fp64's.  Errors in
+    // units of 2^-24: a weight is off by 2.1 |a| + 4 (a: its exponent, of three
+    // roundings; exp2: two steps of 2^-23), a row's sum by 2.1 log2(vocab) + 4 for
+    // its weights, 9 for a step's additions, 7 a step for the running sum and its
+    // rescalings, and 6 for each of 21 joins: 208 + 7 steps at most.
+    const float tol = (8.f * (float)(a.vocab / (512 * ctas) + 1) + 272.f) * 0x1p-24f;
     for (int rb = 0; rb < nr && !decided; rb += 32) {
       const int r = rb + lane;
-      bool take = false;
+      bool take = false, close = false;
       if (r < nr && r0 + r < rows - 1) {
         const int rr = begin + r0 + r, x = a.drafts[rr];
         const RowStat st = full[r];
@@ -316,13 +347,29 @@ __global__ void __launch_bounds__(kVfThreads, 3) verify_kernel(const VerifyArgs 
           } else {
             const float lx = logit(logits + (int64_t)rr * a.ld_logits + x);
             const float qx = a.probs ? a.probs[(int64_t)rr * a.ld_probs + x] : 1.f;
-            const float wx = lx == -INFINITY ? 0.f : lx == st.m ? 1.f : exp2f((lx - st.m) * c);
-            take = (double)a.accept_u[rr] * qx * st.s < wx;
+            const float e = lx == st.m ? 0.f : (lx - st.m) * c, wx = lx == -INFINITY ? 0.f : exp2f(e);
+            const double ux = (double)a.accept_u[rr] * qx * st.s;
+            take = ux < wx;
+            close = fabs(ux - wx) <= (double)wx * (tol - e * 0x1p-22f) || (wx < 0x1p-120f && ux < 0x1p-119);
           }
         }
       }
-      const unsigned stop = __ballot_sync(0xffffffffu, !take);
-      const int k = stop ? __ffs(stop) - 1 : 32;  // the first row that is not taken (or is the last)
+      unsigned stop = __ballot_sync(0xffffffffu, !take);
+      int k = stop ? __ffs(stop) - 1 : 32;  // the first row that is not taken (or is the last)
+      if constexpr (!kGreedy) {
+        for (unsigned left = __ballot_sync(0xffffffffu, close); left != 0u; left &= left - 1) {
+          const int e = __ffs(left) - 1;
+          if (e > k) break;
+          const int rr = begin + r0 + rb + e, x = a.drafts[rr];
+          const T* row = logits + (int64_t)rr * a.ld_logits;
+          const float m = full[rb + e].m;
+          const Weight64 weight{m, (float)a.inv_t * kTangScale, a.inv_t, (double)m * a.inv_t, table};
+          const double ux = (double)a.accept_u[rr] * (a.probs ? a.probs[(int64_t)rr * a.ld_probs + x] : 1.f);
+          const bool yes = ux * row_weight(row, a.vocab, weight, &bsum[0][0]) < weight.any(logit(row + x));
+          stop = yes ? stop & ~(1u << e) : stop | 1u << e;
+          k = stop ? __ffs(stop) - 1 : 32;
+        }
+      }
       const int n = min(k, nr - rb);
       count += n;
       if (n < nr - rb && n < 32) {
@@ -388,9 +435,9 @@ __global__ void __launch_bounds__(kVfThreads, 3) verify_kernel(const VerifyArgs 
         if (fabs(weight.m_t) < 1e9) {
 #pragma unroll
           for (int k = 0; k < K; ++k) w[k] = weight(v[k]);
-        } else {  // the rounding of m / T is no small one: the maximum's weight is one (infinite logits share it)
+        } else {
 #pragma unroll
-          for (int k = 0; k < K; ++k) w[k] = v[k] == at.m ? 1.0 : weight(v[k]);
+          for (int k = 0; k < K; ++k) w[k] = weight.any(v[k]);
         }
 #pragma unroll
         for (int k = 0; k < K; ++k) {

@@ -93,3 +93,88 @@ def test_temperatures_below_the_limit_are_refused():
             P.verify_drafts(x, i32([0, 1]), i32([0]), x[0, :1], x[0, :1], temperature=t)
     for t in (0.0, 1e-30, 1e30):
         P.verify_drafts(x, i32([0, 1]), i32([0]), x[0, :1], x[0, :1], temperature=t)
+
+
+def neighbours(p):
+    """The largest fp32 number below p (float64) and the smallest that is not."""
+    f = p.float()
+    lo = torch.where(f.double() < p, f, torch.nextafter(f, torch.zeros_like(f)))
+    return lo, torch.nextafter(lo, torch.ones_like(lo))
+
+
+def clear(p, lo, hi):
+    """Both neighbours are further from p than fp64 sums of 10^5 weights are off (1e-12 of it)."""
+    return ((p - lo.double()) > 1e-11 * p) & ((hi.double() - p) > 1e-11 * p)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [7, 3001, 128000])
+@pytest.mark.parametrize("temperature", [0.7, 1.0])
+def test_certain_drafts_are_decided_by_the_numbers_next_to_their_probability(temperature, vocab, dtype):
+    g = gen(vocab)
+    x = peaked(vocab, g).to(dtype)
+    p = softmax64(x, temperature)
+    lo, hi = neighbours(p)
+    some = (clear(p, lo, hi) & (hi < 1)).nonzero()[:, 0]
+    some = some[p[some].argsort(descending=True)][:400]  # the likely ones
+    some = torch.cat([some, (p > 0).nonzero()[:1, 0]])
+    n = len(some)
+    starts = torch.arange(0, 2 * n + 1, 2, dtype=torch.int32, device=DEV)
+    drafts = some.to(torch.int32).repeat_interleave(2)
+    half = torch.full((n,), 0.5, device=DEV)
+    for u, want in ((lo, 1), (hi, 0)):
+        count, tokens = P.verify_drafts(x.expand(2 * n, -1), starts, drafts, u[some].repeat_interleave(2), half,
+                                        temperature=temperature, max_rows=2)
+        assert torch.equal(count[:-1], torch.full_like(count[:-1], want))
+        assert bool(((tokens[:-1, 0].long() == some[:-1]) == bool(want)).all())
+
+
+@pytest.mark.parametrize("temperature", [0.7, 1.0])
+def test_drafts_with_probabilities_are_decided_by_the_numbers_next_to_the_border(temperature):
+    g = gen(5)
+    vocab, n = 32000, 300
+    x = peaked(vocab, g)
+    p = softmax64(x, temperature)
+    some = p.argsort(descending=True)[:n]
+    q = torch.zeros(n, vocab, device=DEV)
+    q[torch.arange(n, device=DEV), some] = (p[some] * (1 + torch.rand(n, generator=g, device=DEV, dtype=torch.float64))).float()
+    qx = q[torch.arange(n, device=DEV), some].double()
+    lo, hi = neighbours(p[some] / qx)  # u q < p
+    sure = clear(p[some] / qx, lo, hi)
+    assert int(sure.sum()) > n * 0.9
+    starts = torch.arange(0, 2 * n + 1, 2, dtype=torch.int32, device=DEV)
+    for u, want in ((lo, 1), (hi, 0)):
+        count, _ = P.verify_drafts(x.expand(2 * n, -1), starts, some.to(torch.int32).repeat_interleave(2),
+                                   u.repeat_interleave(2), torch.full((n,), 0.5, device=DEV),
+                                   draft_probs=q.repeat_interleave(2, 0), temperature=temperature, max_rows=2)
+        assert bool((count[sure] == want).all())
+
+
+@pytest.mark.parametrize("stop", [0, 31, 32, 40, 63, 64, 97, 99])
+def test_a_chain_of_close_decisions_ends_at_the_first_that_is_not_taken(stop):
+    """100 rows: every draft's number is the one just below its probability, but that of row `stop` (99: the last)."""
+    g = gen(stop)
+    vocab, rows = 5000, 100
+    x = torch.randn(rows, vocab, generator=g, device=DEV) * 3
+    p = torch.softmax(x.double(), -1)
+    drafts = x.argmax(-1)
+    px = p.gather(1, drafts[:, None])[:, 0]
+    lo, hi = neighbours(px)
+    sure = clear(px, lo, hi)
+    u = torch.where(sure, lo, lo * 0.9)  # (a number that fp64 cannot tell apart moves away)
+    u[stop] = torch.where(sure[stop], hi[stop], hi[stop] * 1.1)
+    count, tokens = P.verify_drafts(x, i32([0, rows]), drafts.to(torch.int32), u, torch.full((1,), 0.5, device=DEV),
+                                    max_rows=rows)
+    assert count.tolist() == [min(stop, rows - 1)]
+    assert torch.equal(tokens[0, :stop].long(), drafts[:stop]) and bool((tokens[0, stop + 1:] == -1).all())
+
+
+def test_drafts_of_no_weight_and_numbers_of_zero():
+    """u = 0 takes every draft of positive probability, and none of probability zero."""
+    x = torch.zeros(6, 50, device=DEV)
+    x[:, 3] = -200.0  # 1e-87 of the weight: zero in fp32
+    x[:, 4] = -float("inf")
+    x[:, 5] = float("nan")
+    starts, u = i32([0, 2, 4, 6]), torch.zeros(6, device=DEV)
+    count, _ = P.verify_drafts(x, starts, i32([3, 0, 4, 0, 5, 0]), u, u[:3], max_rows=2)
+    assert count.tolist() == [1, 0, 0]
