@@ -250,10 +250,10 @@ __global__ void __launch_bounds__(kPaThreads, (PaCfg<HD, Q8, F32, NN>::kMinCtas)
   // Keys that the tile's last row sees, and this CTA's share of them.
   const int kend = max(0, min(tile.kv, row_limit(a, tile, tile.row0 + rows - 1)));
   const int ck = a.n_splits > 1 ? split_keys<C::kRows>(a, kend, fresh0, kv0) : max(kend, 1);
-  const int active = max(1, (kend + ck - 1) / ck);
+  const int active = split_count(kend, ck);
   const int split = blockIdx.z;  // slowest: CTAs without keys start last
   if (split >= active) return;
-  const int kbeg = split * ck, kfin = min(kend, kbeg + ck);
+  const int kbeg = split * ck, kfin = split_end(kbeg, kend, ck);
 
   // --- the warp's ring: 16-key blocks, warp w takes every W-th (a block lies in one page)
   uint8_t* ring = smem + C::kHead + warp * (C::kStages * C::kStage);

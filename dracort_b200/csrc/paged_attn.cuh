@@ -3,6 +3,7 @@
 #pragma once
 
 #include "paged.cuh"
+#include "paged_split.h"
 
 namespace draco {
 

@@ -270,10 +270,10 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
   const int kend = max(0, min(tile.kv, row_limit(a, tile, tile.row0 + rows - 1)));
   int ck = (kend + a.n_splits - 1) / a.n_splits;
   ck = max(kTcKeys, (ck + kTcKeys - 1) & ~(kTcKeys - 1));
-  const int active = max(1, (kend + ck - 1) / ck);
+  const int active = split_count(kend, ck);
   const int split = blockIdx.x / a.c.kv_heads;
   if (split >= active) return;
-  const int kbeg = split * ck, kfin = min(kend, kbeg + ck);
+  const int kbeg = split * ck, kfin = split_end(kbeg, kend, ck);
   const int nj = __shfl_sync(0xffffffffu, (kfin - kbeg + kTcKeys - 1) / kTcKeys, 0);  // key tiles
   const int ns = __shfl_sync(0xffffffffu, (kfin - kbeg + kTcStep - 1) / kTcStep, 0);  // steps
   // the first tile in which some row is masked (or keys end)
