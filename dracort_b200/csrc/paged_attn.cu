@@ -887,11 +887,10 @@ static PaPlan plan_of(int n, int n_seqs, int group, int kv_heads, int hd, int ma
 }
 
 // New tokens from which a sequence goes to the tensor-memory kernel, or 0: none
-// does.  Its CTA takes 256 rows at a time however few there are.
-constexpr int kTcMinRows = 64;
+// does.
 static int tc_from(const PagedView& c, int n, int hd, int dtype, int group, int max_q, int max_kv) {
   if (!paged_attn_tc_takes(c, hd, dtype, group, 1 << c.page_shift)) return 0;
-  const int from = kTcMinRows / group + 1;
+  const int from = tc_min_tokens(group);
   if (max_q < from) return 0;
   // (its tiles are the grid's y)
   return paged_attn_tc_plan(n, c.n_seqs, group, c.kv_heads, hd, max_kv).tiles <= 65535 ? from : 0;

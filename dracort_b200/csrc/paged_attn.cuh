@@ -86,8 +86,13 @@ __device__ __forceinline__ int row_limit(const PagedAttnArgs& a, const RowTile& 
 }
 
 // the tensor-memory kernel (paged_attn_tc.cu)
+// New tokens from which a sequence goes there: 65 rows.  Its CTA takes 256 rows at
+// a time however few there are.
+constexpr int kTcMinRows = 64;
+inline int tc_min_tokens(int group) { return kTcMinRows / group + 1; }
 struct TcPlan {
   int rt, splits;
+  int by_tokens;  // partial results by record_place (else by tile)
   int64_t tiles, units;
   size_t bytes;  // of partial results
 };

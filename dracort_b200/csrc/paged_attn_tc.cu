@@ -71,6 +71,7 @@ struct __align__(64) TcParams {
   int hd;
   int box_rows;  // rows of a TMA box: min(page_size, 128)
   int page_rows; // rows in the key (or value) buffer: pages * kv_heads * page_size
+  int by_tokens; // partial results by record_place (else by tile)
   int* status;
 };
 
@@ -459,7 +460,8 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
 #pragma unroll 1
     for (int i = 0; i < kTcBadWords; ++i) any_bad |= s_bad[i];
     const int rr = tile.row0 + r;
-    const int64_t unit = (int64_t)tile_id * a.c.kv_heads + kvh;
+    const int64_t place = P.by_tokens ? record_place(tile.start, tile.row0, a.group, 2 * P.rt, a.min_new) : tile_id;
+    const int64_t unit = place * a.c.kv_heads + kvh;
     float* rec = a.recs + (unit * a.n_splits + split) * (int64_t)(2 * P.rt) * (hd + 2);
     __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(a.out) + (int64_t)(tile.start + rr / a.group) * a.ldo +
                           (int64_t)(kvh * a.group + rr % a.group) * hd;
@@ -873,7 +875,12 @@ TcPlan paged_attn_tc_plan(int n, int n_seqs, int group, int kv_heads, int hd, in
   TcPlan p;
   p.rt = group * (kTcRows / group);
   p.tiles = (int64_t)n * group / (2 * p.rt) + n_seqs;
-  p.units = p.tiles * kv_heads;
+  // Partial results take 256 rows of fp32 a place: of many sequences few are long
+  // enough for this kernel (200 steps beside a chunk of 512 tokens, 8 heads of 128:
+  // 115 MB, where a place for every tile would take 1.95 GB).
+  const int64_t by_tokens = record_places(n, group, 2 * p.rt, tc_min_tokens(group));
+  p.by_tokens = by_tokens < p.tiles;
+  p.units = std::min(by_tokens, p.tiles) * kv_heads;
   // One CTA per SM: when the row tiles leave SMs idle, as many splits as fit
   // one wave.  A split's partial rows cost a round trip through the L2, so a
   // second wave of splits never pays.
@@ -927,6 +934,7 @@ int paged_attn_tc_launch(const PagedAttnArgs& a, int hd, const TcPlan& p, int* s
   TcParams P;
   P.a = a;
   P.a.n_splits = p.splits;
+  P.by_tokens = p.by_tokens;
   P.rt = p.rt;
   P.hd = hd;
   P.status = status;

@@ -18,4 +18,14 @@ namespace draco {
 DRACO_BOTH int split_count(int kend, int ck) { return kend > 0 ? 1 + (kend - 1) / ck : 1; }
 DRACO_BOTH int split_end(int kbeg, int kend, int ck) { return kend - kbeg < ck ? kend : kbeg + ck; }
 
+// Places of partial results for the row tiles (R rows each) of the sequences of
+// `from` new tokens or more, among n tokens, `group` rows a token: the tile at row
+// row0 of the sequence that begins at token `start`.  They are distinct without a
+// sum over the sequences: a sequence of m >= from tokens moves the next one's first
+// place on by floor(m group / R) + 1 at least, which its tiles need.
+DRACO_BOTH int64_t record_place(int start, int row0, int group, int R, int from) {
+  return (int64_t)start * group / R + start / from + row0 / R;
+}
+DRACO_BOTH int64_t record_places(int n, int group, int R, int from) { return (int64_t)n * group / R + n / from; }
+
 }  // namespace draco

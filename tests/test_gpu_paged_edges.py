@@ -8,6 +8,7 @@ torch = pytest.importorskip("torch")
 if not torch.cuda.is_available():  # pragma: no cover
     pytest.skip("needs a CUDA GPU", allow_module_level=True)
 
+import test_gpu_paged as T  # noqa: E402
 from dracort_b200 import paged_ops as P  # noqa: E402
 
 DEV = torch.device("cuda", 0)
@@ -33,3 +34,21 @@ def test_the_longest_sequence(tokens, dtype):
                             i32([length]), max_q=tokens, max_kv=length)
     assert P.attention_paged_status() == 0
     assert float((out.double() - want).abs().max()) <= want * 2.0 ** -8
+
+
+@pytest.mark.parametrize("heads,kv", [(8, 8), (8, 2), (6, 1), (40, 2)])
+@pytest.mark.parametrize("cache", ["bf16", "q8_0"])
+def test_chunks_among_many_steps(cache, heads, kv):
+    """Chunks that are split, at several places among 90 sequences of a token or none, some at the least length that
+    the long chunks' kernel takes; run again, the same numbers."""
+    least = 64 // (heads // kv) + 1
+    new = [1, 0, 1, 1] * 22 + [1, 1]
+    new[0], new[30], new[31], new[60], new[89] = least, 290, least, least - 1, 150
+    past = [(s * 131) % 700 for s in range(90)]
+    past[0], past[30], past[31], past[89] = 3000, 2500, 4000, 2000
+    b = T.batch(new, past, heads, kv, 64, 64, cache, BF16, seed=41)
+    out = torch.full_like(b[0], float("nan"))
+    P.attention_paged(*b, max_q=290, max_kv=4000 + least, out=out)
+    T.check(*b, out)
+    for _ in range(3):
+        assert torch.equal(P.attention_paged(*b, max_q=290, max_kv=4000 + least), out)

@@ -2,6 +2,7 @@
 entries refuse, and the arithmetic of splits, record slots and page pools."""
 
 import ctypes
+import random
 import shutil
 import subprocess
 from pathlib import Path
@@ -53,10 +54,16 @@ def split(tmp_path_factory):
     d = tmp_path_factory.mktemp("split")
     (d / "s.cpp").write_text('#include "paged_split.h"\nextern "C" {\n'
                              "int count(int kend, int ck) { return draco::split_count(kend, ck); }\n"
-                             "int end(int kbeg, int kend, int ck) { return draco::split_end(kbeg, kend, ck); }\n}\n")
+                             "int end(int kbeg, int kend, int ck) { return draco::split_end(kbeg, kend, ck); }\n"
+                             "long long place(int start, int row0, int group, int R, int from) {\n"
+                             "  return draco::record_place(start, row0, group, R, from); }\n"
+                             "long long places(int n, int group, int R, int from) {\n"
+                             "  return draco::record_places(n, group, R, from); }\n}\n")
     subprocess.run([gxx, "-O1", "-ftrapv", "-shared", "-fPIC", "-I", str(CSRC), "-o", str(d / "s.so"), str(d / "s.cpp")],
                    check=True)
-    return ctypes.CDLL(str(d / "s.so"))
+    so = ctypes.CDLL(str(d / "s.so"))
+    so.place.restype = so.places.restype = ctypes.c_longlong
+    return so
 
 
 @pytest.mark.parametrize("kend", [1, 63, 64, 65, 9001, 1430000000, 1431655765, 1 << 30, LONGEST - 1, LONGEST])
@@ -72,3 +79,37 @@ def test_splits_cover_every_key_once(split, kend, n):
 
 def test_a_sequence_of_no_keys_has_one_empty_split(split):
     assert split.count(0, 64) == 1 and split.end(0, 0, 64) == 0
+
+
+# ---------------------------------------------------------------------------
+# partial results of long chunks beside many short sequences
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 7, 8, 20, 64, 65, 128])
+def test_long_chunks_have_places_of_their_own(split, group):
+    rng = random.Random(group)
+    rows, frm = 2 * group * (128 // group), 64 // group + 1
+    for _ in range(200):
+        new = [rng.choice([0, 1, 1, frm - 1, frm, frm, frm + 1, rng.randint(1, 3 * rows // group + 1)])
+               for _ in range(rng.randint(1, 60))]
+        n, start, seen = sum(new) + rng.choice([0, 0, 5]), 0, []
+        for m in new:
+            if m >= frm:
+                seen += [split.place(start, r, group, rows, frm) for r in range(0, m * group, rows)]
+            start += m
+        assert len(set(seen)) == len(seen)
+        assert all(0 <= p < split.places(n, group, rows, frm) for p in seen)
+    # the places of any token count stay in range, at the largest ones too
+    n = 0x7FFF0000 // group
+    last = (frm * group - 1) // rows * rows
+    assert split.place(n - frm, last, group, rows, frm) < split.places(n, group, rows, frm)
+
+
+@pytest.mark.parametrize("heads,kv,head_dim", [(8, 8, 128), (32, 8, 128), (32, 32, 64), (6, 1, 96), (64, 1, 128)])
+def test_workspace_of_many_steps_beside_a_chunk(heads, kv, head_dim):
+    """What a batch of steps and one or several chunks takes is bounded by the tokens, not by the sequences."""
+    for steps in (0, 1, 10, 64, 200, 1000):
+        for chunks, size in ((1, 100), (1, 512), (3, 700), (1, 4000)):
+            c = N.KvCache(type=N.KV_BF16, kv_heads=kv, head_dim=head_dim, page_size=64, n_pages=8, n_seqs=steps + chunks,
+                          max_pages=256, table_stride=256, k=PTR, v=PTR, block_table=PTR)
+            need = lib.draco_attention_paged_workspace_bytes(c, steps + chunks * size, heads, size, 8000, N.DTYPE_BF16)
+            assert N.PAGED_WORKSPACE_HEAD <= need < 200 << 20, (steps, chunks, size, need)
