@@ -78,6 +78,7 @@ EXPORTED_SYMBOLS = (
     "draco_kv_read",
     "draco_attention_paged",
     "draco_attention_paged_workspace_bytes",
+    "draco_attention_paged_status",
     "draco_verify_drafts",
     "draco_verify_drafts_at",
 )
@@ -340,6 +341,8 @@ def load() -> ctypes.CDLL:
         lib.draco_attention_paged.argtypes = [ctypes.POINTER(KvCache), ctypes.POINTER(AttentionPagedArgs), c_int, vp]
         lib.draco_attention_paged_workspace_bytes.restype = ctypes.c_size_t
         lib.draco_attention_paged_workspace_bytes.argtypes = [ctypes.POINTER(KvCache)] + [c_int] * 5
+        lib.draco_attention_paged_status.restype = c_int
+        lib.draco_attention_paged_status.argtypes = [c_int, ctypes.POINTER(c_int)]
         lib.draco_verify_drafts.restype = c_int
         lib.draco_verify_drafts.argtypes = [ctypes.POINTER(VerifyArgs), vp]
         lib.draco_verify_drafts_at.restype = c_int

@@ -613,6 +613,12 @@ size_t draco_attention_paged_workspace_bytes(const draco_kv_cache* cache, int n,
   return paged_attn_workspace_bytes(c, n, heads / c.kv_heads, cache->head_dim, dtype, max_q, max_kv);
 }
 
+int draco_attention_paged_status(int replace, int* status) {
+  if (!status) return fail(DRACO_ERR_ARG, "attention_paged_status: null pointer");
+  const cudaError_t e = paged_attn_status(replace, status);
+  return e == cudaSuccess ? ok() : cuda_fail(e, "attention_paged_status");
+}
+
 int draco_verify_drafts(const draco_verify_args* args, void* stream) {
   if (!args) return fail(DRACO_ERR_ARG, "verify_drafts: null arguments");
   return draco_verify_drafts_at(args, (double)args->temperature, stream);

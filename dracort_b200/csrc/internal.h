@@ -72,6 +72,7 @@ cudaError_t launch_kv_read(const PagedView& c, int hd, int dtype, const int* seq
                            void* v_out, int64_t ldk, int64_t ldv, cudaStream_t st);
 int paged_attn_launch(PagedAttnArgs a, int hd, int dtype, int max_q, int max_kv, void* ws, size_t ws_bytes,
                       cudaStream_t st, char* msg, size_t ml);
+cudaError_t paged_attn_status(int replace, int* status);
 size_t paged_attn_workspace_bytes(const PagedView& c, int n, int group, int hd, int dtype, int max_q, int max_kv);
 int verify_launch(const draco_verify_args& v, double temperature, cudaStream_t st, char* msg, size_t ml);
 

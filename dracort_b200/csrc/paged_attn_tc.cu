@@ -239,6 +239,10 @@ __device__ __forceinline__ void regs_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// What a wait that ran out leaves, beside the workspace's word: a workspace may be
+// dropped, or zeroed by the next replay of a graph, before anybody asks.
+__device__ int tc_status;
+
 struct TcBars {
   uint64_t q_full, q_ready;
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], v_clean[2];
@@ -842,6 +846,7 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
   __syncthreads();
   if (s_abort && tid == 0) {
     atomicExch(P.status, DRACO_ERR_TIMEOUT);
+    atomicExch(&tc_status, DRACO_ERR_TIMEOUT);
     if (nj > 0) mbar_wait_bounded(&bars.q_full, 0, kTcWaitNs);
   }
   if (warp == 8) {
@@ -891,6 +896,12 @@ TcPlan paged_attn_tc_plan(int n, int n_seqs, int group, int kv_heads, int hd, in
   if (p.units > kPagedCounters) p.splits = 1;
   p.bytes = p.splits > 1 ? (size_t)p.units * p.splits * (2 * p.rt) * (hd + 2) * sizeof(float) : 0;
   return p;
+}
+
+cudaError_t paged_attn_status(int replace, int* status) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, tc_status, sizeof(int));
+  if (e == cudaSuccess && *status != replace) e = cudaMemcpyToSymbol(tc_status, &replace, sizeof(int));
+  return e;
 }
 
 template <int HDP, bool Q8>

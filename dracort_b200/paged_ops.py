@@ -350,24 +350,31 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 def attention_paged_status(workspace: Optional[torch.Tensor] = None) -> int:
     """Device status of attention_paged: 0, or DRACO_ERR_TIMEOUT after a bounded
     wait inside a kernel ran out (the outputs of that call are then invalid).
-    Waits for the GPU; reads the given workspace, or all that this module keeps
-    on the current device, and makes a workspace that reports an error ready for
-    use again."""
+    Waits for the GPU.  Without a workspace: of all calls on the current device
+    since the last one that asked, those replayed from graphs and those with
+    workspaces of their callers included.  With one: of the calls that used it.
+    A workspace that reports an error, the given one or any that this module
+    keeps, is made ready for use again (a caller's own only when it is given)."""
+    rc = 0
     if workspace is None:
         dev = _current_device()
         with _ws_lock:
             kept = [ws for (d, _), ws in _workspaces.items() if d == dev]
         torch.cuda.synchronize(dev)
+        word = ctypes.c_int()
+        N.check(N.load().draco_attention_paged_status(0, ctypes.byref(word)), "attention_paged_status")
+        rc = word.value
     else:
+        dev = workspace.device
         kept = [workspace]
-        torch.cuda.synchronize(workspace.device)
+        torch.cuda.synchronize(dev)
     for ws in kept:
-        rc = int(ws[N.PAGED_WORKSPACE_STATUS:N.PAGED_WORKSPACE_STATUS + 4].view(torch.int32).item())
-        if rc:
+        found = int(ws[N.PAGED_WORKSPACE_STATUS:N.PAGED_WORKSPACE_STATUS + 4].view(torch.int32).item())
+        if found:
             ws[:N.PAGED_WORKSPACE_HEAD].zero_()
-            torch.cuda.synchronize(ws.device)
-            return rc
-    return 0
+            rc = rc or found
+    torch.cuda.synchronize(dev)
+    return rc
 
 
 def attention_paged_workspace_nbytes(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,

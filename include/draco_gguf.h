@@ -541,7 +541,9 @@ int draco_kv_read(const draco_kv_cache* cache, const int* seq, const int* pos, i
  * use, left ready for the next call on the same stream; two calls that may
  * overlap need two.  The int32 at DRACO_PAGED_WORKSPACE_STATUS is nonzero
  * (DRACO_ERR_TIMEOUT) after a bounded device wait ran out, the outputs of that
- * call then being invalid; zero the head again before reusing it. */
+ * call then being invalid; zero the head again before reusing it.  A word of the
+ * device records it too (draco_attention_paged_status), whatever becomes of the
+ * workspace. */
 #define DRACO_PAGED_WORKSPACE_STATUS 8192
 #define DRACO_PAGED_WORKSPACE_HEAD 8256
 typedef struct draco_attention_paged_args {
@@ -562,6 +564,10 @@ int draco_attention_paged(const draco_kv_cache* cache, const draco_attention_pag
                           void* stream);
 size_t draco_attention_paged_workspace_bytes(const draco_kv_cache* cache, int n, int heads, int max_q, int max_kv,
                                              int dtype);
+/* The current device's status word, and `replace` (0: clear) in its place:
+ * DRACO_ERR_TIMEOUT after a wait of any draco_attention_paged call ran out, one
+ * replayed from a graph included.  Covers what has finished: synchronize first. */
+int draco_attention_paged_status(int replace, int* status);
 
 /* Verification of drafted tokens (speculative sampling; the reference verifies
  * n-gram drafts greedily, draco/runtime/cpu/speculative.py).  Sequence s owns

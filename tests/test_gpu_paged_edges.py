@@ -1,5 +1,7 @@
 """The serving operators over the paged cache at the ends of their ranges."""
 
+import ctypes
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -9,6 +11,7 @@ if not torch.cuda.is_available():  # pragma: no cover
     pytest.skip("needs a CUDA GPU", allow_module_level=True)
 
 import test_gpu_paged as T  # noqa: E402
+from dracort_b200 import _native as N  # noqa: E402
 from dracort_b200 import paged_ops as P  # noqa: E402
 
 DEV = torch.device("cuda", 0)
@@ -52,3 +55,60 @@ def test_chunks_among_many_steps(cache, heads, kv):
     T.check(*b, out)
     for _ in range(3):
         assert torch.equal(P.attention_paged(*b, max_q=290, max_kv=4000 + least), out)
+
+
+def set_status(value):
+    """The device's status word, as a kernel whose wait ran out leaves it."""
+    old = ctypes.c_int(-1)
+    torch.cuda.synchronize()
+    N.check(N.load().draco_attention_paged_status(value, ctypes.byref(old)))
+    return old.value
+
+
+def test_status_outlives_workspaces_and_replays():
+    """An error is reported once, after the workspace of its call was replaced by a larger one, and after replays of
+    a graph whose workspace is zeroed by each."""
+    small = T.batch([1], [300], 8, 2, 64, 64, "bf16", BF16, seed=42)
+    large = T.batch([300], [3000], 8, 2, 64, 64, "bf16", BF16, seed=43)
+    want = P.attention_paged(*large)
+    P.attention_paged_status()
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        P.attention_paged(*small, max_q=1, max_kv=301)
+        key = (0, st.cuda_stream)
+        first = P._workspaces[key]
+        P._workspaces[key] = first[:N.PAGED_WORKSPACE_HEAD].clone()  # (the kept ones begin at 1 MB)
+        assert set_status(N.DRACO_ERR_TIMEOUT) == 0
+        out = P.attention_paged(*large)
+        assert P._workspaces[key].numel() > first.numel()
+    assert P.attention_paged_status() == N.DRACO_ERR_TIMEOUT
+    assert P.attention_paged_status() == 0
+    assert torch.equal(out, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = P.attention_paged(*large)
+    graph.replay()
+    assert set_status(N.DRACO_ERR_TIMEOUT) == 0
+    graph.replay()
+    assert P.attention_paged_status() == N.DRACO_ERR_TIMEOUT
+    assert P.attention_paged_status() == 0
+    assert torch.equal(out, want)
+
+
+def test_every_workspace_with_an_error_is_made_ready_again():
+    b = T.batch([1, 1], [4000, 3000], 8, 2, 128, 64, "q8_0", BF16, seed=44)
+    want = P.attention_paged(*b, max_q=1, max_kv=4001)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for i, st in enumerate(streams):
+        with torch.cuda.stream(st):
+            P.attention_paged(*b, max_q=1, max_kv=4001)
+            ws = P._workspaces[(0, st.cuda_stream)]
+            if i != 1:  # counters that an aborted merge left, and the status
+                ws[:N.PAGED_WORKSPACE_HEAD].view(torch.int32)[:64] = 3
+                ws[N.PAGED_WORKSPACE_STATUS:N.PAGED_WORKSPACE_STATUS + 4].view(torch.int32).fill_(5 + i)
+    assert P.attention_paged_status() in (5, 7)
+    assert P.attention_paged_status() == 0
+    for st in streams:
+        with torch.cuda.stream(st):
+            assert torch.equal(P.attention_paged(*b, max_q=1, max_kv=4001), want)

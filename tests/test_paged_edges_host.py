@@ -113,3 +113,7 @@ def test_workspace_of_many_steps_beside_a_chunk(heads, kv, head_dim):
                           max_pages=256, table_stride=256, k=PTR, v=PTR, block_table=PTR)
             need = lib.draco_attention_paged_workspace_bytes(c, steps + chunks * size, heads, size, 8000, N.DTYPE_BF16)
             assert N.PAGED_WORKSPACE_HEAD <= need < 200 << 20, (steps, chunks, size, need)
+
+
+def test_status_needs_a_place_for_it():
+    assert lib.draco_attention_paged_status(0, None) == N.DRACO_ERR_ARG
