@@ -1,6 +1,7 @@
 """The serving operators over the paged cache at the ends of their ranges."""
 
 import ctypes
+from pathlib import Path
 
 import pytest
 
@@ -12,6 +13,7 @@ if not torch.cuda.is_available():  # pragma: no cover
 
 import test_gpu_paged as T  # noqa: E402
 from dracort_b200 import _native as N  # noqa: E402
+from dracort_b200 import gguf_executor as X  # noqa: E402
 from dracort_b200 import paged_ops as P  # noqa: E402
 
 DEV = torch.device("cuda", 0)
@@ -112,3 +114,28 @@ def test_every_workspace_with_an_error_is_made_ready_again():
     for st in streams:
         with torch.cuda.stream(st):
             assert torch.equal(P.attention_paged(*b, max_q=1, max_kv=4001), want)
+
+
+@pytest.mark.parametrize("others", [1, 2])
+def test_drafted_generation_in_a_full_pool(others, monkeypatch):
+    """Four pages, one or two of them another sequence's, the rest just what the generation takes: drafts (wrong ones,
+    whose pages come back) ask for no page that the tokens do not come to need, so the tokens are those without
+    drafts; one token more than the pool holds is refused, as it is without drafts."""
+    name = str(Path(__file__).resolve().parent / "golden" / "tiny_llama_decode.gguf")
+    page = 2 * 2 * 4 * 16 * 32 * 2  # 2 layers of keys and values, 4 heads of 32, 16 positions of bf16
+    be = X.GPUExecutionBackend(name, 3, "bf16", 4 * page, page_size=16, q6k_order="d_first")
+    prompt, held = [5, 9, 5, 9, 5], 16 * (4 - others)
+    count = held + 1 - len(prompt)  # (the last token is not cached)
+    free = be.generate_speculative(prompt, count, num_drafts=0)
+    s = be.new_sequence()
+    be.forward_step(s, [1] * (16 * others), 0)
+    drafted = []
+    monkeypatch.setattr(X, "ngram_drafts", lambda ids, n, ngram: drafted.append(n) or [
+        (t + 1) % be.config.vocab_size for t in free[len(ids):len(ids) + max(n, 0)]])
+    assert be.generate_speculative(prompt, count, num_drafts=20) == free
+    assert max(drafted) == 20 and drafted[-1] == 0
+    for num_drafts in (0, 20):
+        with pytest.raises(RuntimeError, match="free pages"):
+            be.generate_speculative(prompt, count + 1, num_drafts=num_drafts)
+    be.end_sequence(s)
+    assert sorted(be._free_pages) == [0, 1, 2, 3]
