@@ -178,3 +178,20 @@ def test_drafts_of_no_weight_and_numbers_of_zero():
     starts, u = i32([0, 2, 4, 6]), torch.zeros(6, device=DEV)
     count, _ = P.verify_drafts(x, starts, i32([3, 0, 4, 0, 5, 0]), u, u[:3], max_rows=2)
     assert count.tolist() == [1, 0, 0]
+
+
+@pytest.mark.parametrize("seqs", [20, 21, 22, 23, 37, 38])
+def test_as_many_sequences_as_clusters_of_either_size(seqs):
+    """Around the number of sequences from which they get fewer blocks each: the same tokens as one by one."""
+    g = gen(seqs)
+    vocab = 20011
+    x = torch.stack([peaked(vocab, g) for _ in range(2 * seqs)])
+    q = torch.softmax(x + 0.5 * torch.randn(2 * seqs, vocab, generator=g, device=DEV), -1)
+    d = torch.multinomial(q, 1, generator=g)[:, 0].to(torch.int32)
+    au, su = torch.rand(2 * seqs, generator=g, device=DEV), torch.rand(seqs, generator=g, device=DEV)
+    starts = torch.arange(0, 2 * seqs + 1, 2, dtype=torch.int32, device=DEV)
+    count, tokens = P.verify_drafts(x, starts, d, au, su, draft_probs=q, temperature=0.9, max_rows=2)
+    for s in range(seqs):
+        r = slice(2 * s, 2 * s + 2)
+        c, t = P.verify_drafts(x[r], i32([0, 2]), d[r], au[r], su[s:s + 1], draft_probs=q[r], temperature=0.9, max_rows=2)
+        assert torch.equal(count[s:s + 1], c) and torch.equal(tokens[s:s + 1], t)
