@@ -306,7 +306,12 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise DracoFormatError(f"q must be [tokens, heads, head_dim], not {tuple(shape)}")
     n, heads, hd = shape
     c, _, seqs, held = _cache_struct(k_cache, v_cache, block_table, hd)
-    dev, dtype, dt = k_cache.get_device(), q.dtype, _dtype(q, "q")
+    dev = k_cache.get_device()
+    if _current_device() != dev:  # the plan, the capture and the workspace are those of the tensors' device
+        with torch.cuda.device(dev):
+            return attention_paged(q, k_cache, v_cache, block_table, q_start, kv_len, max_q, max_kv, scale, out,
+                                   workspace)
+    dtype, dt = q.dtype, _dtype(q, "q")
     ldq = _rows(q, "q", dev, n, dtype, hd)
     if out is None:
         out, ldo = _like(q, shape), heads * hd
@@ -325,7 +330,7 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         ptr, nbytes = (0, 0) if ws is None else (ws.data_ptr(), ws.numel() * ws.element_size())
         a = _ATTENTION.pack(q.data_ptr(), out.data_ptr(), ldq, ldo, start_ptr, len_ptr, n, heads, max_q, max_kv,
                             0.0 if scale is None else scale, ptr, nbytes)
-        return _call(dev, lib.attention_paged, c, a, dt)
+        return lib.attention_paged(c, a, dt, _current_stream(dev))
 
     if workspace is not None:
         if workspace.get_device() != dev or not workspace.is_contiguous():
@@ -339,7 +344,7 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         rc = run(_workspaces.get(key))
         if rc == N.DRACO_ERR_WORKSPACE:  # none yet, or too small
             need = lib.workspace_bytes(c, n, heads, max_q, max_kv, dt)
-            with _ws_lock, torch.cuda.device(dev):
+            with _ws_lock:
                 ws = _workspaces[key] = _new_workspace(k_cache, max(need, 1 << 20))
             rc = run(ws)
     if rc:
@@ -382,7 +387,10 @@ def attention_paged_workspace_nbytes(k_cache: torch.Tensor, v_cache: torch.Tenso
                                      dtype: torch.dtype) -> int:
     """Bytes of the workspace of an attention_paged call of n tokens."""
     c, _, _, held = _cache_struct(k_cache, v_cache, block_table, head_dim)
-    need = _lib().workspace_bytes(c, n, heads, max(min(max_q, n), -1), max(min(max_kv, held), -1), _DTYPES[dtype])
+    if dtype not in _DTYPES:
+        raise ValueError(f"dtype must be float32 or bfloat16, not {dtype}")
+    with torch.cuda.device(k_cache.get_device()):
+        need = _lib().workspace_bytes(c, n, heads, max(min(max_q, n), -1), max(min(max_kv, held), -1), _DTYPES[dtype])
     if need == 0:
         raise DracoFormatError(N.last_error() or "attention_paged: unsupported arguments")
     return int(need)

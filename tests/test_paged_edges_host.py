@@ -6,10 +6,13 @@ import random
 import shutil
 import subprocess
 from pathlib import Path
+from types import SimpleNamespace
 
 import pytest
+import torch
 
 from dracort_b200 import _native as N
+from dracort_b200 import paged_ops as P
 
 PTR = 1 << 20  # an aligned address; every call below returns before it would be read
 
@@ -117,3 +120,46 @@ def test_workspace_of_many_steps_beside_a_chunk(heads, kv, head_dim):
 
 def test_status_needs_a_place_for_it():
     assert lib.draco_attention_paged_status(0, None) == N.DRACO_ERR_ARG
+
+
+# ---------------------------------------------------------------------------
+# tensors on another device than the current one (fakes: one device is enough)
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("capturing", [None, 0, 1])
+def test_attention_on_another_device_than_the_current_one(capturing, monkeypatch):
+    """Device 0 is current, the tensors are on device 1: the capture that counts is device 1's, sizes are asked, the
+    workspace is made and the call is enqueued with device 1 current."""
+    current, seen = [0], []
+
+    class Device:
+        def __init__(self, d):
+            self.d = d
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.d
+
+        def __exit__(self, *e):
+            current[0] = self.before
+
+    class Lib:
+        def attention_paged(self, *args):
+            seen.append(("call", current[0], args[-1]))
+            return N.DRACO_ERR_WORKSPACE if sum(s[0] == "call" for s in seen) == 1 and capturing != 1 else 0
+
+        def workspace_bytes(self, *args):
+            seen.append(("size", current[0]))
+            return 1 << 14
+
+    cache = SimpleNamespace(get_device=lambda: 1, new_empty=lambda n, dtype: (
+        seen.append(("workspace", current[0], n)) or torch.empty(n, dtype=dtype)))
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[0] == capturing)
+    for name, fake in (("_current_device", lambda: current[0]), ("_current_stream", lambda d: 100 + d),
+                       ("_cache_struct", lambda *a: (b"", 2, 1, 64)), ("_rows", lambda *a: 64),
+                       ("_vector", lambda *a: 0), ("_lib", Lib), ("_workspaces", {})):
+        monkeypatch.setattr(P, name, fake)
+    P.attention_paged(torch.zeros(1, 2, 32), cache, None, None, None, None)
+    assert current == [0] and {s[1] for s in seen} == {1}
+    assert [s for s in seen if s[0] == "call"][-1] == ("call", 1, 101)
+    assert [s[2] for s in seen if s[0] == "workspace"] == [1 << 14 if capturing == 1 else 1 << 20]
+    assert list(P._workspaces) == ([] if capturing == 1 else [(1, 101)])
