@@ -61,7 +61,6 @@
 namespace draco {
 
 constexpr int kPaThreads = 128;
-constexpr float kPaLazy = 8.f;
 constexpr int kPaMinSplit = 128;  // keys of a split at least: 2 blocks of each warp
 constexpr int kPaMaxSplits = 64;  // two a lane of the merging warp
 constexpr float kPaFixed = 250.f;  // keys' worth of time that a CTA's beginning and merge take (12k clocks at 45-60 a key)
@@ -419,6 +418,7 @@ __global__ void __launch_bounds__(kPaThreads, (PaCfg<HD, Q8, F32, NN>::kMinCtas)
   float m[NN][2], l[NN][2];
 #pragma unroll
   for (int n = 0; n < NN; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
+  bool huge = false;
   // dim behind accumulator i, elements 0/1 (h = 0) or 2/3 (h = 1)
   auto dim_of = [&](int i, int h) -> int { return Q8 ? 32 * (i >> 1) + 4 * g + 2 * (i & 1) + h : 16 * i + g + 8 * h; };
 
@@ -539,6 +539,7 @@ __global__ void __launch_bounds__(kPaThreads, (PaCfg<HD, Q8, F32, NN>::kMinCtas)
       grow |= fmaxf(s[n][1], s[n][3]) * sc[n][1] > m[n][1] + kPaLazy;
     }
     if (__any_sync(0xffffffffu, grow)) {
+      huge = false;
 #pragma unroll
       for (int n = 0; n < NN; ++n)
 #pragma unroll
@@ -550,19 +551,31 @@ __global__ void __launch_bounds__(kPaThreads, (PaCfg<HD, Q8, F32, NN>::kMinCtas)
           const float nm = fmaxf(m[n][e], x);
           const float f = nm == -INFINITY ? 1.f : fast_exp2(m[n][e] - nm);
           m[n][e] = nm, l[n][e] *= f;
+          huge |= is_huge(nm);
 #pragma unroll
           for (int i = 0; i < HD / 16; ++i) acc[i][n][e] *= f, acc[i][n][e + 2] *= f;
         }
+      huge = __any_sync(0xffffffffu, huge);
     }
+    if (huge) {
 #pragma unroll
-    for (int n = 0; n < NN; ++n)
+      for (int n = 0; n < NN; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float ref = m[n][e] == -INFINITY ? 0.f : m[n][e] - kShift;
-        s[n][e] = fast_exp2(fmaf(s[n][e], sc[n][e], -ref));
-        s[n][e + 2] = fast_exp2(fmaf(s[n][e + 2], sc[n][e], -ref));
-        l[n][e] += s[n][e] + s[n][e + 2];
-      }
+        for (int e = 0; e < 4; ++e) {
+          s[n][e] = fast_exp2(huge_exponent(s[n][e], sc[n][e & 1], m[n][e & 1]) + kShift);
+          l[n][e & 1] += s[n][e];
+        }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NN; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float ref = m[n][e] == -INFINITY ? 0.f : m[n][e] - kShift;
+          s[n][e] = fast_exp2(fmaf(s[n][e], sc[n][e], -ref));
+          s[n][e + 2] = fast_exp2(fmaf(s[n][e + 2], sc[n][e], -ref));
+          l[n][e] += s[n][e] + s[n][e + 2];
+        }
+    }
     if (edge) {
       // values that are not finite and that some rows of the tile do not see
       bool bad = false;

@@ -85,6 +85,19 @@ __device__ __forceinline__ int row_limit(const PagedAttnArgs& a, const RowTile& 
   return t.kv - t.new_tok + row / a.group + 1;
 }
 
+// Scores past 2^20.  m is the largest c S rounded to fp32, and c S - m in one step
+// is that rounding at the largest key: up to 2 at 2^25, where fp16's P overflows,
+// and up to 128 at 2^31, where any does.  With c S rounded first the largest gives
+// 0, and others at most kPaLazy, but for the rounding of m + kPaLazy: the minimum.
+constexpr float kPaLazy = 8.f;     // log2 units by which scores may outgrow m
+constexpr float kPaHuge = 1048576.f;
+__device__ __forceinline__ bool is_huge(float m) { return fabsf(m) > kPaHuge && m != -INFINITY; }
+__device__ __forceinline__ float huge_exponent(float s, float sc, float m) {
+  float x = __fsub_rn(__fmul_rn(s, sc), m == -INFINITY ? 0.f : m);  // (NaN for infinite scores)
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(kPaLazy));
+  return x;
+}
+
 // the tensor-memory kernel (paged_attn_tc.cu)
 // New tokens from which a sequence goes there: 65 rows.  Its CTA takes 256 rows at
 // a time however few there are.

@@ -384,6 +384,9 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
     }
     constexpr float kShift = Q8 ? 6.f : 0.f;
     float m = -INFINITY, l = 0.f;
+    // the exponents are slope s - ref, and m grows when scores outgrow `most`: what
+    // follows from m, set where m is
+    float ref = 0.f, slope = sc, most = -INFINITY;
     for (int i = 0; i < ns && ok; ++i) {
       if (!(ok = wait_warp(&bars.s_full[w][i & 1], i >> 1))) break;
       tca_after();
@@ -406,11 +409,19 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
         x1 = max_nan(x1, s[e + 2], s[e + 3]);
       }
       const float mx = max_nan(x0, x1, x1) * sc;
-      if (__any_sync(0xffffffffu, !(mx <= m + 8.f))) {
+      if (__any_sync(0xffffffffu, !(mx <= most))) {
         const float n = max_nan(m, mx, mx);
         const float f = n == -INFINITY ? 1.f : tca_exp2(m - n);
         m = n;
         l *= f;
+        // (a row with an infinite score is NaN, as inf - inf)
+        ref = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7FC00000) : m - kShift;
+        slope = sc, most = m + kPaLazy;
+        if (__any_sync(0xffffffffu, is_huge(m))) {  // ... and so on every step from here
+#pragma unroll
+          for (int e = 0; e < kTcStep; ++e) s[e] = huge_exponent(s[e], sc, m);
+          ref = -kShift, slope = 1.f, most = __int_as_float(0x7FC00000);
+        }
         if (i > 0) {  // O of the steps so far, once their products are done
           if (!(ok = wait_warp(&bars.pv_done[w][(i - 1) & 1], (i - 1) >> 1))) break;
           tca_after();
@@ -425,9 +436,7 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
           }
         }
       }
-      // (a row with an infinite score is NaN, as inf - inf)
-      const float ref = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7FC00000) : m - kShift;
-      const uint64_t sc2 = pair2(sc, sc), ref2 = pair2(-ref, -ref);
+      const uint64_t sc2 = pair2(slope, slope), ref2 = pair2(-ref, -ref);
       float l0 = 0.f, l1 = 0.f;
       // P.  A quarter of the exponentials go to the FMA pipe over bf16 pages (four
       // prompts 265 -> 257 us); over Q8_0, whose converters use that pipe, none

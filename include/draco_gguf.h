@@ -533,7 +533,8 @@ int draco_kv_read(const draco_kv_cache* cache, const int* seq, const int* pos, i
  * max_kv are upper bounds of the sequences' new tokens and cached positions.
  * They choose the kernels and size the launch and the workspace: tight ones
  * are faster; tokens of a sequence past max_q may be left out.
- * scale is at most 65536; 0 means 1 / sqrt(head_dim).  m, l and the output are accumulated in
+ * scale is at most 65536; 0 means 1 / sqrt(head_dim); scale |q| is finite up to
+ * 1e30.  m, l and the output are accumulated in
  * fp32; fp32 activations keep fp32 accuracy, bf16 ones round the
  * probabilities to 16 bits.
  * Workspace: at least draco_attention_paged_workspace_bytes() bytes, 16-byte

@@ -139,3 +139,51 @@ def test_drafted_generation_in_a_full_pool(others, monkeypatch):
             be.generate_speculative(prompt, count + 1, num_drafts=num_drafts)
     be.end_sequence(s)
     assert sorted(be._free_pages) == [0, 1, 2, 3]
+
+
+@pytest.mark.parametrize("size", [1e3, 1e7, 1e9, 1e14, 1e20, 1e28])
+@pytest.mark.parametrize("cache", ["bf16", "q8_0"])
+@pytest.mark.parametrize("dtype,new", [(F32, 3), (BF16, 3), (BF16, 40)])
+def test_scores_of_any_size(dtype, new, cache, size):
+    """Scores far past 2^24, whose roundings are whole units: all weight on the largest score where it leads by a
+    thousandth (fp32 sums of 64 products are off by less than 64 2^-24 of their largest).  Its value is then off by
+    the output's rounding, and for bf16 activations by those of P (the sum is of unrounded ones) and of V: 2^-8 + 2^-8
+    over bf16 pages, 2^-8 + 2 2^-11 over Q8_0."""
+    b = T.batch([new], [300], 4, 2, 64, 16, cache, dtype, seed=45)
+    q = (b[0].float() * size).to(dtype)
+    out = P.attention_paged(q, *b[1:], max_q=new, max_kv=300 + new)
+    k, v = (T.R.sequence(T.R.values(c), b[3][0], 300 + new, c.shape[0]).repeat_interleave(2, 0) for c in b[1:3])
+    s = q.double().transpose(0, 1) @ k.transpose(1, 2) / 8
+    s.masked_fill_(torch.ones(new, 300 + new, dtype=torch.bool, device=DEV).triu(301), -float("inf"))
+    top, at = s.topk(2, -1)
+    lead = top[..., 0] - top[..., 1] > 1e-3 * top[..., 0].abs() + 40
+    assert float(lead.double().mean()) > 0.5
+    want = v.gather(1, at[..., :1].expand(-1, -1, 64))
+    got = out.double().transpose(0, 1)
+    assert torch.isfinite(got).all()
+    tol = 2.0 ** -20 if dtype is F32 else (2.0 ** -7 if cache == "bf16" else 2.0 ** -8 + 2.0 ** -10) * (1 + 2.0 ** -8)
+    assert float(((got - want).abs() / want.abs().clamp_min(1e-6))[lead].max()) <= tol
+
+
+@pytest.mark.parametrize("cache", ["bf16", "q8_0"])
+@pytest.mark.parametrize("dtype,new", [(F32, 3), (BF16, 3), (BF16, 40)])
+def test_rows_beside_rows_of_huge_scores(dtype, new, cache):
+    """Rows of ordinary and of huge scores in one tile, tokens that see nothing, a key that is not finite."""
+    b = T.batch([new], [300], 4, 2, 64, 16, cache, dtype, seed=46)
+    q = b[0].clone()
+    q[1::3] *= 1e9
+    out = P.attention_paged(q, *b[1:], max_q=new, max_kv=300 + new)
+    want, bound = T.R.attention(*b[:4], b[4].tolist(), b[5].tolist())
+    rows = torch.arange(new, device=DEV) % 3 != 1
+    assert torch.isfinite(out).all()
+    assert float(((out.double() - want).abs() / bound)[rows].max()) <= 1
+    few = i32([new - 2])  # two tokens see nothing
+    out = P.attention_paged(q, *b[1:5], few, max_q=new, max_kv=300 + new)
+    assert not out[:2].any() and torch.isfinite(out).all()
+    page, off = int(b[3][0, 100 // 16]), 100 % 16
+    if cache == "bf16":
+        b[1][page, 0, off] = float("nan")
+    else:
+        T.R.q8_parts(b[1])[1][page, 0, off] = float("nan")
+    out = P.attention_paged(q, *b[1:], max_q=new, max_kv=300 + new)
+    assert torch.isnan(out[:, :2]).all() and torch.isfinite(out[:, 2:]).all()
