@@ -52,6 +52,7 @@ struct VerifyArgs {
   int64_t ld_logits, ld_probs, ld_tokens;
   double inv_t;
   float inv_t_log2;
+  float tol;  // relative error of a row's fp32 sum, and of a weight but for its exponent's part
   int n, vocab, max_rows, greedy;
 };
 
@@ -329,12 +330,7 @@ __global__ void __launch_bounds__(kVfThreads, 3) verify_kernel(const VerifyArgs 
     }
     __syncthreads();
     // The accept decisions, a row to a lane.  The two sides are compared in fp32's
-    // accuracy first; where they lie closer than its errors, in fp64's.  Errors in
-    // units of 2^-24: a weight is off by 2.1 |a| + 4 (a: its exponent, of three
-    // roundings; exp2: two steps of 2^-23), a row's sum by 2.1 log2(vocab) + 4 for
-    // its weights, 9 for a step's additions, 7 a step for the running sum and its
-    // rescalings, and 6 for each of 21 joins: 208 + 7 steps at most.
-    const float tol = (8.f * (float)(a.vocab / (512 * ctas) + 1) + 272.f) * 0x1p-24f;
+    // accuracy first; where they lie closer than its errors, in fp64's.
     for (int rb = 0; rb < nr && !decided; rb += 32) {
       const int r = rb + lane;
       bool take = false, close = false;
@@ -350,7 +346,7 @@ __global__ void __launch_bounds__(kVfThreads, 3) verify_kernel(const VerifyArgs 
             const float e = lx == st.m ? 0.f : (lx - st.m) * c, wx = lx == -INFINITY ? 0.f : exp2f(e);
             const double ux = (double)a.accept_u[rr] * qx * st.s;
             take = ux < wx;
-            close = fabs(ux - wx) <= (double)wx * (tol - e * 0x1p-22f) || (wx < 0x1p-120f && ux < 0x1p-119);
+            close = fabs(ux - wx) <= (double)(wx * (a.tol - e * 0x1p-22f)) || (wx < 0x1p-120f && ux < 0x1p-119);
           }
         }
       }
@@ -638,6 +634,12 @@ int verify_launch(const draco_verify_args& v, double temperature, cudaStream_t s
   a.greedy = temperature == 0.0;
   a.inv_t = a.greedy ? 1.0 : 1.0 / temperature;
   a.inv_t_log2 = (float)(a.inv_t * 1.4426950408889634);
+  // In units of 2^-24: a weight is off by 2.1 |a| + 4 (a: its exponent, of three
+  // roundings; exp2: two steps of 2^-23), a row's sum by 2.1 log2(vocab) + 4 for its
+  // weights, 9 for a step's additions, 7 a step (512 values of a warp, in clusters
+  // of 8 at least) for the running sum and its rescalings, and 6 for each of 21
+  // joins: 212 + 7 steps at most together.
+  a.tol = (8.f * (float)(v.vocab / (512 * (kVfCtas / 2)) + 1) + 272.f) * 0x1p-24f;
   a.n = v.n;
   a.vocab = v.vocab;
   a.max_rows = v.max_rows;
