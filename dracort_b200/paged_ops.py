@@ -438,6 +438,7 @@ def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafts: torch.T
     rows = max(n, 1) if max_rows is None else int(max_rows)
     if rows < 1:
         raise ValueError(f"max_rows {rows} must be at least 1")
+    temperature = float(temperature)
     if not (temperature == 0.0 or 1e-30 <= temperature <= 1e30):
         raise ValueError(f"temperature {temperature} must be 0 (greedy) or lie in 1e-30 .. 1e30")
     accepted = row_start.new_empty(seqs)

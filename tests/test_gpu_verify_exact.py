@@ -2,6 +2,7 @@
 arithmetic of fewer than 64 bits would get wrong, against the definition in
 64 bits."""
 
+import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -195,3 +196,13 @@ def test_as_many_sequences_as_clusters_of_either_size(seqs):
         r = slice(2 * s, 2 * s + 2)
         c, t = P.verify_drafts(x[r], i32([0, 2]), d[r], au[r], su[s:s + 1], draft_probs=q[r], temperature=0.9, max_rows=2)
         assert torch.equal(count[s:s + 1], c) and torch.equal(tokens[s:s + 1], t)
+
+
+def test_temperatures_of_other_number_types():
+    x = peaked(1000, gen(1)).expand(64, -1)
+    u = torch.linspace(0, 0.99, 64, device=DEV)
+    args = (x, torch.arange(65, dtype=torch.int32, device=DEV), i32([0] * 64), u, u)
+    want = P.verify_drafts(*args, temperature=2.0, max_rows=1)
+    for t in (2, np.float32(2), np.float64(2), torch.tensor(2.0)):
+        got = P.verify_drafts(*args, temperature=t, max_rows=1)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
