@@ -8,8 +8,8 @@
 // and sum l, O rescaled when m grows (by more than 8 in the exponent's log2:
 // up to there the old reference only makes the summands larger).
 //
-// What bounds it: few rows share a key, so bytes, and for Q8_0 the conversion
-// of its quants.  Both products have the keys (and values) as the MMA's A
+// What bounds it: few rows share a key, so bytes; for Q8_0 the conversion of its
+// quants and the latency between its steps.  Both products have the keys (and values) as the MMA's A
 // operand and the rows as its 8-column B operand, S^T = K Q^T and O^T = V^T
 // P^T (m16n8k16): a decode step's rows (the heads of a group) fill 8 columns
 // where they would leave 16 rows half empty, S and O take half the registers,
@@ -47,11 +47,16 @@
 //
 // Measured, 32 query heads over 8 of 128 unless said otherwise: 40 decode steps
 // over 500-8000 bf16 positions 136 us (6.0 TB/s); 48 over 900-8000 Q8_0
-// positions 104 us (4.6 TB/s: about 380 instructions for a block of 16 keys, issued
-// at 59 % of the rate by four CTAs an SM); nine sequences of 4-7 drafts, fp32 over
-// up to 6000 Q8_0 positions 56 us (840 instructions a block: two terms of
-// everything); one fp32 step of 32 heads over 1024 bf16 positions 11.0 us, most of
-// it the chain lengths -> page -> keys and the splits' merge.
+// positions 105 us (4.6 TB/s: about 380 instructions for a block of 16 keys; neither
+// their issue, at 59 % of the rate, nor DRAM, at 55 %, is full with four CTAs an SM,
+// so that a part is latency that 16 warps leave open); nine sequences of 4-7 drafts,
+// fp32 over up to 6000 Q8_0 positions 56 us (840 instructions a block, two terms of
+// everything, and each page converted by the two row tiles of its sequence); one
+// fp32 step of 32 heads over 1024 bf16 positions 11 us, most of it the chain
+// lengths -> page -> keys and the splits' merge; 32 fp32 tokens of one sequence over
+// 8160 positions 76 us (bf16) and 61 (Q8_0), in eight row tiles that each load and
+// convert all keys; head_dim 256, 512 bf16 tokens of 16 heads over 4 and 8192
+// positions 1045 us, in 256 row tiles of 8 rows a head.
 #include <algorithm>
 #include <cstdio>
 
@@ -154,8 +159,8 @@ struct PaCfg {
   static constexpr int kRowBytes = Q8 ? HD : HD * 2;
   // rows 16 bytes apart (mod 128) in shared memory: what ldmatrix wants of the 8
   // rows of a matrix.  The Q8_0 loads take 32 bytes of 4 rows, which 32 bytes
-  // apart would not collide in any bank, but were slower (48 steps below: 112 us,
-  // 105 so).
+  // apart would not collide in any bank, but were slower (the 48 steps above: 112
+  // us, 105 so).
   static constexpr int kStride = kRowBytes + 16;
   static constexpr int kScale = Q8 ? HD / 16 : 0;           // scale bytes of a row
   static constexpr int kTile = 16 * (kStride + kScale);     // 16 keys, or values
@@ -165,8 +170,8 @@ struct PaCfg {
   static constexpr int kHead = kQBytes + kInit;
   static constexpr int kMerge = kWarps * kRows * (HD + 4) * 4;    // partial O of the warps
   // shared memory for four CTAs per SM over Q8_0, whose warps compute, three
-  // over bf16 (32 sequences of 4000: 94 us with two, 90 with three), where that
-  // leaves two stages
+  // over bf16 (40 steps over 500-8000: 146 us with two, 135 with three; drafts 46
+  // and 40), where that leaves two stages
   static constexpr int stages() {
     int s = ((Q8 ? 56 : 74) * 1024 - kHead) / (kStage * kWarps);
     return s < 2 ? 2 : s > 6 ? 6 : s;
@@ -861,7 +866,8 @@ __global__ void __launch_bounds__(kPaThreads, (PaCfg<HD, Q8, F32, NN>::kMinCtas)
 // Column tiles of a warp (NN: 1, 2 or 4): the fewest that hold the rows of the
 // longest chunk, since a sequence's keys are read and converted once per row
 // tile; but O's HD * NN / 4 registers leave room for other warps (drafts over
-// Q8_0 in fp32, 16-28 rows of 128: 88 us with NN 4, 72 us with two tiles of NN 2).
+// Q8_0 in fp32, 16-28 rows of 128: 62 us with one tile of NN 4, 56 with two of NN
+// 2, 58 with NN 1; bf16 over bf16 pages 42, 40 and 57).
 static int pick_nn(int max_q, int group, int hd) {
   const int64_t rows = (int64_t)max_q * group;
   const int most = hd <= 64 ? 4 : hd <= 128 ? 2 : 1;
@@ -935,10 +941,10 @@ static cudaError_t launch_t(PagedAttnArgs a, const PaPlan& p, cudaStream_t st) {
   }
   const int64_t slots = (int64_t)ctas * device_sm_count();
   // A few units (one sequence) are all alike: two CTAs an SM, more only add to
-  // the merge (16384 Q8_0 positions, 8 heads: 26.1 us with one, 21.1 with two,
-  // 22.3 with three).  Others have different lengths, which two waves of smaller
-  // pieces may even out (48 sequences of 900-8000 positions: 132 us with one
-  // wave, 115 with two; drafts of nine: 59 and 66): the kernel chooses.
+  // the merge (16384 Q8_0 positions, 8 heads: 24.8 us with one, 19.8 with two,
+  // 20.0 with three).  Others have different lengths, which two waves of smaller
+  // pieces may even out (48 sequences of 900-8000 positions: 117 us with one
+  // wave, 105 with two; drafts of nine: 56 and 64): the kernel chooses.
   const bool few = p.units * 8 <= slots;
   a.want = (float)(few ? 2LL * device_sm_count() : slots) / (float)a.c.kv_heads;
   a.waves = few ? 1 : 2;

@@ -32,12 +32,12 @@
 // 32 would do) and about as many of softmax per tile (64 exponentials a row, a
 // quarter of them on the FMA pipe, and the loads and stores of tensor memory);
 // with the barriers between the two it takes 1660.  Steps of 128 keys would feed
-// the MMAs better, but leave no second buffer of scores (the four prompts below:
-// 309 us).  Four softmax warpgroups, turns between the tiles and P formed before
-// the maximum is known were no faster.  32 query heads over 8, bf16: four
+// the MMAs better, but leave no second buffer of scores.  Four softmax
+// warpgroups, turns between the tiles and P formed before the maximum is known
+// were no faster.  32 query heads over 8, bf16: four
 // prompts of 700-4000 tokens 257 us (805 TFLOP/s of unmasked products); 512
-// tokens over 16384 cached 164 us, over Q8_0 209 us, whose tiles are converted
-// once per 256 rows; 8192 tokens, 32 heads 519 us (1060 TFLOP/s).
+// tokens over 16384 cached 163 us, over Q8_0 210 us, whose tiles are converted
+// once per 256 rows; 8192 tokens, 32 heads 521-534 us (1040 TFLOP/s).
 //
 // Q8_0: operands are fp16, q is scaled per row by a power of two and P by 2^6,
 // as in paged_attn.cu.
@@ -439,8 +439,8 @@ __global__ void __launch_bounds__(TcCfg<HDP, Q8>::kThreads, 1)
       const uint64_t sc2 = pair2(slope, slope), ref2 = pair2(-ref, -ref);
       float l0 = 0.f, l1 = 0.f;
       // P.  A quarter of the exponentials go to the FMA pipe over bf16 pages (four
-      // prompts 265 -> 257 us); over Q8_0, whose converters use that pipe, none
-      // (512 tokens over 16384: 209 us, 236 with a quarter).
+      // prompts 268 -> 257 us); over Q8_0, whose converters use that pipe, none
+      // (512 tokens over 16384: 210 us, 228 with a quarter).
       auto form = [&](auto poly) {
 #pragma unroll
         for (int c = 0; c < kTcStep / 32; ++c) {

@@ -19,9 +19,8 @@
 // block's maximum goes through shuffles.
 //
 // Measured: 8.4k prompt tokens (bf16, 32 query and 8 key/value heads of 128) to
-// Q8_0 and back as fp32 57 us (5.0 TB/s); 20011 rows of 8 heads read from Q8_0
-// as bf16 23 us (5.4 TB/s; 31 us when a thread's 32 bytes were its own); one
-// token of 32 heads written and read 4.8 us.
+// Q8_0 and back as fp32 56 us (5.1 TB/s); 20011 rows of 8 heads read from Q8_0
+// as bf16 23 us (5.4 TB/s); one token of 32 heads written and read 4.8 us.
 #include <algorithm>
 #include <cstdio>
 
@@ -375,8 +374,8 @@ static int kv_unroll(int n, int rows, int lanes, int most) {
   return (int64_t)n * rows * lanes > 2048LL * device_sm_count() ? most : 1;
 }
 // A block's span: up to 16 steps and kKvTokens tokens, as many as make whole
-// waves of blocks (8.4k prompt tokens to Q8_0 and back with 16 steps each, 2.2
-// and 1.8 waves: 73 us; whole waves of 12 and 15: 66).
+// waves of blocks (20000 prompt tokens to Q8_0 and back: 140 us with 16 steps
+// each, 128 in whole waves; 13500: 114 and 89).
 static KvWalk kv_walk(int n, int rows, int per_step, int unroll, int ctas) {
   KvWalk w;
   w.n = n;
@@ -410,7 +409,7 @@ static cudaError_t launch_walk(Kernel kernel, const KvWalk& w, cudaStream_t st, 
 template <typename T, int HD, bool Q8>
 static cudaError_t append_t(const PagedView& c, const draco_kv_append_args& a, cudaStream_t st) {
   using S = KvShape<HD>;
-  constexpr int kMost = sizeof(T) == 4 ? 2 : 4;  // 32 registers of loads in flight (bf16, 8.4k tokens: two rows 73 us, four 66)
+  constexpr int kMost = sizeof(T) == 4 ? 2 : 4;  // 32 registers of loads in flight (bf16, 8.4k tokens to Q8_0 and back: one row 65 us, two 64, four 56)
   const int rows = a.heads + 2 * c.kv_heads, u = kv_unroll(a.n, rows, S::kLanes, kMost);
   const KvWalk w = kv_walk(a.n, rows, S::kRows, u,
                            u == 1 ? kv_ctas<kv_append_kernel<T, HD, Q8, 1>>() : kv_ctas<kv_append_kernel<T, HD, Q8, kMost>>());
@@ -423,7 +422,7 @@ template <typename T, int HD, bool Q8>
 static cudaError_t read_t(const PagedView& c, const int* seq, const int* pos, int n, void* k_out, void* v_out,
                           int64_t ldk, int64_t ldv, cudaStream_t st) {
   using S = KvShape<HD>;
-  constexpr int kMost = 2;  // (four: as fast, with half the warps)
+  constexpr int kMost = 2;  // (20011 rows of Q8_0: one 23.9 us, two 23.0, four 23.0 with half the warps)
   const int rows = 2 * c.kv_heads, u = kv_unroll(n, rows, S::kLanes, kMost);
   const KvWalk w = kv_walk(n, rows, S::kRows, u,
                            u == 1 ? kv_ctas<kv_read_kernel<T, HD, Q8, 1>>() : kv_ctas<kv_read_kernel<T, HD, Q8, kMost>>());

@@ -18,11 +18,13 @@
 // since an index out of 10^5 hangs on differences of one in 10^5 or less.
 //
 // Measured: 48 sequences of 2-8 rows of 128000 fp32 logits with the drafter's
-// probabilities 72 us (2.1 TB/s); for a sequence of five rows 15 us of it read
+// probabilities 73 us (2.1 TB/s); for a sequence of five rows 15 us of it read
 // the logits, 17 are the two passes of fp64 weights over the row drawn from (the
 // sum of p, then of max(p - q, 0)), 5 find the token, 13 go to barriers and
-// decisions; longer sequences take the rest.  One sequence of five rows of 32000
-// 11.6 us.
+// decisions.  The rest is imbalance: a sequence's rows are all read by its own 8
+// CTAs, eight rows as well as two, and the longest sequences end last.  bf16 logits
+// 62 us; greedy 37; 48 sequences of one row 27.  One sequence of five rows of 32000
+// 11.6 us, greedy 5.7; of one row of 128000 13.
 #include <cooperative_groups.h>
 
 #include <cstdio>

@@ -253,7 +253,9 @@ def kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Ten
             pos: torch.Tensor, head_dim: int, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
     """The keys and values at position pos[i] of sequence seq[i] (int32 [n]), as
     [n, kv_heads, head_dim] float32 (exact) or bfloat16 (rounded once); rows
-    outside the cache are zeros."""
+    outside the cache are zeros.  For a host that moves a sequence to another
+    cache type, device or process, or keeps a prefix outside the pages; attention
+    reads the pages themselves."""
     c, kv_heads, _, _ = _cache_struct(k_cache, v_cache, block_table, head_dim)
     dev, n = k_cache.get_device(), seq.shape[0] if seq.dim() else 0
     if dtype not in _DTYPES:
